@@ -521,6 +521,113 @@ typedef struct lm_head_args {
 
 LM_API int lm_head(const lm_head_args* args);
 
+/*
+ * The microscaled 4-bit weight format (NVFP4) and its conversions. A matrix [rows, cols], cols a multiple of 16, is held as codes [rows, cols / 2]
+ * (two to a byte, the even column in the low nibble), e4m3 scales [rows, cols / 16] and one float32 `scale`: value = e2m1(code) * e4m3(scale) * scale: the
+ * layout checkpoints of this format have (the reference's weight formats, monolith/formats).
+ *
+ * lm_quantize_nvfp4: block scale = e4m3(a / (6 * scale)) with a the block's largest magnitude, code = e2m1(x / (block scale * scale)); both quotients are the real
+ *   ones, rounded once to nearest, ties to even, saturating at 448 and 6 (so the codes do not depend on the arithmetic); the sign bit of a code is that of x; a block scale of
+ *   0 has magnitudes of 0. find_scale: scale = (largest finite magnitude) / 2688 is formed and written, or 1 where that is no normal number; otherwise it is read
+ *   (one that is not a positive normal number gives blocks of NaN). A block that holds a NaN or an infinity gets the scale NaN: what is computed from it is NaN.
+ *   BF16 or FP32 input.
+ * lm_dequantize_nvfp4: the float32 values, fl32(e2m1 * e4m3 * scale).
+ */
+typedef struct lm_quantize_nvfp4_args {
+  uint32_t struct_size;
+  int32_t dtype;               /* LM_DTYPE_*: type of x */
+  const void* x;               /* [rows, row_stride] */
+  int64_t rows, cols, row_stride;
+  float* scale;                /* [1]: read, or (find_scale) written */
+  int32_t find_scale;
+  int32_t pad_;
+  void* amax;                  /* 4 bytes of scratch, find_scale only */
+  uint8_t* codes; int64_t codes_stride;    /* out [rows, codes_stride] bytes, >= cols / 2 */
+  uint8_t* scales; int64_t scales_stride;  /* out [rows, scales_stride] bytes, >= cols / 16 */
+  void* stream;
+} lm_quantize_nvfp4_args;
+
+typedef struct lm_dequantize_nvfp4_args {
+  uint32_t struct_size;
+  int32_t pad_;
+  const uint8_t* codes; int64_t codes_stride;
+  const uint8_t* scales; int64_t scales_stride;
+  const float* scale;
+  int64_t rows, cols;
+  float* out; int64_t out_stride;          /* [rows, out_stride] */
+  void* stream;
+} lm_dequantize_nvfp4_args;
+
+LM_API int lm_quantize_nvfp4(const lm_quantize_nvfp4_args* args);
+LM_API int lm_dequantize_nvfp4(const lm_dequantize_nvfp4_args* args);
+
+/*
+ * lm_head with a weight in that format: logits[r, v] = bf16(scale * sum_k x[r, k] * e2m1(codes[v, k]) * e4m3(scales[v, k / 16])), FP32 accumulation of the exact products, x as for
+ * lm_head (BF16 rows, or the fused RMSNorm's BF16 output). 1 .. LM_HEAD_NVFP4_MAX_ROWS rows. hidden_dim a multiple of 64, at most 12,736; codes
+ * and their stride 16-byte aligned, scales and theirs 4-byte aligned. A logit does not depend on where its row of the weight lies (a shard of the weight gives the bits
+ * of the whole). Stands in for the reference's NVFP4 matrix-vector kernel on the `lm_head` op (kernels/common/gemv_nvfp4_rows.metal, monolith/nn/lm_head.py:50-60).
+ * workspace: lm_head_nvfp4_workspace_bytes(rows, hidden_dim) bytes, 256-byte aligned, any contents (0 bytes: NULL); calls that can overlap need one each.
+ */
+#define LM_HEAD_NVFP4_MAX_ROWS 65536
+typedef struct lm_head_nvfp4_args {
+  uint32_t struct_size;
+  int32_t one_plus;            /* the norm's scale is 1 + norm_weight */
+  int64_t rows;
+  const void* hidden;          /* [rows, hidden_stride] BF16 */
+  int64_t hidden_stride;
+  const uint8_t* codes; int64_t codes_stride;    /* [vocab, codes_stride] bytes */
+  const uint8_t* scales; int64_t scales_stride;  /* [vocab, scales_stride] bytes */
+  const float* scale;          /* [1] */
+  int64_t hidden_dim, vocab;
+  const void* norm_weight;     /* [hidden_dim] BF16 or NULL */
+  float eps;
+  int32_t pad_;
+  void* logits;                /* out [rows, logits_stride] BF16 */
+  int64_t logits_stride;
+  void* workspace; size_t workspace_bytes;
+  void* stream;
+} lm_head_nvfp4_args;
+
+LM_API int lm_head_nvfp4(const lm_head_nvfp4_args* args);
+LM_API size_t lm_head_nvfp4_workspace_bytes(int64_t rows, int64_t hidden_dim);
+
+/*
+ * The logits' processing in front of the sampler: penalties for repeated tokens by request, biases by token, grammar masks. No counterpart in lithos-metal.
+ * Per row r, with c_all(v) the occurrences of v in history[r, 0 .. len_r) and c_out(v) those from position prompt_len[r] on (ids outside [0, vocab) are ignored), in binary32:
+ *   z = logits[r, v];  c_all(v) > 0: z = z > 0 ? z / repetition : z * repetition;  c_out(v) > 0: z = (z - presence) - frequency * c_out(v);
+ *   every entry of the row's bias list with id v, in list order: z = z + value;  bit v of the row's mask clear: z = -inf;
+ * rounded once to the logits' type. Logits that none of this names are copied, or in place (out == logits, same stride) left as they are. With frequency 0 and no prompt the penalties are
+ * those of lm_sample. A row whose mask allows nothing is all -inf (lm_argmax then gives token 0; a draw from it is unspecified).
+ * Strides of history and bias lists may be 0 (one list for every row); history_len makes one buffer serve the rows of a speculative round. out overlaps logits
+ * entirely (in place) or not at all. No workspace.
+ */
+typedef struct lm_logits_args {
+  uint32_t struct_size;
+  int32_t dtype;               /* LM_DTYPE_* */
+  const void* logits;          /* [rows, row_stride] */
+  int64_t rows, vocab, row_stride;
+  void* out;                   /* [rows, out_stride] same type */
+  int64_t out_stride;
+  const int32_t* history;      /* [rows, hist_stride] token ids, or NULL; at most 65,536 a row */
+  int64_t hist_len, hist_stride;
+  const int32_t* history_len;  /* [rows] how many of them count (limited to 0 .. hist_len), or NULL: hist_len */
+  const int32_t* prompt_len;   /* [rows] how many of those are the prompt's (repetition penalty only), or NULL: 0 */
+  /* knobs: a device array with one entry per row, or NULL to use the scalar */
+  const float* repetition; float repetition_s;   /* > 0; 1 = off */
+  const float* presence;   float presence_s;
+  const float* frequency;  float frequency_s;
+  const int32_t* bias_ids; int64_t bias_ids_stride;       /* [rows, bias_ids_stride] token ids; those outside [0, vocab) are skipped */
+  const float* bias_values; int64_t bias_values_stride;   /* [rows, bias_values_stride] */
+  int64_t bias_len;            /* entries per row, at most 8191; 0 = none */
+  const uint32_t* mask;        /* [mask_count, mask_stride] words: bit v & 31 of word v >> 5 set = token v allowed; or NULL */
+  int64_t mask_stride;         /* in words, >= ceil(vocab / 32) */
+  int64_t mask_count;
+  const int32_t* mask_rows;    /* [rows] which mask a row has: negative = none, mask_count or more = everything masked; or NULL: mask r for row r */
+  void* stream;
+} lm_logits_args;
+
+LM_API int lm_process_logits(const lm_logits_args* args);
+
 LM_API int lm_abi_version(void);
 LM_API const char* lm_error_string(int code);
 LM_API const char* lm_last_cuda_error(void);   /* text of the last CUDA error seen by this thread's calls, "" if none */

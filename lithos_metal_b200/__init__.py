@@ -10,8 +10,10 @@ from .step_state import StepStateLayout, accept_scan, advance, confidence, verif
 from .records import accept_args_from_record, sample_args_from_record, select_args_from_record
 from .tiles import TileSampler
 from .head import lm_head
+from .logits import process_logits
+from .nvfp4 import Nvfp4Weight, quantize_nvfp4
 from . import parallel
 
-__all__ = ["TileSampler", "lm_head", "GreedySampler", "StochasticSampler", "SamplingParams", "SampleOutput", "sample", "argmax", "sample_row", "thresholds",
+__all__ = ["TileSampler", "lm_head", "Nvfp4Weight", "quantize_nvfp4", "process_logits", "GreedySampler", "StochasticSampler", "SamplingParams", "SampleOutput", "sample", "argmax", "sample_row", "thresholds",
            "warped_probabilities", "verify", "draft_q", "DraftQ", "StepStateLayout", "accept_scan", "verify_select", "advance", "confidence", "parallel",
            "sample_args_from_record", "select_args_from_record", "accept_args_from_record"]

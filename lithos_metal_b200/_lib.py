@@ -120,7 +120,42 @@ class HeadArgs(C.Structure):
     ]
 
 
-EXPORTS = ["lm_head", "lm_accept_scan", "lm_verify_select", "lm_advance", "lm_step_state_bytes", "lm_sample", "lm_argmax", "lm_argmax_i64", "lm_argmax_static", "lm_vocab_local", "lm_vocab_merge", "lm_vocab_record_bytes", "lm_vocab_candidate_cap", "lm_vocab_pieces", "lm_verify", "lm_draft_q", "lm_confidence", "lm_tile_state_bytes", "lm_tile_begin", "lm_tile_consume", "lm_tile_finish", "lm_workspace_bytes", "lm_verify_workspace_bytes", "lm_uniform01", "lm_abi_version",
+class QuantizeNvfp4Args(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("x", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("row_stride", C.c_int64),
+        ("scale", C.c_void_p), ("find_scale", C.c_int32), ("pad_", C.c_int32), ("amax", C.c_void_p), ("codes", C.c_void_p), ("codes_stride", C.c_int64),
+        ("scales", C.c_void_p), ("scales_stride", C.c_int64), ("stream", C.c_void_p),
+    ]
+
+
+class DequantizeNvfp4Args(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("pad_", C.c_int32), ("codes", C.c_void_p), ("codes_stride", C.c_int64), ("scales", C.c_void_p), ("scales_stride", C.c_int64),
+        ("scale", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64), ("stream", C.c_void_p),
+    ]
+
+
+class HeadNvfp4Args(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("one_plus", C.c_int32), ("rows", C.c_int64), ("hidden", C.c_void_p), ("hidden_stride", C.c_int64), ("codes", C.c_void_p),
+        ("codes_stride", C.c_int64), ("scales", C.c_void_p), ("scales_stride", C.c_int64), ("scale", C.c_void_p), ("hidden_dim", C.c_int64), ("vocab", C.c_int64),
+        ("norm_weight", C.c_void_p), ("eps", C.c_float), ("pad_", C.c_int32), ("logits", C.c_void_p), ("logits_stride", C.c_int64), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p),
+    ]
+
+
+class LogitsArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("logits", C.c_void_p), ("rows", C.c_int64), ("vocab", C.c_int64), ("row_stride", C.c_int64),
+        ("out", C.c_void_p), ("out_stride", C.c_int64), ("history", C.c_void_p), ("hist_len", C.c_int64), ("hist_stride", C.c_int64), ("history_len", C.c_void_p),
+        ("prompt_len", C.c_void_p), ("repetition", C.c_void_p), ("repetition_s", C.c_float), ("presence", C.c_void_p), ("presence_s", C.c_float),
+        ("frequency", C.c_void_p), ("frequency_s", C.c_float), ("bias_ids", C.c_void_p), ("bias_ids_stride", C.c_int64), ("bias_values", C.c_void_p),
+        ("bias_values_stride", C.c_int64), ("bias_len", C.c_int64), ("mask", C.c_void_p), ("mask_stride", C.c_int64), ("mask_count", C.c_int64),
+        ("mask_rows", C.c_void_p), ("stream", C.c_void_p),
+    ]
+
+
+EXPORTS = ["lm_quantize_nvfp4", "lm_dequantize_nvfp4", "lm_head_nvfp4", "lm_head_nvfp4_workspace_bytes", "lm_process_logits", "lm_head", "lm_accept_scan", "lm_verify_select", "lm_advance", "lm_step_state_bytes", "lm_sample", "lm_argmax", "lm_argmax_i64", "lm_argmax_static", "lm_vocab_local", "lm_vocab_merge", "lm_vocab_record_bytes", "lm_vocab_candidate_cap", "lm_vocab_pieces", "lm_verify", "lm_draft_q", "lm_confidence", "lm_tile_state_bytes", "lm_tile_begin", "lm_tile_consume", "lm_tile_finish", "lm_workspace_bytes", "lm_verify_workspace_bytes", "lm_uniform01", "lm_abi_version",
            "lm_error_string", "lm_last_cuda_error", "lm_device_sm_count"]
 
 _lib = None
@@ -171,6 +206,10 @@ def lib():
         L.lm_head.argtypes = [C.POINTER(HeadArgs)]
         L.lm_vocab_pieces.restype = C.c_int32
         L.lm_vocab_pieces.argtypes = [C.c_int32, C.c_int32, C.c_int64, C.c_int64]
+        for fn, args in ((L.lm_quantize_nvfp4, QuantizeNvfp4Args), (L.lm_dequantize_nvfp4, DequantizeNvfp4Args), (L.lm_head_nvfp4, HeadNvfp4Args), (L.lm_process_logits, LogitsArgs)):
+            fn.restype, fn.argtypes = C.c_int, [C.POINTER(args)]
+        L.lm_head_nvfp4_workspace_bytes.restype = C.c_size_t
+        L.lm_head_nvfp4_workspace_bytes.argtypes = [C.c_int64, C.c_int64]
         for fn in (L.lm_accept_scan, L.lm_verify_select, L.lm_advance):
             fn.restype, fn.argtypes = C.c_int, [C.POINTER(StepArgs)]
         L.lm_step_state_bytes.restype = C.c_size_t
@@ -198,7 +237,7 @@ class _NoHost:
     def _leave(self, *args):
         return None
 
-    sample = stochastic = argmax = draft_q = verify = lm_head = _leave
+    sample = stochastic = argmax = draft_q = verify = lm_head = lm_head_nvfp4 = process_logits = _leave
 
 
 def host():
@@ -213,7 +252,7 @@ def host():
             m = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(m)
             sampler, verify = (importlib.import_module(f"{__package__}.{n}") for n in ("sampler", "verify"))
-            names = ("lm_sample", "lm_argmax", "lm_argmax_i64", "lm_verify", "lm_draft_q", "lm_head", "lm_workspace_bytes", "lm_verify_workspace_bytes")
+            names = ("lm_sample", "lm_argmax", "lm_argmax_i64", "lm_verify", "lm_draft_q", "lm_head", "lm_head_nvfp4", "lm_head_nvfp4_workspace_bytes", "lm_process_logits", "lm_workspace_bytes", "lm_verify_workspace_bytes")
             m.init({n: C.cast(getattr(L, n), C.c_void_p).value for n in names}, sampler.SamplingParams, sampler.SampleOutput, verify.DraftQ, check, sampler._workspace)
         except (ImportError, OSError, RuntimeError) as e:
             warnings.warn(f"lithos_metal_b200: no native call path ({e}); calls go through ctypes", RuntimeWarning, stacklevel=3)

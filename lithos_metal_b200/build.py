@@ -22,7 +22,7 @@ OUT = os.path.join(HERE, "_lib", "liblithos_b200.so")
 # the native call path of the Python layer: named for what it was compiled against, so that another Python or torch never loads it
 HOST_OUT = os.path.join(HERE, "_lib", f"lithos_host.{sys.implementation.cache_tag}-torch{metadata.version('torch')}.so")
 HOST_SOURCE = "host_ext.cpp"
-SOURCES = ["lithos_b200.cu", "cluster.cu"]
+SOURCES = ["lithos_b200.cu", "cluster.cu", "tail_ops.cu"]
 # (No -split-compile: with it ptxas made one of two different kernels from the same cluster.cu, as its threads happened to finish, and the one --
 # five builds in eight -- was up to 17 % slower: 32 FP32 rows of 151,936 without a filter 28.8 us instead of 24.8.)
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden",

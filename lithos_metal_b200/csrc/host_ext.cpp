@@ -31,6 +31,9 @@ struct Abi {
   decltype(&lm_verify) verify = nullptr;
   decltype(&lm_draft_q) draft_q = nullptr;
   decltype(&lm_head) head = nullptr;
+  decltype(&lm_head_nvfp4) head_nvfp4 = nullptr;
+  decltype(&lm_head_nvfp4_workspace_bytes) head_nvfp4_workspace_bytes = nullptr;
+  decltype(&lm_process_logits) process_logits = nullptr;
   decltype(&lm_workspace_bytes) workspace_bytes = nullptr;
   decltype(&lm_verify_workspace_bytes) verify_workspace_bytes = nullptr;
 } abi;
@@ -417,6 +420,104 @@ PyObject* py_lm_head(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// lm_head_nvfp4(hidden, codes, scales, scale, norm_weight, eps, one_plus, out) -> logits; the weight's tensors were checked when its Nvfp4Weight was made
+PyObject* py_lm_head_nvfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) { PyErr_SetString(PyExc_TypeError, "lm_head_nvfp4: 8 arguments"); return nullptr; }
+  const at::Tensor *x = as_tensor(args[0]), *c = as_tensor(args[1]), *s = as_tensor(args[2]), *g = as_tensor(args[3]), *nw = args[4] == Py_None ? nullptr : as_tensor(args[4]);
+  if (!x || !c || !s || !g || (args[4] != Py_None && !nw)) return none();
+  const at::Device dev = c->device();
+  const int64_t V = c->size(0), H = c->size(1) * 2;
+  if (x->device() != dev || x->dim() != 2 || x->scalar_type() != at::kBFloat16 || x->size(1) != H || x->stride(1) != 1 || (x->size(0) > 1 && x->stride(0) < H)) return none();
+  const int64_t rows = x->size(0);
+  if (nw && (nw->dim() != 1 || !plain_vector(*nw, at::kBFloat16, dev, H))) return none();
+  if (!PyFloat_Check(args[5]) || !PyBool_Check(args[6])) return none();
+  at::Tensor out;
+  if (args[7] == Py_None) out = make({rows, V}, at::kBFloat16, dev);
+  else {
+    const at::Tensor* t = as_tensor(args[7]);
+    if (!t || t->device() != dev || t->dim() != 2 || t->size(0) != rows || t->size(1) != V || t->scalar_type() != at::kBFloat16 || t->stride(1) != 1 || (rows > 1 && t->stride(0) < V)) return none();
+    out = *t;
+  }
+  lm_head_nvfp4_args a{};
+  a.struct_size = sizeof(a);
+  a.rows = rows; a.hidden = ptr(*x); a.hidden_stride = row_stride(*x);
+  a.codes = static_cast<const uint8_t*>(c->const_data_ptr()); a.codes_stride = row_stride(*c); a.scales = static_cast<const uint8_t*>(s->const_data_ptr()); a.scales_stride = row_stride(*s);
+  a.scale = static_cast<const float*>(g->const_data_ptr()); a.hidden_dim = H; a.vocab = V;
+  a.norm_weight = nw ? ptr(*nw) : nullptr;
+  a.eps = static_cast<float>(PyFloat_AS_DOUBLE(args[5])); a.one_plus = args[6] == Py_True ? 1 : 0;
+  a.logits = ptr(out); a.logits_stride = row_stride(out);
+  const int64_t bytes = static_cast<int64_t>(abi.head_nvfp4_workspace_bytes(rows, H));
+  at::Tensor ws;                                                            // (of the call: calls that overlap never share one)
+  if (bytes) { ws = make({bytes}, at::kByte, dev); a.workspace = ptr(ws); a.workspace_bytes = static_cast<size_t>(bytes); }
+  a.stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const int rc = call(dev, nullptr, [&] { return abi.head_nvfp4(&a); });
+  if (rc != LM_OK) return failed(rc, "lm_head_nvfp4");
+  if (args[7] != Py_None) { Py_INCREF(args[7]); return args[7]; }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// process_logits(logits, history, history_len, prompt_len, repetition, presence, frequency, bias_ids, bias_values, mask, mask_rows, out) -> out
+PyObject* py_process_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 12) { PyErr_SetString(PyExc_TypeError, "process_logits: 12 arguments"); return nullptr; }
+  const at::Tensor* x = as_tensor(args[0]);
+  if (!x || !plain_rows(*x) || (x->size(0) > 1 && x->stride(0) < x->size(1))) return none();
+  const at::Device dev = x->device();
+  const int64_t rows = x->size(0), vocab = x->size(1);
+  lm_logits_args a{};
+  // a list per row, or one for all: [rows, n] with unit stride along a row
+  auto list = [&](PyObject* o, at::ScalarType type, const void** p, int64_t* len, int64_t* stride) {
+    const at::Tensor* t = as_tensor(o);
+    if (!t || t->device() != dev || t->dim() != 2 || t->size(0) != rows || t->scalar_type() != type || t->stride(1) != 1) return false;
+    *p = t->const_data_ptr(); *len = t->size(1); *stride = t->stride(0);
+    return true;
+  };
+  auto vec = [&](PyObject* o, const int32_t** p) {
+    if (o == Py_None) return true;
+    const at::Tensor* t = as_tensor(o);
+    if (!t || !plain_vector(*t, at::kInt, dev, rows)) return false;
+    *p = static_cast<const int32_t*>(t->const_data_ptr());
+    return true;
+  };
+  if (args[1] != Py_None) {
+    const void* p = nullptr;
+    if (!list(args[1], at::kInt, &p, &a.hist_len, &a.hist_stride) || !vec(args[2], &a.history_len) || !vec(args[3], &a.prompt_len)) return none();
+    a.history = static_cast<const int32_t*>(p);
+  }
+  if (!knob_f(args[4], rows, dev, &a.repetition, &a.repetition_s) || !knob_f(args[5], rows, dev, &a.presence, &a.presence_s) || !knob_f(args[6], rows, dev, &a.frequency, &a.frequency_s)) return none();
+  if (!a.repetition && !(a.repetition_s > 0.0f)) return none();
+  if (args[7] != Py_None || args[8] != Py_None) {
+    const void *p = nullptr, *q = nullptr;
+    int64_t len = 0;
+    if (!list(args[7], at::kInt, &p, &a.bias_len, &a.bias_ids_stride) || !list(args[8], at::kFloat, &q, &len, &a.bias_values_stride) || len != a.bias_len) return none();
+    a.bias_ids = static_cast<const int32_t*>(p); a.bias_values = static_cast<const float*>(q);
+  }
+  if (args[9] != Py_None) {
+    const at::Tensor* t = as_tensor(args[9]);
+    if (!t || t->device() != dev || t->dim() != 2 || t->scalar_type() != at::kInt || t->stride(1) != 1 || (t->size(0) > 1 && t->stride(0) < t->size(1)) || t->size(1) < (vocab + 31) / 32) return none();
+    if (!vec(args[10], &a.mask_rows) || (!a.mask_rows && t->size(0) != rows)) return none();
+    a.mask = static_cast<const uint32_t*>(t->const_data_ptr()); a.mask_stride = row_stride(*t); a.mask_count = t->size(0);
+  } else if (args[10] != Py_None) return none();
+  at::Tensor out;
+  if (args[11] == Py_None) out = make({rows, vocab}, x->scalar_type(), dev);
+  else {
+    const at::Tensor* t = as_tensor(args[11]);
+    if (!t || t->device() != dev || t->dim() != 2 || t->size(0) != rows || t->size(1) != vocab || t->scalar_type() != x->scalar_type() || t->stride(1) != 1 || (rows > 1 && t->stride(0) < vocab)) return none();
+    out = *t;
+  }
+  a.struct_size = sizeof(a);
+  a.dtype = dtype_code(*x); a.logits = ptr(*x); a.rows = rows; a.vocab = vocab; a.row_stride = row_stride(*x);
+  a.out = ptr(out); a.out_stride = row_stride(out);
+  a.stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const int rc = call(dev, nullptr, [&] { return abi.process_logits(&a); });
+  if (rc != LM_OK) return failed(rc, "lm_process_logits");
+  if (args[11] != Py_None) { Py_INCREF(args[11]); return args[11]; }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // init(addresses: dict of ABI function addresses, SamplingParams, SampleOutput, DraftQ, check, workspace)
 PyObject* py_init(PyObject*, PyObject* args) {
   PyObject *addresses, *t0, *t1, *t2, *f0, *f1;
@@ -428,10 +529,13 @@ PyObject* py_init(PyObject*, PyObject* args) {
   abi.verify = reinterpret_cast<decltype(abi.verify)>(get("lm_verify"));
   abi.draft_q = reinterpret_cast<decltype(abi.draft_q)>(get("lm_draft_q"));
   abi.head = reinterpret_cast<decltype(abi.head)>(get("lm_head"));
+  abi.head_nvfp4 = reinterpret_cast<decltype(abi.head_nvfp4)>(get("lm_head_nvfp4"));
+  abi.head_nvfp4_workspace_bytes = reinterpret_cast<decltype(abi.head_nvfp4_workspace_bytes)>(get("lm_head_nvfp4_workspace_bytes"));
+  abi.process_logits = reinterpret_cast<decltype(abi.process_logits)>(get("lm_process_logits"));
   abi.workspace_bytes = reinterpret_cast<decltype(abi.workspace_bytes)>(get("lm_workspace_bytes"));
   abi.verify_workspace_bytes = reinterpret_cast<decltype(abi.verify_workspace_bytes)>(get("lm_verify_workspace_bytes"));
   if (PyErr_Occurred()) return nullptr;
-  if (!abi.sample || !abi.argmax || !abi.argmax_i64 || !abi.verify || !abi.draft_q || !abi.head || !abi.workspace_bytes || !abi.verify_workspace_bytes) {
+  if (!abi.sample || !abi.argmax || !abi.argmax_i64 || !abi.verify || !abi.draft_q || !abi.head || !abi.head_nvfp4 || !abi.head_nvfp4_workspace_bytes || !abi.process_logits || !abi.workspace_bytes || !abi.verify_workspace_bytes) {
     PyErr_SetString(PyExc_ValueError, "init: an address is missing");
     return nullptr;
   }
@@ -448,6 +552,8 @@ PyMethodDef methods[] = {
     {"draft_q", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_draft_q)), METH_FASTCALL, nullptr},
     {"verify", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_verify)), METH_FASTCALL, nullptr},
     {"lm_head", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_lm_head)), METH_FASTCALL, nullptr},
+    {"lm_head_nvfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_lm_head_nvfp4)), METH_FASTCALL, nullptr},
+    {"process_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_process_logits)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "lithos_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,174 @@
+// C ABI of the operators between the projection and the sampler: the microscaled 4-bit weight, the projection with it, and the logits' processing. As in
+// lithos_b200.cu: argument checks, launch geometry, kernel launches; no allocation, no synchronisation.
+#include <cuda_runtime.h>
+
+#include "common.cuh"
+#include "host.cuh"
+#include "lm_head_nvfp4.cuh"
+#include "logits.cuh"
+#include "nvfp4.cuh"
+
+using namespace lm;
+
+namespace {
+
+bool misaligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
+
+// The sizes of a matrix in the 4-bit format (nvfp4.cuh).
+int fp4_matrix_ok(int64_t rows, int64_t cols, const void* codes, int64_t codes_stride, const void* scales, int64_t scales_stride, const void* scale) {
+  if (!codes || !scales || !scale || codes_stride < cols / 2 || scales_stride < cols / kFp4Block) return LM_E_INVALID;
+  if (cols % kFp4Block != 0 || cols > 0x7FFFFFFF || rows > 0x7FFFFFFF) return LM_E_UNSUPPORTED;
+  return LM_OK;
+}
+
+// Blocks of a grid-stride kernel over `items` threads' work.
+unsigned stride_grid(long long items, int threads, int sms, int per_sm) {
+  const long long want = (items + threads - 1) / threads, most = static_cast<long long>(sms) * per_sm;
+  return static_cast<unsigned>(want < most ? want : most);
+}
+
+}  // namespace
+
+extern "C" {
+
+int lm_quantize_nvfp4(const lm_quantize_nvfp4_args* a) {
+  if (!a || a->struct_size != sizeof(lm_quantize_nvfp4_args)) return LM_E_INVALID;
+  if (a->rows < 0 || a->cols < 0 || (a->dtype != LM_DTYPE_BF16 && a->dtype != LM_DTYPE_F32)) return LM_E_INVALID;
+  if (a->rows == 0 || a->cols == 0) return LM_OK;
+  if (!a->x || a->row_stride < a->cols || (a->find_scale && !a->amax)) return LM_E_INVALID;
+  int rc = fp4_matrix_ok(a->rows, a->cols, a->codes, a->codes_stride, a->scales, a->scales_stride, a->scale);
+  if (rc != LM_OK) return rc;
+  int sms = 0;
+  rc = sm_count(&sms);
+  if (rc != LM_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  QuantDev P;
+  P.x = a->x; P.dtype = a->dtype; P.rows = a->rows; P.cols = static_cast<int>(a->cols); P.row_stride = a->row_stride;
+  P.scale = a->scale; P.amax = static_cast<uint32_t*>(a->amax); P.find = a->find_scale ? 1 : 0;
+  P.codes = a->codes; P.codes_stride = a->codes_stride; P.scales = a->scales; P.scales_stride = a->scales_stride;
+  const long long blocks = a->rows * (a->cols / kFp4Block);
+  const unsigned grid = stride_grid(blocks, kQuantThreads, sms, 16);
+  const bool f32 = a->dtype == LM_DTYPE_F32;
+  if (P.find) {
+    const cudaError_t e = cudaMemsetAsync(P.amax, 0, sizeof(uint32_t), st);
+    if (e != cudaSuccess) return cuda_fail(e);
+    rc = f32 ? launch_stream(false, nvfp4_amax_kernel<true>, dim3(grid), kQuantThreads, 0, 1, st, P)
+             : launch_stream(false, nvfp4_amax_kernel<false>, dim3(grid), kQuantThreads, 0, 1, st, P);
+    if (rc != LM_OK) return rc;
+  }
+  return f32 ? launch_stream(false, nvfp4_quantize_kernel<true>, dim3(grid), kQuantThreads, 0, 1, st, P)
+             : launch_stream(false, nvfp4_quantize_kernel<false>, dim3(grid), kQuantThreads, 0, 1, st, P);
+}
+
+int lm_dequantize_nvfp4(const lm_dequantize_nvfp4_args* a) {
+  if (!a || a->struct_size != sizeof(lm_dequantize_nvfp4_args)) return LM_E_INVALID;
+  if (a->rows < 0 || a->cols < 0) return LM_E_INVALID;
+  if (a->rows == 0 || a->cols == 0) return LM_OK;
+  if (!a->out || a->out_stride < a->cols) return LM_E_INVALID;
+  int rc = fp4_matrix_ok(a->rows, a->cols, a->codes, a->codes_stride, a->scales, a->scales_stride, a->scale);
+  if (rc != LM_OK) return rc;
+  int sms = 0;
+  rc = sm_count(&sms);
+  if (rc != LM_OK) return rc;
+  DequantDev P{a->codes, a->codes_stride, a->scales, a->scales_stride, a->scale, a->rows, static_cast<int>(a->cols), a->out, a->out_stride};
+  return launch_stream(false, nvfp4_dequantize_kernel, dim3(stride_grid(a->rows * (a->cols / 8), kQuantThreads, sms, 16)), kQuantThreads, 0, 1, static_cast<cudaStream_t>(a->stream), P);
+}
+
+size_t lm_head_nvfp4_workspace_bytes(int64_t rows, int64_t hidden_dim) {
+  (void)rows; (void)hidden_dim;
+  return 0;
+}
+
+int lm_head_nvfp4(const lm_head_nvfp4_args* a) {
+  if (!a || a->struct_size != sizeof(lm_head_nvfp4_args)) return LM_E_INVALID;
+  if (a->rows < 0 || a->vocab < 0 || a->hidden_dim < 1) return LM_E_INVALID;
+  if (a->rows == 0 || a->vocab == 0) return LM_OK;
+  if (!a->hidden || !a->logits || a->hidden_stride < a->hidden_dim || a->logits_stride < a->vocab) return LM_E_INVALID;
+  int rc = fp4_matrix_ok(a->vocab, a->hidden_dim, a->codes, a->codes_stride, a->scales, a->scales_stride, a->scale);
+  if (rc != LM_OK) return rc;
+  if (a->rows > LM_HEAD_NVFP4_MAX_ROWS || a->vocab > LM_MAX_VOCAB || (a->hidden_dim % 64) != 0 || a->hidden_dim > kH4MaxHidden) return LM_E_UNSUPPORTED;
+  if (misaligned(a->codes, 16) || (a->codes_stride % 16) != 0 || misaligned(a->scales, 4) || (a->scales_stride % 4) != 0) return LM_E_UNSUPPORTED;   // 16- and 4-byte loads
+  Head4Dev P;
+  P.x_stride = a->hidden_stride;
+  P.codes = a->codes; P.codes_stride = a->codes_stride; P.scales = a->scales; P.scales_stride = a->scales_stride; P.scale = a->scale;
+  P.hidden = static_cast<int>(a->hidden_dim); P.vocab = static_cast<int>(a->vocab);
+  P.gamma = static_cast<const uint16_t*>(a->norm_weight); P.eps = a->eps; P.one_plus = a->one_plus; P.logits_stride = a->logits_stride;
+  int sms = 0;
+  rc = sm_count(&sms);
+  if (rc != LM_OK) return rc;
+  const size_t smem = head4_smem_bytes(P.hidden);
+  rc = ensure_dynamic_smem(kSlotHeadNvfp4, reinterpret_cast<const void*>(lm_head_nvfp4_kernel), smem);
+  if (rc != LM_OK) return rc;
+  int per_sm = 1;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, lm_head_nvfp4_kernel, kH4Threads, smem) != cudaSuccess || per_sm < 1) per_sm = 1;
+  const long long tiles = (a->vocab + kH4Tile - 1) / kH4Tile, most = static_cast<long long>(per_sm) * sms;
+  const unsigned grid = static_cast<unsigned>(tiles < most ? tiles : most);
+  for (int64_t r = 0; r < a->rows; r += kH4Rows) {
+    P.x = static_cast<const uint16_t*>(a->hidden) + r * a->hidden_stride;
+    P.logits = static_cast<uint16_t*>(a->logits) + r * a->logits_stride;
+    P.rows = static_cast<int>(a->rows - r < kH4Rows ? a->rows - r : kH4Rows);
+    rc = launch_beside(lm_head_nvfp4_kernel, dim3(grid), kH4Threads, smem, 1, static_cast<cudaStream_t>(a->stream), P);
+    if (rc != LM_OK) return rc;
+  }
+  return LM_OK;
+}
+
+// Whether writing `out` can change what is read of `in` (both [rows, vocab] in elements of `size` bytes): same place and strides is in place, sharing nothing is fine.
+static int logits_overlap(const lm_logits_args* a, int64_t size, bool* same) {
+  const uintptr_t in = reinterpret_cast<uintptr_t>(a->logits), out = reinterpret_cast<uintptr_t>(a->out);
+  *same = in == out && (a->rows == 1 || a->row_stride == a->out_stride);
+  if (*same) return LM_OK;
+  const uintptr_t row = static_cast<uintptr_t>(a->vocab * size);
+  const uintptr_t in_end = in + static_cast<uintptr_t>((a->rows - 1) * a->row_stride * size) + row, out_end = out + static_cast<uintptr_t>((a->rows - 1) * a->out_stride * size) + row;
+  if (in_end <= out || out_end <= in) return LM_OK;
+  if (a->row_stride != a->out_stride) return LM_E_INVALID;
+  const uintptr_t stride = static_cast<uintptr_t>(a->row_stride * size), gap = (out > in ? out - in : in - out) % stride;    // columns of one wider matrix
+  return gap >= row && stride - gap >= row ? LM_OK : LM_E_INVALID;
+}
+
+int lm_process_logits(const lm_logits_args* a) {
+  if (!a || a->struct_size != sizeof(lm_logits_args)) return LM_E_INVALID;
+  if (a->rows < 0 || a->vocab < 0 || (a->dtype != LM_DTYPE_BF16 && a->dtype != LM_DTYPE_F32)) return LM_E_INVALID;
+  if (a->rows == 0 || a->vocab == 0) return LM_OK;
+  if (!a->logits || !a->out || a->row_stride < a->vocab || a->out_stride < a->vocab) return LM_E_INVALID;
+  if (a->history && (a->hist_len < 0 || a->hist_stride < 0)) return LM_E_INVALID;
+  if (a->history && a->repetition == nullptr && !(a->repetition_s > 0.0f)) return LM_E_INVALID;
+  if (a->bias_len < 0 || (a->bias_len > 0 && (!a->bias_ids || !a->bias_values || a->bias_ids_stride < 0 || a->bias_values_stride < 0))) return LM_E_INVALID;
+  if (a->mask && (a->mask_stride < (a->vocab + 31) / 32 || a->mask_count < (a->mask_rows ? 0 : a->rows))) return LM_E_INVALID;
+  if (a->vocab > LM_MAX_VOCAB || a->rows > 0x7FFFFFFF || (a->history && a->hist_len > kLogitsMaxHistory) || a->bias_len > kLogitsMaxBias || a->mask_count > 0x7FFFFFFF) return LM_E_UNSUPPORTED;
+  const int64_t size = a->dtype == LM_DTYPE_F32 ? 4 : 2;
+  if (misaligned(a->logits, static_cast<size_t>(size)) || misaligned(a->out, static_cast<size_t>(size))) return LM_E_INVALID;
+  bool same = false;
+  int rc = logits_overlap(a, size, &same);
+  if (rc != LM_OK) return rc;
+  const bool lists = (a->history && a->hist_len > 0) || a->bias_len > 0;
+  if (same && !lists && !a->mask) return LM_OK;                             // nothing to do
+  int sms = 0;
+  rc = sm_count(&sms);
+  if (rc != LM_OK) return rc;
+  LogitsDev P;
+  P.in = a->logits; P.in_stride = a->row_stride; P.out = a->out; P.out_stride = a->out_stride; P.in_place = same ? 1 : 0;
+  P.rows = static_cast<int>(a->rows); P.vocab = static_cast<int>(a->vocab);
+  P.history = a->hist_len > 0 ? a->history : nullptr; P.hist_len = static_cast<int>(a->hist_len); P.hist_stride = a->hist_stride; P.lengths = a->history_len; P.prompts = a->prompt_len;
+  P.rho = a->repetition; P.rho_s = a->repetition_s; P.pi = a->presence; P.pi_s = a->presence_s; P.phi = a->frequency; P.phi_s = a->frequency_s;
+  P.bias_ids = a->bias_ids; P.bias_ids_stride = a->bias_ids_stride; P.bias_values = a->bias_values; P.bias_values_stride = a->bias_values_stride; P.bias_len = static_cast<int>(a->bias_len);
+  P.mask = a->mask; P.mask_stride = a->mask_stride; P.mask_rows = a->mask_rows; P.mask_count = static_cast<int>(a->mask_count);
+  // slices: as many as give every SM four blocks, within the bounds of the tables
+  const long long total = static_cast<long long>(a->rows) * a->vocab;
+  long long per = (total / (4LL * sms) + 255) / 256 * 256;
+  if (per < kLogitsMinSlice) per = kLogitsMinSlice;
+  if (per > kLogitsMaxSlice) per = kLogitsMaxSlice;
+  P.slices = static_cast<int>((a->vocab + per - 1) / per);
+  P.slice = static_cast<int>(((a->vocab + P.slices - 1) / P.slices + 31) / 32 * 32);
+  P.slices = static_cast<int>((a->vocab + P.slice - 1) / P.slice);
+  const size_t smem = lists ? static_cast<size_t>(P.slice) * 4 * (a->bias_len > 0 ? 2 : 1) : 0;
+  const bool f32 = a->dtype == LM_DTYPE_F32;
+  rc = ensure_dynamic_smem(f32 ? kSlotLogitsF32 : kSlotLogits, f32 ? reinterpret_cast<const void*>(logits_kernel<true>) : reinterpret_cast<const void*>(logits_kernel<false>), smem);
+  if (rc != LM_OK) return rc;
+  const long long items = static_cast<long long>(P.rows) * P.slices;
+  const unsigned grid = static_cast<unsigned>(items < 0x7FFFFFFF ? items : 0x7FFFFFFF);
+  cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  return f32 ? launch_beside(logits_kernel<true>, dim3(grid), kLogitsThreads, smem, 1, st, P) : launch_beside(logits_kernel<false>, dim3(grid), kLogitsThreads, smem, 1, st, P);
+}
+
+}  // extern "C"

@@ -1,0 +1,297 @@
+"""The microscaled 4-bit weight and the projection with it on the GPU, against the binary64 restatement (oracle/nvfp4.py). Codes and block scales are equal, bit for
+bit: they are defined as roundings of real quotients. A logit is the BF16 rounding (half a step: 2^-8 of the value) of a sum whose FP32 accumulation may be off by
+2^-23 of the magnitudes' sum per addition."""
+import numpy as np
+import pytest
+import torch
+
+import lithos_metal_b200 as lm
+import oracle
+from oracle import head as o_head
+from oracle import nvfp4 as o
+
+pytestmark = pytest.mark.gpu
+
+
+def bf16(codes):
+    return torch.from_numpy(np.ascontiguousarray(codes).view(np.int16)).cuda().view(torch.bfloat16)
+
+
+def quantized(x, scale=None):
+    w = lm.quantize_nvfp4(x, scale=scale)
+    return w, w.codes.cpu().numpy(), w.scales.cpu().numpy(), np.float32(w.scale.item())
+
+
+def random_weight(rng, vocab, hidden, g=0.01):
+    """Any codes and any finite positive scales: what a checkpoint could hold."""
+    codes = rng.integers(0, 256, (vocab, hidden // 2), dtype=np.uint8)
+    scales = rng.integers(0, 127, (vocab, hidden // 16)).astype(np.uint8)
+    return codes, scales, np.float32(g)
+
+
+def as_weight(codes, scales, g):
+    return lm.Nvfp4Weight(torch.from_numpy(codes).cuda(), torch.from_numpy(scales).cuda(), torch.tensor([g], dtype=torch.float32, device="cuda"))
+
+
+def check_head(got, x, codes, scales, g, extra=0.0):
+    want, bound = o.head(x, codes, scales, g)
+    bound = bound + extra
+    error = np.abs(got.float().cpu().numpy().astype(np.float64) - want)
+    limit = bound + 2.0 ** -8 * (np.abs(want) + bound)
+    assert (error <= limit).all(), float((error / np.maximum(limit, 1e-300)).max())
+
+
+# ---- the format -----------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(1, 16), (3, 48), (257, 1040), (64, 4096)])
+def test_codes_are_the_definitions(rows, cols, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(rows + cols)
+    x = (torch.randn(rows, cols, generator=gen, device="cuda") * 0.03 * torch.exp(2.0 * torch.randn(rows, 1, generator=gen, device="cuda"))).to(dtype)
+    w, codes, scales, g = quantized(x)
+    host = x.float().cpu().numpy()
+    assert g == o.global_scale(host)
+    want_codes, want_scales = o.quantize(host, g)
+    assert np.array_equal(scales, want_scales) and np.array_equal(codes, want_codes)
+    assert np.array_equal(w.dequantize().cpu().numpy(), (o.values(codes, scales, np.float32(1.0)).astype(np.float32) * g))
+    given = torch.tensor([float(g) * 1.7], dtype=torch.float32, device="cuda")
+    _, codes, scales, g2 = quantized(x, given)
+    want_codes, want_scales = o.quantize(host, g2)
+    assert np.array_equal(scales, want_scales) and np.array_equal(codes, want_codes)
+
+
+@pytest.mark.parametrize("g", [1.0, 2.0 ** -7, 0.3, 2.0 ** -120, 2.0 ** 110])
+def test_every_border_and_its_neighbours(g):
+    """Inputs on, just below and just above every border between two codes, and every border between two block scales."""
+    g = np.float32(g)
+    rng = np.random.default_rng(7)
+    blocks = []
+    for s in list(range(1, 127, 5)) + [126]:
+        unit = o.E4M3[s] * np.float64(g)
+        for border in (o.E2M1[:-1] + o.E2M1[1:]) / 2:
+            v = np.float32(border * unit)
+            b = np.zeros(16, dtype=np.float32)
+            b[0] = np.float32(6 * unit)                                      # keeps the block's scale where it is
+            b[1:4] = [np.nextafter(v, np.float32(0)), v, np.nextafter(v, np.float32(np.inf))]
+            b[4:7] = -b[1:4]
+            blocks.append(b)
+    for lo, hi in zip(o.E4M3[:-1], o.E4M3[1:]):
+        v = np.float32((lo + hi) / 2 * 6.0 * np.float64(g))
+        for a in (np.nextafter(v, np.float32(0)), v, np.nextafter(v, np.float32(np.inf))):
+            b = (rng.standard_normal(16) * 0.2 * a).astype(np.float32).clip(-a, a)
+            b[5] = -a
+            blocks.append(b)
+    x = np.stack(blocks)
+    _, codes, scales, _ = quantized(torch.from_numpy(x).cuda(), torch.tensor([g], device="cuda"))
+    want_codes, want_scales = o.quantize(x, g)
+    assert np.array_equal(scales, want_scales) and np.array_equal(codes, want_codes)
+
+
+def test_zeros_infinities_and_nan():
+    x = np.zeros((6, 64), dtype=np.float32)
+    x[1, 3], x[2, 20], x[3, 40] = np.inf, np.nan, -np.inf
+    x[1:4, 63] = 1.5
+    x[4] = -0.0
+    x[5, :16] = 1e-20                                                        # far below the block scale of the largest: scale 0
+    w, codes, scales, g = quantized(torch.from_numpy(x).cuda())
+    want_codes, want_scales = o.quantize(x, g)
+    assert g == np.float32(1.5) / np.float32(2688) and np.array_equal(scales, want_scales) and np.array_equal(codes, want_codes)
+    v = w.dequantize().cpu().numpy()
+    assert np.isnan(v[1, :16]).all() and np.isnan(v[2, 16:32]).all() and np.isnan(v[3, 32:48]).all() and np.isfinite(v[[0, 4, 5]]).all()
+    assert v[1, 63] == np.float32(2688.0) * g        # (code 6, scale 448: 2688 times fl32(1.5 / 2688), two roundings from 1.5: up to 2^-23 of it away)
+    # nothing but zeros, an empty matrix, and scales that are none
+    w, codes, scales, g = quantized(torch.zeros(2, 32, device="cuda"))
+    assert g == 1.0 and not codes.any() and not scales.any()
+    assert lm.quantize_nvfp4(torch.zeros(0, 32, device="cuda")).dequantize().shape == (0, 32)
+    for bad in (0.0, -1.0, float("nan"), float("inf")):
+        _, codes, scales, _ = quantized(torch.ones(1, 16, device="cuda"), torch.tensor([bad], device="cuda"))
+        assert scales.tolist() == [[127]] and not codes.any()
+
+
+def test_strides_of_a_view():
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    wide = torch.randn(40, 200, generator=gen, device="cuda")
+    for x in (wide[:, 3:3 + 96], wide[::2, 8:8 + 96], wide.bfloat16()[:, 5:5 + 96], wide[:, :96].T.contiguous().T[:, :96]):
+        _, codes, scales, g = quantized(x)
+        want_codes, want_scales = o.quantize(x.float().cpu().numpy(), g)
+        assert np.array_equal(scales, want_scales) and np.array_equal(codes, want_codes)
+    w = lm.quantize_nvfp4(wide[:, :96].contiguous())
+    out = torch.full((40, 101), 7.0, device="cuda")
+    w.dequantize(out=out[:, 3:99])
+    assert torch.equal(out[:, 3:99], w.dequantize()) and (out[:, :3] == 7).all() and (out[:, 99:] == 7).all()
+    part = w[10:25]
+    assert part.shape == (15, 96) and torch.equal(part.dequantize(), w.dequantize()[10:25])
+
+
+# ---- the projection ---------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16, 17, 33, 64, 100, 129, 256, 300])
+@pytest.mark.parametrize("hidden,vocab", [(64, 17), (192, 1000), (1024, 4099)])
+def test_head_against_the_definition(rows, hidden, vocab):
+    rng = np.random.default_rng(rows * 7 + vocab)
+    codes, scales, g = random_weight(rng, vocab, hidden)
+    x = bf16(oracle.f32_to_bf16((rng.standard_normal((rows, hidden)) * np.exp(rng.standard_normal((rows, 1)) * 3)).astype(np.float32)))
+    got = lm.lm_head(x, as_weight(codes, scales, g))
+    assert got.shape == (rows, vocab) and got.dtype == torch.bfloat16
+    check_head(got, x.float().cpu().numpy(), codes, scales, g)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 8, 20, 130])
+@pytest.mark.parametrize("one_plus", [True, False])
+def test_head_with_the_norm_fused(rows, one_plus):
+    rng = np.random.default_rng(rows)
+    hidden, vocab, eps = 2048, 3001, 1e-5
+    codes, scales, g = random_weight(rng, vocab, hidden)
+    x = oracle.f32_to_bf16((rng.standard_normal((rows, hidden)) * 2).astype(np.float32))
+    gamma = oracle.f32_to_bf16((rng.standard_normal(hidden) * 0.1).astype(np.float32))
+    got = lm.lm_head(bf16(x), as_weight(codes, scales, g), bf16(gamma), eps=eps, one_plus=one_plus)
+    # The norm's output is rounded to BF16: where the binary64 value lies next to a midpoint the FP32 one may round to its other neighbour. In FP32 some 21 roundings lie in a sum of
+    # squares (8 of a thread's, the joining), 2 in the mean and eps, all under the root (half of each), then the root, 1 + weight and two products: less than 16 * 2^-24 in all.
+    xf, gf = o_head._f32(x).astype(np.float64), o_head._f32(gamma).astype(np.float64)
+    y = xf / np.sqrt((xf * xf).mean(-1, keepdims=True) + np.float64(np.float32(eps))) * ((1.0 + gf) if one_plus else gf)
+    near = 2.0 ** -20 * np.abs(y)
+    lo, hi = (o_head._f32(o_head._bf16((y + d).astype(np.float32))).astype(np.float64) for d in (-near, near))
+    w = np.abs(o.values(codes, scales, g))
+    check_head(got, lo, codes, scales, g, extra=np.abs(hi - lo) @ w.T)
+
+
+@pytest.mark.parametrize("rows", [1, 8, 40, 200])
+def test_values_of_any_size_in_x(rows):
+    """Elements of a row further apart than binary16 reaches, subnormal rows, zero rows: the products are exact all the same."""
+    rng = np.random.default_rng(11 + rows)
+    hidden, vocab = 256, 300
+    codes, scales, g = random_weight(rng, vocab, hidden, 2.0 ** -9)
+    x = (rng.standard_normal((rows, hidden)) * 2.0 ** rng.integers(-60, 40, (rows, hidden))).astype(np.float32)
+    x[0] = 0.0
+    if rows > 4:
+        x[2] = rng.standard_normal(hidden).astype(np.float32) * 1e-39          # BF16 subnormals
+        x[3, :] = 0.0
+        x[3, 7], x[3, 100] = 3e37, 1e-30
+        x[4] = rng.standard_normal(hidden).astype(np.float32)
+    t = bf16(oracle.f32_to_bf16(x))
+    got = lm.lm_head(t, as_weight(codes, scales, g))
+    host = t.float().cpu().numpy().astype(np.float64)
+    want, bound = o.head(host, codes, scales, g)
+    error = np.abs(got.float().cpu().numpy().astype(np.float64) - want)
+    limit = bound + 2.0 ** -8 * (np.abs(want) + bound) + 2.0 ** -133           # (and half a BF16 subnormal step)
+    limit[np.abs(want) > 3.0e38] = np.inf                                    # (beyond BF16)
+    assert (error <= limit).all() and (got[0] == 0).all()
+    # a row with infinities or NaN does not reach the other rows
+    t2 = t.clone()
+    t2[-1, 5] = float("inf")
+    t2[-1, 9] = float("nan")
+    again = lm.lm_head(t2, as_weight(codes, scales, g))
+    assert torch.isnan(again[-1]).all()
+    if rows > 1:
+        e2 = np.abs(again[:-1].float().cpu().numpy().astype(np.float64) - want[:-1])
+        assert (e2 <= limit[:-1]).all()
+
+
+@pytest.mark.parametrize("rows", [1, 8, 24, 140])
+def test_a_nan_scale_reaches_its_row_of_the_weight_only(rows):
+    rng = np.random.default_rng(2)
+    codes, scales, g = random_weight(rng, 90, 128)
+    x = bf16(oracle.f32_to_bf16(rng.standard_normal((rows, 128)).astype(np.float32)))
+    whole = lm.lm_head(x, as_weight(codes, scales, g))
+    scales[33, 2] = 127
+    got = lm.lm_head(x, as_weight(codes, scales, g))
+    assert torch.isnan(got[:, 33]).all()
+    keep = torch.arange(90, device="cuda") != 33
+    assert torch.equal(got[:, keep].view(torch.int16), whole[:, keep].view(torch.int16))
+    # negative scales are numbers too
+    scales[33, 2] = 0x80 | 50
+    check_head(lm.lm_head(x, as_weight(codes, scales, g)), x.float().cpu().numpy(), codes, scales, g)
+
+
+@pytest.mark.parametrize("rows", [1, 8, 30, 256])
+def test_a_shard_of_the_weight_gives_the_bits_of_the_whole(rows):
+    rng = np.random.default_rng(9)
+    codes, scales, g = random_weight(rng, 9000, 512)
+    w = as_weight(codes, scales, g)
+    x = bf16(oracle.f32_to_bf16(rng.standard_normal((rows, 512)).astype(np.float32)))
+    whole = lm.lm_head(x, w)
+    for shards in (2, 3, 8):
+        parts = [lm.lm_head(x, w[lo:lo + width]) for lo, width in (lm.parallel.shard_vocab(9000, s, shards) for s in range(shards))]
+        assert torch.equal(torch.cat(parts, dim=1).view(torch.int16), whole.view(torch.int16))
+
+
+@pytest.mark.parametrize("rows", [3, 8, 50, 256])
+def test_strides_and_a_given_place(rows):
+    rng = np.random.default_rng(4)
+    codes, scales, g = random_weight(rng, 333, 192)
+    wide_c, wide_s = torch.zeros(333, 96 + 32, dtype=torch.uint8, device="cuda"), torch.zeros(333, 16, dtype=torch.uint8, device="cuda")
+    wide_c[:, 16:112], wide_s[:, 4:16] = torch.from_numpy(codes).cuda(), torch.from_numpy(scales).cuda()
+    w = lm.Nvfp4Weight(wide_c[:, 16:112], wide_s[:, 4:16].view(torch.float8_e4m3fn), torch.tensor([g], device="cuda"))
+    x = bf16(oracle.f32_to_bf16(rng.standard_normal((rows, 192 + 7)).astype(np.float32)))[:, 3:195]      # rows at odd addresses
+    whole = lm.lm_head(x.contiguous(), as_weight(codes, scales, g))
+    out = torch.full((rows + 2, 340), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = lm.lm_head(x, w, out=out[1:rows + 1, 5:338])
+    assert got.data_ptr() == out[1:, 5:].data_ptr() and torch.equal(got.view(torch.int16), whole.view(torch.int16))
+    assert (out[0] == 7).all() and (out[-1] == 7).all() and (out[:, :5] == 7).all() and (out[:, 338:] == 7).all()
+    assert lm.lm_head(x[:0], w).shape == (0, 333) and lm.lm_head(x, w[:0]).shape == (rows, 0)
+
+
+def test_refusals():
+    w = lm.quantize_nvfp4(torch.ones(20, 64, device="cuda"))
+    x = torch.zeros(2, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        lm.quantize_nvfp4(torch.zeros(2, 24, device="cuda"))
+    with pytest.raises(TypeError):
+        lm.quantize_nvfp4(torch.zeros(2, 32, dtype=torch.float16, device="cuda"))
+    with pytest.raises(RuntimeError):
+        lm.quantize_nvfp4(torch.zeros(2, 32))
+    with pytest.raises(ValueError):
+        lm.quantize_nvfp4(torch.zeros(2, 32, device="cuda"), scale=torch.ones(2, device="cuda"))
+    with pytest.raises(ValueError):
+        lm.lm_head(x.float(), w)
+    with pytest.raises(ValueError):
+        lm.lm_head(x[:, :32], w)
+    with pytest.raises(ValueError):
+        lm.lm_head(x, w, torch.ones(63, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(ValueError):
+        lm.lm_head(x, w, out=torch.zeros(2, 21, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(ValueError):
+        lm.Nvfp4Weight(w.codes, w.scales[:, :2], w.scale)
+    with pytest.raises(ValueError):
+        lm.Nvfp4Weight(w.codes.to(torch.int8), w.scales, w.scale)
+    with pytest.raises(TypeError):
+        w[3]
+    with pytest.raises(lm._lib.LithosError):                                 # a hidden size that is no multiple of 64
+        lm.lm_head(torch.zeros(2, 48, dtype=torch.bfloat16, device="cuda"), lm.quantize_nvfp4(torch.ones(20, 48, device="cuda")))
+    with pytest.raises(lm._lib.LithosError):                                 # codes off their alignment
+        c = torch.zeros(20 * 32 + 8, dtype=torch.uint8, device="cuda")[8:].view(20, 32)
+        lm.lm_head(x, lm.Nvfp4Weight(c, w.scales, w.scale))
+
+
+def test_captured_replayed_and_on_another_stream():
+    rng = np.random.default_rng(5)
+    codes, scales, g = random_weight(rng, 5000, 256)
+    w = as_weight(codes, scales, g)
+    a, b = (bf16(oracle.f32_to_bf16(rng.standard_normal((n, 256)).astype(np.float32))) for n in (8, 70))
+    want = [lm.lm_head(t, w).clone() for t in (a, b)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = [lm.lm_head(t, w) for t in (a, b)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(want, other))
+    graphs, outs = [], []
+    for t in (a, b):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(lm.lm_head(t, lm.quantize_nvfp4(w.dequantize(), scale=w.scale)))
+        graphs.append(graph)
+    keep = [t.clone() for t in (a, b)]
+    for t in (a, b):
+        t.mul_(-1.0)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):                                                       # both at once
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    again = lm.quantize_nvfp4(w.dequantize(), scale=w.scale)
+    for t, out in zip(keep, outs):
+        assert torch.equal(out, lm.lm_head(-t, again))
