@@ -48,6 +48,12 @@ __device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b) { uint32_t
 __device__ __forceinline__ uint16_t f32_to_f16(float f) { uint16_t r; asm("cvt.rn.f16.f32 %0, %1;" : "=h"(r) : "f"(f)); return r; }
 __device__ __forceinline__ uint16_t f32_to_bf16(float f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f)); }
 
+// A BF16 value times 2^shift as binary16; false where that is not exact (a product that vanishes in binary32 included).
+__device__ __forceinline__ bool scaled_f16(uint16_t bf16, int shift, uint16_t* h) {
+  const float f = ldexpf(__uint_as_float(static_cast<uint32_t>(bf16) << 16), shift);
+  *h = f32_to_f16(f);
+  return f16_lo(*h) == f && (f != 0.0f || (bf16 & 0x7FFFu) == 0u);
+}
 // The sum of a logit times g and 2^-n (n: what x was multiplied by), in binary64 so that no intermediate leaves the range.
 __device__ __forceinline__ float head4_finish(double sum, float g, int n) {
   return __double2float_rn(sum * static_cast<double>(g) * __hiloint2double((1023 - n) << 20, 0));
@@ -122,9 +128,8 @@ static __global__ void __launch_bounds__(kH4Threads, 2) lm_head_nvfp4_kernel(Hea
 #pragma unroll
     for (int r = 0; r < kH4Rows; r++) {
       uint16_t* p = reinterpret_cast<uint16_t*>(smem_raw + r * row_bytes + head4_x_offset(k));
-      const float f = ldexpf(__uint_as_float(static_cast<uint32_t>(*p) << 16), shift[r]);
-      const uint16_t h = f32_to_f16(f);
-      bad |= f16_lo(h) != f;
+      uint16_t h;
+      bad |= !scaled_f16(*p, shift[r], &h);
       *p = h;
     }
   }

@@ -5,6 +5,7 @@
 #include "common.cuh"
 #include "host.cuh"
 #include "lm_head_nvfp4.cuh"
+#include "lm_head_nvfp4_batch.cuh"
 #include "logits.cuh"
 #include "nvfp4.cuh"
 
@@ -75,8 +76,44 @@ int lm_dequantize_nvfp4(const lm_dequantize_nvfp4_args* a) {
 }
 
 size_t lm_head_nvfp4_workspace_bytes(int64_t rows, int64_t hidden_dim) {
-  (void)rows; (void)hidden_dim;
-  return 0;
+  if (rows <= kH4Rows || hidden_dim < 1 || rows > LM_HEAD_NVFP4_MAX_ROWS || hidden_dim > kH4MaxHidden) return 0;
+  return batch4_workspace_bytes(rows, hidden_dim);
+}
+
+// More rows than a decode step has: the rows of x prepared once, then one launch for every 256 of them.
+static int head_nvfp4_batch(const lm_head_nvfp4_args* a, int sms) {
+  if (!a->workspace || misaligned(a->workspace, 256) || a->workspace_bytes < batch4_workspace_bytes(a->rows, a->hidden_dim)) return LM_E_WORKSPACE;
+  cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  unsigned char* ws = static_cast<unsigned char*>(a->workspace);
+  const int padded = batch4_padded(a->rows);
+  Rows4Dev R;
+  R.x = static_cast<const uint16_t*>(a->hidden); R.x_stride = a->hidden_stride; R.rows = static_cast<int>(a->rows); R.hidden = static_cast<int>(a->hidden_dim);
+  R.gamma = static_cast<const uint16_t*>(a->norm_weight); R.eps = a->eps; R.one_plus = a->one_plus;
+  R.xt = ws; ws += batch4_xt_bytes(a->rows, a->hidden_dim);
+  ws = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~static_cast<uintptr_t>(255));
+  R.xb = reinterpret_cast<uint16_t*>(ws); ws += batch4_xb_bytes(a->rows, a->hidden_dim);
+  R.shift = reinterpret_cast<int*>(ws); R.bad = R.shift + padded;
+  int rc = launch_beside(nvfp4_rows_kernel, dim3(static_cast<unsigned>(padded)), kB4RowsThreads, static_cast<size_t>(R.hidden) * 2, 1, st, R);
+  if (rc != LM_OK) return rc;
+  Batch4Dev P;
+  P.codes = a->codes; P.codes_stride = a->codes_stride; P.scales = a->scales; P.scales_stride = a->scales_stride; P.scale = a->scale;
+  P.hidden = R.hidden; P.vocab = static_cast<int>(a->vocab); P.logits_stride = a->logits_stride;
+  rc = ensure_dynamic_smem(kSlotHeadNvfp4Batch, reinterpret_cast<const void*>(lm_head_nvfp4_batch_kernel), kB4SmemLimit);
+  if (rc != LM_OK) return rc;
+  const int tiles = (P.vocab + kB4Tile - 1) / kB4Tile;
+  for (int64_t r = 0; r < a->rows; r += kB4MaxN) {
+    P.rows = static_cast<int>(a->rows - r < kB4MaxN ? a->rows - r : kB4MaxN);
+    P.n = batch4_padded(P.rows);
+    P.xt = R.xt + static_cast<size_t>(r) * R.hidden * 2; P.xb = R.xb + static_cast<size_t>(r) * R.hidden; P.shift = R.shift + r; P.bad = R.bad + r;
+    P.logits = static_cast<uint16_t*>(a->logits) + r * a->logits_stride;
+    P.column_stride = P.n <= 32 ? 32 : P.n <= 64 ? 64 : P.n <= 128 ? 128 : 256;
+    P.per_pass = 512 / P.column_stride;
+    P.x_stages = static_cast<int>((kB4SmemLimit - batch4_smem_bytes(P.n, 0)) / static_cast<size_t>(batch4_x_stage_bytes(P.n)));
+    if (P.x_stages > kB4MaxXStages) P.x_stages = kB4MaxXStages;
+    rc = launch_stream(true, lm_head_nvfp4_batch_kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), kB4Threads, batch4_smem_bytes(P.n, P.x_stages), 1, st, P);
+    if (rc != LM_OK) return rc;
+  }
+  return LM_OK;
 }
 
 int lm_head_nvfp4(const lm_head_nvfp4_args* a) {
@@ -96,6 +133,7 @@ int lm_head_nvfp4(const lm_head_nvfp4_args* a) {
   int sms = 0;
   rc = sm_count(&sms);
   if (rc != LM_OK) return rc;
+  if (a->rows > kH4Rows) return head_nvfp4_batch(a, sms);
   const size_t smem = head4_smem_bytes(P.hidden);
   rc = ensure_dynamic_smem(kSlotHeadNvfp4, reinterpret_cast<const void*>(lm_head_nvfp4_kernel), smem);
   if (rc != LM_OK) return rc;
@@ -103,14 +141,8 @@ int lm_head_nvfp4(const lm_head_nvfp4_args* a) {
   if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, lm_head_nvfp4_kernel, kH4Threads, smem) != cudaSuccess || per_sm < 1) per_sm = 1;
   const long long tiles = (a->vocab + kH4Tile - 1) / kH4Tile, most = static_cast<long long>(per_sm) * sms;
   const unsigned grid = static_cast<unsigned>(tiles < most ? tiles : most);
-  for (int64_t r = 0; r < a->rows; r += kH4Rows) {
-    P.x = static_cast<const uint16_t*>(a->hidden) + r * a->hidden_stride;
-    P.logits = static_cast<uint16_t*>(a->logits) + r * a->logits_stride;
-    P.rows = static_cast<int>(a->rows - r < kH4Rows ? a->rows - r : kH4Rows);
-    rc = launch_beside(lm_head_nvfp4_kernel, dim3(grid), kH4Threads, smem, 1, static_cast<cudaStream_t>(a->stream), P);
-    if (rc != LM_OK) return rc;
-  }
-  return LM_OK;
+  P.x = static_cast<const uint16_t*>(a->hidden); P.logits = static_cast<uint16_t*>(a->logits); P.rows = static_cast<int>(a->rows);
+  return launch_beside(lm_head_nvfp4_kernel, dim3(grid), kH4Threads, smem, 1, static_cast<cudaStream_t>(a->stream), P);
 }
 
 // Whether writing `out` can change what is read of `in` (both [rows, vocab] in elements of `size` bytes): same place and strides is in place, sharing nothing is fine.

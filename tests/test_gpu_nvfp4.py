@@ -187,6 +187,21 @@ def test_values_of_any_size_in_x(rows):
         assert (e2 <= limit[:-1]).all()
 
 
+@pytest.mark.parametrize("rows", [1, 3, 9])
+@pytest.mark.parametrize("small", [1e-7, 1e-9, 1e-20, 1e-30, 1e-39])
+def test_a_small_element_beside_a_large_one(rows, small):
+    """Where the large element's code is 0 the small one's product is the whole logit."""
+    rng = np.random.default_rng(3)
+    codes, scales, g = random_weight(rng, 200, 64, 2.0 ** -6)
+    codes[::2, 3] &= 0xF8                                                   # column 6: magnitude 0 in every other row
+    x = np.zeros((rows, 64), dtype=np.float32)
+    x[:, 6], x[:, 33] = 1e6, small
+    t = bf16(oracle.f32_to_bf16(x))
+    want, bound = o.head(t.float().cpu().numpy(), codes, scales, g)
+    error = np.abs(lm.lm_head(t, as_weight(codes, scales, g)).float().cpu().numpy().astype(np.float64) - want)
+    assert (error <= bound + 2.0 ** -8 * (np.abs(want) + bound) + 2.0 ** -134).all()      # (2^-134: half a BF16 subnormal step)
+
+
 @pytest.mark.parametrize("rows", [1, 8, 24, 140])
 def test_a_nan_scale_reaches_its_row_of_the_weight_only(rows):
     rng = np.random.default_rng(2)
