@@ -1,13 +1,14 @@
 // The vocabulary projection with a 4-bit weight for more rows than a decode step has (9 and up): logits = x * W^T on tcgen05, 128 vocabulary rows (M) by up to
 // 256 rows of x (N) to an accumulator, FP32 in tensor memory.
 //
-// W arrives as codes and leaves shared memory as binary16: 16 warps take a tile's codes from global memory (several tiles ahead, in registers), multiply by the block scales
-// (exact, nvfp4.cuh) and store the operand in the 128-byte swizzle; one thread issues the products. x is prepared once per call by nvfp4_rows_kernel: normalised if a norm is
+// W arrives in shared memory as codes and goes to tensor memory as binary16: 16 warps turn codes into binary16, multiply by the block scales (exact, nvfp4.cuh) and store the A
+// operand there, a lane a row; one thread issues the products. (With A in shared memory a tile's 32 KB were written and read there once more: 218 us with 16 rows, 384 with 256, bound by
+// shared memory's bandwidth.) x is prepared once per call by nvfp4_rows_kernel: normalised if a norm is
 // fused, scaled by a power of two per row, rounded to binary16 (exact; rows where it is not are done over, in FP64, at the end), laid out so that the columns of a step are
 // one contiguous piece: an untiled bulk copy brings it.
 //
-// A block owns a contiguous range of tiles and walks the hidden dimension once for as many of them as tensor memory holds accumulators (512 columns: 2 tiles of 256 rows, 16 of
-// 32): x then crosses from L2 once for all of these. The order of a logit's additions is that of the hidden dimension, whatever the tile or the block.
+// A block owns a contiguous range of tiles and walks the hidden dimension once for as many of them as tensor memory holds accumulators beside four operands (256 columns: a tile of
+// 256 rows, 8 of 32): x then crosses from L2 once for all of these. The order of a logit's additions is that of the hidden dimension, whatever the tile or the block.
 // Every wait has a limit; a block whose wait ran out writes NaN.
 #pragma once
 #include "common.cuh"
@@ -19,13 +20,15 @@ namespace lm {
 constexpr int kB4Tile = 128;                 // vocabulary rows per tile (M)
 constexpr int kB4MaxN = 256;                 // rows of x per launch
 constexpr int kB4Cols = 128;                 // columns per step
-constexpr int kB4Stages = 3;                 // tiles of W in shared memory
-constexpr int kB4StageBytes = kB4Tile * kB4Cols * 2;
-constexpr int kB4DequantWarps = 16, kB4DoneWarps = 4;
+constexpr int kB4Groups = 4;                 // tiles of W in the making, and as many operands in tensor memory
+constexpr int kB4Ahead = 4;                  // tiles of a group whose codes are in shared memory or on the way, at most
+constexpr int kB4WarpBytes = 32 * (kB4Cols / 2 + kB4Cols / kFp4Block);      // a warp's 32 rows of a tile: codes and scales
+constexpr int kB4OperandColumns = kB4Cols / 2;                              // of tensor memory, per tile of W
+constexpr int kB4SumColumns = 512 - kB4Groups * kB4OperandColumns;          // ... for the accumulators
+constexpr int kB4DequantWarps = 4 * kB4Groups, kB4DoneWarps = 4;
 constexpr int kB4MmaWarp = kB4DequantWarps, kB4CopyWarp = kB4MmaWarp + 1, kB4FirstDoneWarp = kB4CopyWarp + 1;
 constexpr int kB4Threads = 32 * (kB4FirstDoneWarp + kB4DoneWarps);
-constexpr int kB4Ahead = 6;                  // tiles whose codes are in flight
-constexpr int kB4MaxXStages = 4;
+constexpr int kB4MaxXStages = 4, kB4MaxSums = kB4SumColumns / 32;
 constexpr int kB4RowsThreads = 256;
 constexpr uint32_t kB4WaitLimit = 1u << 20;
 constexpr int kB4SmemLimit = 232448;
@@ -35,7 +38,7 @@ struct Batch4Dev {
   int hidden; int vocab; int rows; int n;    // n: rows padded to a multiple of 16
   const uint8_t* xt; const uint16_t* xb; const int* shift; const int* bad;
   uint16_t* logits; int64_t logits_stride;
-  int per_pass; int column_stride; int x_stages;
+  int per_pass; int column_stride; int ahead; int x_stages;
 };
 
 // Workspace: x in binary16 by steps of 64 columns, [group][hidden / 64][rows of the group, padded][128 bytes, swizzled]; x in BF16 [rows][hidden]; shift and bad [padded rows].
@@ -46,7 +49,9 @@ __host__ inline size_t batch4_workspace_bytes(int64_t rows, int64_t hidden) {
   return batch4_xt_bytes(rows, hidden) + batch4_xb_bytes(rows, hidden) + 2 * (static_cast<size_t>(batch4_padded(rows)) * 4 + 255) / 256 * 256 + 512;
 }
 __host__ __device__ inline int batch4_x_stage_bytes(int n) { return n * kB4Cols * 2; }
-__host__ inline size_t batch4_smem_bytes(int n, int x_stages) { return 1024 + kB4Stages * kB4StageBytes + static_cast<size_t>(x_stages) * batch4_x_stage_bytes(n) + kB4MaxN * 4 + 256; }
+__host__ inline size_t batch4_smem_bytes(int n, int ahead, int x_stages) {
+  return 1024 + static_cast<size_t>(x_stages) * batch4_x_stage_bytes(n) + static_cast<size_t>(ahead) * kB4DequantWarps * kB4WarpBytes + kB4MaxN * 4 + 512;
+}
 
 struct Rows4Dev {
   const uint16_t* x; int64_t x_stride; int rows; int hidden;
@@ -158,6 +163,11 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, vola
   *given_up = 1u;
   return false;
 }
+__device__ __forceinline__ bool elected() {                                 // true in one lane of a warp that is together, always the same
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0u;
+}
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
@@ -168,8 +178,16 @@ __device__ __forceinline__ void products_commit(uint32_t bar) {
 __device__ __forceinline__ uint64_t operand(uint32_t address) {
   return static_cast<uint64_t>((address >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ void product_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t form, bool add) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(form), "r"(add ? 1u : 0u) : "memory");
+__device__ __forceinline__ void product_f16(bool one, uint32_t d, uint32_t a, uint64_t b, uint32_t form, uint32_t add) {     // a: in tensor memory
+  if (one) asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(form), "r"(add) : "memory");
+}
+__device__ __forceinline__ void operand16(uint32_t address, const uint32_t (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if (N == 16) asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
 }
 __device__ __forceinline__ void accumulators32(uint32_t address, uint32_t (&v)[32]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -179,6 +197,13 @@ __device__ __forceinline__ void accumulators32(uint32_t address, uint32_t (&v)[3
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ uint32_t picked(const uint32_t (&v)[32], int j) {
+  uint32_t r = v[0];
+#pragma unroll
+  for (int i = 1; i < 32; i++) r = i == j ? v[i] : r;
+  return r;
+}
+
 // The tiles and steps of a block in the order they are taken: passes of per_pass tiles, in a pass the steps, in a step the tiles.
 struct Walk4 {
   int first, last, end, per_pass, steps;     // the pass' tiles [first, last)
@@ -186,26 +211,27 @@ struct Walk4 {
   __device__ __forceinline__ Walk4(int begin, int end_, int per_pass_, int steps_)
       : first(begin), last(min(begin + per_pass_, end_)), end(end_), per_pass(per_pass_), steps(steps_), tile(begin), step(0) {}
   __device__ __forceinline__ bool more() const { return first < end; }
-  __device__ __forceinline__ void next() {
-    if (++tile < last) return;
-    tile = first;
-    if (++step < steps) return;
-    step = 0; first = last; last = min(first + per_pass, end); tile = first;
+  __device__ __forceinline__ void skip(int n) {
+    tile += n;
+    while (tile >= last && first < end) {
+      if (++step < steps) { tile -= last - first; continue; }
+      step = 0; first = last; last = min(first + per_pass, end);
+    }
   }
 };
 
 static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kernel(Batch4Dev P) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_address(smem_raw) & 1023u)) & 1023u);
-  unsigned char* ws = smem;                                                 // W: kB4Stages tiles
-  unsigned char* xs = ws + kB4Stages * kB4StageBytes;                        // x: x_stages steps
+  unsigned char* xs = smem;                                                 // x: x_stages steps
   const int x_bytes = batch4_x_stage_bytes(P.n);
-  float* factor = reinterpret_cast<float*>(xs + P.x_stages * x_bytes);        // [n] g * 2^-shift
+  unsigned char* cs = xs + P.x_stages * x_bytes;                             // codes and scales: [warp][ahead]
+  float* factor = reinterpret_cast<float*>(cs + P.ahead * kB4DequantWarps * kB4WarpBytes);     // [n] g * 2^-shift
   uint64_t* bars = reinterpret_cast<uint64_t*>(factor + kB4MaxN);
-  uint32_t* words = reinterpret_cast<uint32_t*>(bars + 2 * kB4Stages + 2 * kB4MaxXStages + 3);     // [0] tensor memory, [1] given up
+  uint32_t* words = reinterpret_cast<uint32_t*>(bars + 2 * kB4Groups + 2 * kB4MaxXStages + 2 * kB4MaxSums + 1);     // [0] tensor memory, [1] given up
   volatile uint32_t* given_up = words + 1;
-  const uint32_t w_full = smem_address(bars), w_empty = w_full + 8 * kB4Stages, x_full = w_empty + 8 * kB4Stages, x_empty = x_full + 8 * kB4MaxXStages, acc_full = x_empty + 8 * kB4MaxXStages,
-                 acc_empty = acc_full + 8, drained = acc_empty + 8;
+  const uint32_t w_full = smem_address(bars), w_empty = w_full + 8 * kB4Groups, x_full = w_empty + 8 * kB4Groups, x_empty = x_full + 8 * kB4MaxXStages, acc_full = x_empty + 8 * kB4MaxXStages,
+                 acc_empty = acc_full + 8 * kB4MaxSums, drained = acc_empty + 8 * kB4MaxSums;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int H = P.hidden, steps = (H + kB4Cols - 1) / kB4Cols;
   const int n_tiles = (P.vocab + kB4Tile - 1) / kB4Tile;
@@ -215,9 +241,10 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 0) {
-    for (int s = 0; s < kB4Stages; s++) { barrier_init(w_full + 8 * s, kB4DequantWarps); barrier_init(w_empty + 8 * s, 1); }
+    for (int s = 0; s < kB4Groups; s++) { barrier_init(w_full + 8 * s, 4); barrier_init(w_empty + 8 * s, 1); }
     for (int s = 0; s < kB4MaxXStages; s++) { barrier_init(x_full + 8 * s, 1); barrier_init(x_empty + 8 * s, 1); }
-    barrier_init(acc_full, 1); barrier_init(acc_empty, kB4DoneWarps); barrier_init(drained, 1);
+    for (int s = 0; s < kB4MaxSums; s++) { barrier_init(acc_full + 8 * s, 1); barrier_init(acc_empty + 8 * s, kB4DoneWarps); }
+    barrier_init(drained, 1);
     words[1] = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -235,97 +262,114 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
   const uint32_t tmem = words[0];
 
   if (warp < kB4DequantWarps) {
-    // ---- W: a warp has 8 rows of a tile, 4 lanes to a row, 32 columns each (16 bytes of codes, two scales)
-    const int r8 = lane >> 2, q = lane & 3, row = 8 * warp + r8;
-    // (the four 16-byte chunks of a lane in an order that keeps 8 lanes -- 2 rows, 2 halves of 64 columns -- on different banks)
-    const bool swap = q >= 2;
-    const uint32_t base = static_cast<uint32_t>((q >> 1) * (kB4Tile * 128) + row * 128);
-    uint32_t offset[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) offset[i] = base + static_cast<uint32_t>((((q & 1) * 4 + (swap ? i ^ 2 : i)) ^ r8) << 4);
-    uint4 c[kB4Ahead];
-    uint32_t s[kB4Ahead];
-    Walk4 load(begin, end, P.per_pass, steps), use = load;
-    auto fetch = [&](uint4& cc, uint32_t& ss) {
-      cc = make_uint4(0u, 0u, 0u, 0u); ss = 0u;
+    // ---- W: a group of 4 warps has a tile, a lane a row of it (a lane of tensor memory). Codes come by asynchronous copies, four lanes to a row; the 16-byte piece q of row r lies at
+    // 64 r + 16 (q ^ (r / 2 mod 4)), so that 8 lanes reading their rows' piece meet different banks.
+    const int group = warp >> 2, quarter = warp & 3, r8 = lane >> 2, q = lane & 3;
+    unsigned char* mine = cs + warp * P.ahead * kB4WarpBytes;
+    const uint32_t to = smem_address(mine);
+    const uint32_t piece = static_cast<uint32_t>(r8 * 64 + ((q ^ ((r8 >> 1) & 3)) << 4));
+    const uint32_t codes_stride = static_cast<uint32_t>(P.codes_stride), scales_stride = static_cast<uint32_t>(P.scales_stride), last_row = static_cast<uint32_t>(P.vocab - 1);
+    const bool pairs = ((reinterpret_cast<uintptr_t>(P.scales) | scales_stride) & 7u) == 0;
+    Walk4 load(begin, end, P.per_pass, steps);
+    load.skip(group);
+    Walk4 use = load;
+    int slot = 0;
+    auto fetch = [&]() {                                                     // the next tile's columns of a step into the next slot
       if (load.more()) {
-        const int64_t v = min(load.tile * kB4Tile + row, P.vocab - 1);       // (rows beyond the vocabulary: the last one again, never stored)
-        const int k = load.step * kB4Cols + q * 32;
-        if (k < H) {
-          cc = __ldcs(reinterpret_cast<const uint4*>(P.codes + v * P.codes_stride + (k >> 1)));
-          ss = __ldg(reinterpret_cast<const uint16_t*>(P.scales + v * P.scales_stride + (k >> 4)));
+        const int row = load.tile * kB4Tile + 32 * quarter, k = load.step * kB4Cols;
+        const uint32_t at = to + slot * kB4WarpBytes;
+        if (k + q * 32 < H) {                                                // (the last step may have 64 columns only)
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            const uint32_t v = min(static_cast<uint32_t>(row + 8 * u + r8), last_row);           // (rows beyond the vocabulary: the last one again, never stored)
+            copy_async<16>(at + piece + u * 512, P.codes + static_cast<uint64_t>(v) * codes_stride + (k >> 1) + q * 16);
+          }
         }
-        load.next();
+        const uint8_t* from = P.scales + static_cast<uint64_t>(min(static_cast<uint32_t>(row + lane), last_row)) * scales_stride + (k >> 4);
+        const uint32_t sa = at + 2048 + lane * 8;
+        if (k + 64 < H && pairs) copy_async<8>(sa, from);
+        else { copy_async<4>(sa, from); if (k + 64 < H) copy_async<4>(sa + 4, from + 4); }
+        load.skip(kB4Groups);
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (++slot == P.ahead) slot = 0;
     };
-#pragma unroll
-    for (int u = 0; u < kB4Ahead; u++) fetch(c[u], s[u]);
-    int stage = 0; uint32_t phase = 0u;
+    for (int d = 0; d < P.ahead - 1; d++) fetch();
+    const uint32_t operand = tmem + kB4SumColumns + static_cast<uint32_t>(group * kB4OperandColumns) + (static_cast<uint32_t>(quarter * 32) << 16);
+    uint32_t phase = 1u;
+    int from = 0;
     bool go = true;
-    while (go && use.more()) {
+    for (; go && use.more(); use.skip(kB4Groups)) {
+      if (P.ahead == 4) asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else if (P.ahead == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+      fetch();
+      const unsigned char* row = mine + from * kB4WarpBytes + lane * 64;
+      const uint2 sc = *reinterpret_cast<const uint2*>(mine + from * kB4WarpBytes + 2048 + lane * 8);
+      if (++from == P.ahead) from = 0;
+      go = __all_sync(kFull, barrier_wait(w_empty + 8 * group, phase, given_up));
+      phase ^= 1u;
+      if (!go) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-      for (int u = 0; u < kB4Ahead; u++) {
-        if (!go || !use.more()) break;
-        const uint4 cc = c[u];
-        const uint32_t pair = e4m3_to_f16(s[u]);
-        const bool half = use.step * kB4Cols + q * 32 < H;                   // (the last step may have 64 columns only)
-        fetch(c[u], s[u]);
-        const uint32_t s0 = __byte_perm(pair, 0u, swap ? 0x3232 : 0x1010), s1 = __byte_perm(pair, 0u, swap ? 0x1010 : 0x3232);
-        const uint32_t w[4] = {swap ? cc.z : cc.x, swap ? cc.w : cc.y, swap ? cc.x : cc.z, swap ? cc.y : cc.w};
-        uint4 h[4];
+      for (int i = 0; i < 4; i++) {                                          // 32 columns
+        const uint4 cc = *reinterpret_cast<const uint4*>(row + ((i ^ ((lane >> 1) & 3)) << 4));
+        const uint32_t pair = e4m3_to_f16((i < 2 ? sc.x : sc.y) >> (16 * (i & 1)));
+        const uint32_t w[4] = {cc.x, cc.y, cc.z, cc.w};
+        uint32_t v[16];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          uint32_t v[4];
-          e2m1_to_f16(w[i], v);
-          const uint32_t sc = i < 2 ? s0 : s1;
-          h[i] = make_uint4(f16x2_mul(v[0], sc), f16x2_mul(v[1], sc), f16x2_mul(v[2], sc), f16x2_mul(v[3], sc));
+        for (int j = 0; j < 4; j++) {
+          uint32_t h[4];
+          e2m1_to_f16(w[j], h);
+          const uint32_t s = __byte_perm(pair, 0u, j < 2 ? 0x1010 : 0x3232);
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[4 * j + e] = f16x2_mul(h[e], s);
         }
-        go = barrier_wait(w_empty + 8 * stage, phase ^ 1u, given_up);
-        if (go && half) {
-          unsigned char* out = ws + stage * kB4StageBytes;
+        operand16(operand + i * 16, v);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) barrier_arrive(w_full + 8 * group);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else if (warp == kB4MmaWarp) {
+    // (the whole warp walks, and one lane issues: its operands are then uniform values. A single lane's walk took 1300 clocks a tile.)
+    const uint32_t form = (1u << 4) | (static_cast<uint32_t>(P.n >> 3) << 17) | (static_cast<uint32_t>(kB4Tile >> 4) << 24);   // binary16 operands, FP32 accumulators
+    const bool one = elected();
+    int group = 0, xs_ = 0;
+    uint32_t wp = 0u, xp = 0u, ap = 1u;
+    bool go = true;
+    for (int first = begin; go && first < end; first += P.per_pass, ap ^= 1u) {
+      const int count = min(P.per_pass, end - first);
+      for (int step = 0; go && step < steps; step++) {
+        go = barrier_wait(x_full + 8 * xs_, xp, given_up);
+        const uint64_t b = operand(smem_address(xs) + xs_ * x_bytes), b2 = b + static_cast<uint64_t>(P.n * 8);      // (64 columns on: n * 128 bytes)
+        const bool both = H - step * kB4Cols > 64, last = step == steps - 1;
+        for (int sum = 0; go && sum < count; sum++) {
+          if (step == 0) go = barrier_wait(acc_empty + 8 * sum, ap, given_up);             // (the first pass finds them empty)
+          go = go && barrier_wait(w_full + 8 * group, wp, given_up);
+          if (!go) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t d = tmem + static_cast<uint32_t>(sum * P.column_stride), a = tmem + kB4SumColumns + static_cast<uint32_t>(group * kB4OperandColumns);
 #pragma unroll
-          for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(out + offset[i]) = h[i];
+          for (int k = 0; k < 4; k++) product_f16(one, d, a + 8 * k, b + 2 * k, form, k > 0 ? 1u : static_cast<uint32_t>(step));
+          if (both) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) product_f16(one, d, a + 32 + 8 * k, b2 + 2 * k, form, 1u);
+          }
+          if (one) products_commit(w_empty + 8 * group);
+          if (last && one) products_commit(acc_full + 8 * sum);
+          if (++group == kB4Groups) { group = 0; wp ^= 1u; }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) barrier_arrive(w_full + 8 * stage);
-        if (++stage == kB4Stages) { stage = 0; phase ^= 1u; }
-        use.next();
-        go = __all_sync(kFull, go);
+        if (one) products_commit(x_empty + 8 * xs_);
+        if (++xs_ == P.x_stages) { xs_ = 0; xp ^= 1u; }
       }
     }
-  } else if (warp == kB4MmaWarp) {
-    if (lane == 0) {
-      const uint32_t form = (1u << 4) | (static_cast<uint32_t>(P.n >> 3) << 17) | (static_cast<uint32_t>(kB4Tile >> 4) << 24);   // binary16 operands, FP32 accumulators
-      int ws_ = 0, xs_ = 0; uint32_t wp = 0u, xp = 0u, ap = 1u;
-      bool go = true;
-      for (Walk4 at(begin, end, P.per_pass, steps); go && at.more(); at.next()) {
-        if (at.tile == at.first) {
-          if (at.step == 0) { go = barrier_wait(acc_empty, ap, given_up); ap ^= 1u; }     // (the first pass finds them empty)
-          go = go && barrier_wait(x_full + 8 * xs_, xp, given_up);
-        }
-        go = go && barrier_wait(w_full + 8 * ws_, wp, given_up);
-        if (!go) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t d = tmem + static_cast<uint32_t>((at.tile - at.first) * P.column_stride);
-        const int halves = H - at.step * kB4Cols > 64 ? 2 : 1;
-        for (int half = 0; half < halves; half++) {
-          const uint64_t a = operand(smem_address(ws) + ws_ * kB4StageBytes + half * (kB4Tile * 128)), b = operand(smem_address(xs) + xs_ * x_bytes + half * P.n * 128);
-#pragma unroll
-          for (int k = 0; k < 4; k++) product_f16(d, a + 2 * k, b + 2 * k, form, at.step + half + k > 0);
-        }
-        products_commit(w_empty + 8 * ws_);
-        if (++ws_ == kB4Stages) { ws_ = 0; wp ^= 1u; }
-        if (at.tile == at.last - 1) {
-          products_commit(x_empty + 8 * xs_);
-          if (++xs_ == P.x_stages) { xs_ = 0; xp ^= 1u; }
-          if (at.step == steps - 1) products_commit(acc_full);
-        }
-      }
-      if (!go) {                                                            // what is under way ends before the block does
-        products_commit(drained);
-        for (uint32_t i = 0; i < kB4WaitLimit && !barrier_try(drained, 0u); i++) {}
-      }
+    if (!go && one) {                                                       // what is under way ends before the block does
+      products_commit(drained);
+      for (uint32_t i = 0; i < kB4WaitLimit && !barrier_try(drained, 0u); i++) {}
     }
   } else if (warp == kB4CopyWarp) {
     if (lane == 0) {
@@ -356,28 +400,33 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     uint32_t phase = 0u;
     for (int first = begin; go && first < end; first += P.per_pass, phase ^= 1u) {
       const int last = min(first + P.per_pass, end);
-      go = __all_sync(kFull, barrier_wait(acc_full, phase, given_up));
-      if (!go) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       for (int tile = first; tile < last; tile++) {
+        go = __all_sync(kFull, barrier_wait(acc_full + 8 * (tile - first), phase, given_up));
+        if (!go) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const int v = tile * kB4Tile + part * 32 + lane;
         for (int r0 = 0; r0 < P.n; r0 += 32) {
           uint32_t a[32];
           accumulators32(tmem + (static_cast<uint32_t>(part * 32) << 16) + static_cast<uint32_t>((tile - first) * P.column_stride + r0), a);
-          if (v < P.vocab) {
+          uint16_t* out = P.logits + r0 * P.logits_stride + v;
+          if (!plain) {
+            for (int j = 0; j < 32; j++)
+              if (v < P.vocab && r0 + j < P.rows) out[j * P.logits_stride] = f32_to_bf16(head4_finish(__uint_as_float(picked(a, j)), g, P.shift[r0 + j]));
+          } else {
+            const int there = v < P.vocab ? P.rows - r0 : 0;                  // rows of logits among the 32
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-              const int r = r0 + j;
-              if (r >= P.rows) break;
-              const float z = plain ? __fmul_rn(__uint_as_float(a[j]), factor[r]) : head4_finish(__uint_as_float(a[j]), g, P.shift[r]);
-              P.logits[r * P.logits_stride + v] = f32_to_bf16(z);
+            for (int j = 0; j < 32; j += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(factor + r0 + j);
+              const float fj[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+              for (int e = 0; e < 4; e++, out += P.logits_stride) if (j + e < there) *out = f32_to_bf16(__fmul_rn(__uint_as_float(a[j + e]), fj[e]));
             }
           }
         }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) barrier_arrive(acc_empty + 8 * (tile - first));
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) barrier_arrive(acc_empty);
     }
   }
   __syncwarp();

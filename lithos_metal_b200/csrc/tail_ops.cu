@@ -107,10 +107,11 @@ static int head_nvfp4_batch(const lm_head_nvfp4_args* a, int sms) {
     P.xt = R.xt + static_cast<size_t>(r) * R.hidden * 2; P.xb = R.xb + static_cast<size_t>(r) * R.hidden; P.shift = R.shift + r; P.bad = R.bad + r;
     P.logits = static_cast<uint16_t*>(a->logits) + r * a->logits_stride;
     P.column_stride = P.n <= 32 ? 32 : P.n <= 64 ? 64 : P.n <= 128 ? 128 : 256;
-    P.per_pass = 512 / P.column_stride;
-    P.x_stages = static_cast<int>((kB4SmemLimit - batch4_smem_bytes(P.n, 0)) / static_cast<size_t>(batch4_x_stage_bytes(P.n)));
-    if (P.x_stages > kB4MaxXStages) P.x_stages = kB4MaxXStages;
-    rc = launch_stream(true, lm_head_nvfp4_batch_kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), kB4Threads, batch4_smem_bytes(P.n, P.x_stages), 1, st, P);
+    P.per_pass = kB4SumColumns / P.column_stride;
+    P.x_stages = P.n <= 96 ? 3 : 2;                                         // steps of x in shared memory, and as many tiles of codes as fit beside them
+    P.ahead = kB4Ahead;
+    while (batch4_smem_bytes(P.n, P.ahead, P.x_stages) > kB4SmemLimit) P.ahead--;
+    rc = launch_stream(true, lm_head_nvfp4_batch_kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), kB4Threads, batch4_smem_bytes(P.n, P.ahead, P.x_stages), 1, st, P);
     if (rc != LM_OK) return rc;
   }
   return LM_OK;
@@ -124,6 +125,7 @@ int lm_head_nvfp4(const lm_head_nvfp4_args* a) {
   int rc = fp4_matrix_ok(a->vocab, a->hidden_dim, a->codes, a->codes_stride, a->scales, a->scales_stride, a->scale);
   if (rc != LM_OK) return rc;
   if (a->rows > LM_HEAD_NVFP4_MAX_ROWS || a->vocab > LM_MAX_VOCAB || (a->hidden_dim % 64) != 0 || a->hidden_dim > kH4MaxHidden) return LM_E_UNSUPPORTED;
+  if (a->codes_stride > 0x7FFFFFFF || a->scales_stride > 0x7FFFFFFF) return LM_E_UNSUPPORTED;
   if (misaligned(a->codes, 16) || (a->codes_stride % 16) != 0 || misaligned(a->scales, 4) || (a->scales_stride % 4) != 0) return LM_E_UNSUPPORTED;   // 16- and 4-byte loads
   Head4Dev P;
   P.x_stride = a->hidden_stride;
