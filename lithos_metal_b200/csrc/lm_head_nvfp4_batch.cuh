@@ -15,20 +15,24 @@
 #include "lm_head_nvfp4.cuh"
 #include "nvfp4.cuh"
 
+#include <cuda.h>
+
 namespace lm {
 
 constexpr int kB4Tile = 128;                 // vocabulary rows per tile (M)
 constexpr int kB4MaxN = 256;                 // rows of x per launch
-constexpr int kB4Cols = 128;                 // columns per step
-constexpr int kB4Groups = 4;                 // tiles of W in the making, and as many operands in tensor memory
-constexpr int kB4Ahead = 4;                  // tiles of a group whose codes are in shared memory or on the way, at most
-constexpr int kB4WarpBytes = 32 * (kB4Cols / 2 + kB4Cols / kFp4Block);      // a warp's 32 rows of a tile: codes and scales
-constexpr int kB4OperandColumns = kB4Cols / 2;                              // of tensor memory, per tile of W
-constexpr int kB4SumColumns = 512 - kB4Groups * kB4OperandColumns;          // ... for the accumulators
-constexpr int kB4DequantWarps = 4 * kB4Groups, kB4DoneWarps = 4;
-constexpr int kB4MmaWarp = kB4DequantWarps, kB4CopyWarp = kB4MmaWarp + 1, kB4FirstDoneWarp = kB4CopyWarp + 1;
+constexpr int kB4StepCols = 256;             // columns of a tile's codes that come together: 128 bytes a row, and 16 of scales
+constexpr int kB4Cols = 128;                 // columns of an operand: two a step
+constexpr int kB4XCols = 64;                 // columns of x that come together
+constexpr int kB4Pairs = 2;                  // steps of a tile in the making, and as many in tensor memory: 8 warps each, 4 to an operand
+constexpr int kB4CodeBytes = kB4Tile * kB4StepCols / 2, kB4SlotBytes = kB4CodeBytes + kB4Tile * kB4StepCols / kFp4Block;
+constexpr int kB4MaxCodeSlots = 8, kB4MaxXStages = 8;
+constexpr int kB4OperandColumns = kB4Cols / 2;                              // of tensor memory
+constexpr int kB4SumColumns = 512 - 2 * kB4Pairs * kB4OperandColumns;        // ... for the accumulators
+constexpr int kB4MaxSums = kB4SumColumns / 32;
+constexpr int kB4DequantWarps = 8 * kB4Pairs, kB4DoneWarps = 4;
+constexpr int kB4MmaWarp = kB4DequantWarps, kB4CopyWarp = kB4MmaWarp + 1, kB4CodeWarp = kB4CopyWarp + 1, kB4FirstDoneWarp = kB4CodeWarp + 1;
 constexpr int kB4Threads = 32 * (kB4FirstDoneWarp + kB4DoneWarps);
-constexpr int kB4MaxXStages = 4, kB4MaxSums = kB4SumColumns / 32;
 constexpr int kB4RowsThreads = 256;
 constexpr uint32_t kB4WaitLimit = 1u << 20;
 constexpr int kB4SmemLimit = 232448;
@@ -38,7 +42,7 @@ struct Batch4Dev {
   int hidden; int vocab; int rows; int n;    // n: rows padded to a multiple of 16
   const uint8_t* xt; const uint16_t* xb; const int* shift; const int* bad;
   uint16_t* logits; int64_t logits_stride;
-  int per_pass; int column_stride; int ahead; int x_stages;
+  int per_pass; int column_stride; int code_slots; int x_stages;
 };
 
 // Workspace: x in binary16 by steps of 64 columns, [group][hidden / 64][rows of the group, padded][128 bytes, swizzled]; x in BF16 [rows][hidden]; shift and bad [padded rows].
@@ -48,9 +52,9 @@ __host__ inline size_t batch4_xb_bytes(int64_t rows, int64_t hidden) { return (s
 __host__ inline size_t batch4_workspace_bytes(int64_t rows, int64_t hidden) {
   return batch4_xt_bytes(rows, hidden) + batch4_xb_bytes(rows, hidden) + 2 * (static_cast<size_t>(batch4_padded(rows)) * 4 + 255) / 256 * 256 + 512;
 }
-__host__ __device__ inline int batch4_x_stage_bytes(int n) { return n * kB4Cols * 2; }
-__host__ inline size_t batch4_smem_bytes(int n, int ahead, int x_stages) {
-  return 1024 + static_cast<size_t>(x_stages) * batch4_x_stage_bytes(n) + static_cast<size_t>(ahead) * kB4DequantWarps * kB4WarpBytes + kB4MaxN * 4 + 512;
+__host__ __device__ inline int batch4_x_stage_bytes(int n) { return n * kB4XCols * 2; }
+__host__ inline size_t batch4_smem_bytes(int n, int code_slots, int x_stages) {
+  return 1024 + static_cast<size_t>(code_slots) * kB4SlotBytes + static_cast<size_t>(x_stages) * batch4_x_stage_bytes(n) + kB4MaxN * 4 + 512;
 }
 
 struct Rows4Dev {
@@ -147,7 +151,7 @@ static __global__ void __launch_bounds__(kB4RowsThreads) nvfp4_rows_kernel(Rows4
 
 __device__ __forceinline__ uint32_t smem_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
-__device__ __forceinline__ void barrier_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void barrier_arrive(uint32_t bar, uint32_t count = 1u) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
 __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
 __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
@@ -171,6 +175,10 @@ __device__ __forceinline__ bool elected() {                                 // t
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
+// A box of 128 rows: 128 bytes of codes in the 128-byte swizzle, or 16 bytes of scales (columns a multiple of that; what lies beyond the matrix arrives as zeros).
+__device__ __forceinline__ void tile_copy(uint32_t dst, const CUtensorMap* map, int column, int row, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(column), "r"(row), "r"(bar) : "memory");
+}
 __device__ __forceinline__ void products_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -184,10 +192,6 @@ __device__ __forceinline__ void product_f16(bool one, uint32_t d, uint32_t a, ui
 __device__ __forceinline__ void operand16(uint32_t address, const uint32_t (&v)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
                "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
-}
-template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
-  if (N == 16) asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
 }
 __device__ __forceinline__ void accumulators32(uint32_t address, uint32_t (&v)[32]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -204,36 +208,23 @@ __device__ __forceinline__ uint32_t picked(const uint32_t (&v)[32], int j) {
   return r;
 }
 
-// The tiles and steps of a block in the order they are taken: passes of per_pass tiles, in a pass the steps, in a step the tiles.
-struct Walk4 {
-  int first, last, end, per_pass, steps;     // the pass' tiles [first, last)
-  int tile, step;
-  __device__ __forceinline__ Walk4(int begin, int end_, int per_pass_, int steps_)
-      : first(begin), last(min(begin + per_pass_, end_)), end(end_), per_pass(per_pass_), steps(steps_), tile(begin), step(0) {}
-  __device__ __forceinline__ bool more() const { return first < end; }
-  __device__ __forceinline__ void skip(int n) {
-    tile += n;
-    while (tile >= last && first < end) {
-      if (++step < steps) { tile -= last - first; continue; }
-      step = 0; first = last; last = min(first + per_pass, end);
-    }
-  }
-};
-
-static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kernel(Batch4Dev P) {
+// A block takes its tiles in passes of per_pass, in a pass the steps of 256 columns, in a step the tiles. These (step, tile) are numbered through: number i has place i % code_slots for its
+// codes and pair i % 2 of the operands in the making.
+static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap scale_map, Batch4Dev P) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_address(smem_raw) & 1023u)) & 1023u);
-  unsigned char* xs = smem;                                                 // x: x_stages steps
   const int x_bytes = batch4_x_stage_bytes(P.n);
-  unsigned char* cs = xs + P.x_stages * x_bytes;                             // codes and scales: [warp][ahead]
-  float* factor = reinterpret_cast<float*>(cs + P.ahead * kB4DequantWarps * kB4WarpBytes);     // [n] g * 2^-shift
+  unsigned char* cs = smem;                                                 // codes, in the 128-byte swizzle: code_slots tiles of a step
+  unsigned char* xs = cs + P.code_slots * kB4CodeBytes;                      // x: x_stages times 64 columns
+  unsigned char* ss = xs + P.x_stages * x_bytes;                             // scales: code_slots times [128 rows][16 bytes]
+  float* factor = reinterpret_cast<float*>(ss + P.code_slots * (kB4SlotBytes - kB4CodeBytes));    // [n] g * 2^-shift
   uint64_t* bars = reinterpret_cast<uint64_t*>(factor + kB4MaxN);
-  uint32_t* words = reinterpret_cast<uint32_t*>(bars + 2 * kB4Groups + 2 * kB4MaxXStages + 2 * kB4MaxSums + 1);     // [0] tensor memory, [1] given up
+  uint32_t* words = reinterpret_cast<uint32_t*>(bars + 2 * (kB4Pairs + kB4MaxXStages + kB4MaxSums + kB4MaxCodeSlots) + 1);     // [0] tensor memory, [1] given up
   volatile uint32_t* given_up = words + 1;
-  const uint32_t w_full = smem_address(bars), w_empty = w_full + 8 * kB4Groups, x_full = w_empty + 8 * kB4Groups, x_empty = x_full + 8 * kB4MaxXStages, acc_full = x_empty + 8 * kB4MaxXStages,
-                 acc_empty = acc_full + 8 * kB4MaxSums, drained = acc_empty + 8 * kB4MaxSums;
+  const uint32_t w_full = smem_address(bars), w_empty = w_full + 8 * kB4Pairs, x_full = w_empty + 8 * kB4Pairs, x_empty = x_full + 8 * kB4MaxXStages, acc_full = x_empty + 8 * kB4MaxXStages,
+                 acc_empty = acc_full + 8 * kB4MaxSums, c_full = acc_empty + 8 * kB4MaxSums, c_empty = c_full + 8 * kB4MaxCodeSlots, drained = c_empty + 8 * kB4MaxCodeSlots;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int H = P.hidden, steps = (H + kB4Cols - 1) / kB4Cols;
+  const int H = P.hidden, steps = (H + kB4StepCols - 1) / kB4StepCols;
   const int n_tiles = (P.vocab + kB4Tile - 1) / kB4Tile;
   const int begin = static_cast<int>(static_cast<long long>(blockIdx.x) * n_tiles / gridDim.x), end = static_cast<int>(static_cast<long long>(blockIdx.x + 1) * n_tiles / gridDim.x);
   if (warp == kB4MmaWarp) {
@@ -241,9 +232,10 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 0) {
-    for (int s = 0; s < kB4Groups; s++) { barrier_init(w_full + 8 * s, 4); barrier_init(w_empty + 8 * s, 1); }
+    for (int s = 0; s < kB4Pairs; s++) { barrier_init(w_full + 8 * s, 8); barrier_init(w_empty + 8 * s, 1); }
     for (int s = 0; s < kB4MaxXStages; s++) { barrier_init(x_full + 8 * s, 1); barrier_init(x_empty + 8 * s, 1); }
     for (int s = 0; s < kB4MaxSums; s++) { barrier_init(acc_full + 8 * s, 1); barrier_init(acc_empty + 8 * s, kB4DoneWarps); }
+    for (int s = 0; s < kB4MaxCodeSlots; s++) { barrier_init(c_full + 8 * s, 1); barrier_init(c_empty + 8 * s, 8); }
     barrier_init(drained, 1);
     words[1] = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -262,67 +254,42 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
   const uint32_t tmem = words[0];
 
   if (warp < kB4DequantWarps) {
-    // ---- W: a group of 4 warps has a tile, a lane a row of it (a lane of tensor memory). Codes come by asynchronous copies, four lanes to a row; the 16-byte piece q of row r lies at
-    // 64 r + 16 (q ^ (r / 2 mod 4)), so that 8 lanes reading their rows' piece meet different banks.
-    const int group = warp >> 2, quarter = warp & 3, r8 = lane >> 2, q = lane & 3;
-    unsigned char* mine = cs + warp * P.ahead * kB4WarpBytes;
-    const uint32_t to = smem_address(mine);
-    const uint32_t piece = static_cast<uint32_t>(r8 * 64 + ((q ^ ((r8 >> 1) & 3)) << 4));
-    const uint32_t codes_stride = static_cast<uint32_t>(P.codes_stride), scales_stride = static_cast<uint32_t>(P.scales_stride), last_row = static_cast<uint32_t>(P.vocab - 1);
-    const bool pairs = ((reinterpret_cast<uintptr_t>(P.scales) | scales_stride) & 7u) == 0;
-    Walk4 load(begin, end, P.per_pass, steps);
-    load.skip(group);
-    Walk4 use = load;
-    int slot = 0;
-    auto fetch = [&]() {                                                     // the next tile's columns of a step into the next slot
-      if (load.more()) {
-        const int row = load.tile * kB4Tile + 32 * quarter, k = load.step * kB4Cols;
-        const uint32_t at = to + slot * kB4WarpBytes;
-        if (k + q * 32 < H) {                                                // (the last step may have 64 columns only)
+    // ---- W: 4 warps make an operand, a lane a row of it (a lane of tensor memory), 8 warps a tile's two. The codes' 16-byte pieces are swizzled: 8 lanes reading their rows' piece
+    // meet different banks.
+    const int pair = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, in_tile = 32 * quarter + lane;
+    const unsigned char *code_row = cs + in_tile * 128, *scale_row = ss + in_tile * 16 + half * 8;
+    const uint32_t operand = tmem + kB4SumColumns + static_cast<uint32_t>((2 * pair + half) * kB4OperandColumns) + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t full = w_full + 8 * pair, empty = w_empty + 8 * pair;
+    int piece[4];
 #pragma unroll
-          for (int u = 0; u < 4; u++) {
-            const uint32_t v = min(static_cast<uint32_t>(row + 8 * u + r8), last_row);           // (rows beyond the vocabulary: the last one again, never stored)
-            copy_async<16>(at + piece + u * 512, P.codes + static_cast<uint64_t>(v) * codes_stride + (k >> 1) + q * 16);
-          }
-        }
-        const uint8_t* from = P.scales + static_cast<uint64_t>(min(static_cast<uint32_t>(row + lane), last_row)) * scales_stride + (k >> 4);
-        const uint32_t sa = at + 2048 + lane * 8;
-        if (k + 64 < H && pairs) copy_async<8>(sa, from);
-        else { copy_async<4>(sa, from); if (k + 64 < H) copy_async<4>(sa + 4, from + 4); }
-        load.skip(kB4Groups);
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (++slot == P.ahead) slot = 0;
-    };
-    for (int d = 0; d < P.ahead - 1; d++) fetch();
-    const uint32_t operand = tmem + kB4SumColumns + static_cast<uint32_t>(group * kB4OperandColumns) + (static_cast<uint32_t>(quarter * 32) << 16);
-    uint32_t phase = 1u;
-    int from = 0;
-    bool go = true;
-    for (; go && use.more(); use.skip(kB4Groups)) {
-      if (P.ahead == 4) asm volatile("cp.async.wait_group 2;" ::: "memory");
-      else if (P.ahead == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    for (int i = 0; i < 4; i++) piece[i] = ((half * 4 + i) ^ (lane & 7)) << 4;
+    uint32_t phase = 1u, slot_phase = 0u;
+    int slot = pair;
+    if (slot >= P.code_slots) { slot -= P.code_slots; slot_phase = 1u; }
+    for (int left = (end - begin) * steps - pair; left > 0; left -= 2) {       // (which tile and step: the copies know)
+      bool go = barrier_wait(c_full + 8 * slot, slot_phase, given_up);
+      uint4 cc[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) cc[i] = *reinterpret_cast<const uint4*>(code_row + slot * kB4CodeBytes + piece[i]);
+      const uint2 sc = *reinterpret_cast<const uint2*>(scale_row + slot * (kB4SlotBytes - kB4CodeBytes));
       __syncwarp();
-      fetch();
-      const unsigned char* row = mine + from * kB4WarpBytes + lane * 64;
-      const uint2 sc = *reinterpret_cast<const uint2*>(mine + from * kB4WarpBytes + 2048 + lane * 8);
-      if (++from == P.ahead) from = 0;
-      go = __all_sync(kFull, barrier_wait(w_empty + 8 * group, phase, given_up));
+      if (lane == 0) barrier_arrive(c_empty + 8 * slot);
+      slot += 2;
+      if (slot >= P.code_slots) { slot -= P.code_slots; slot_phase ^= 1u; }
+      go = __all_sync(kFull, go && barrier_wait(empty, phase, given_up));
       phase ^= 1u;
       if (!go) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
       for (int i = 0; i < 4; i++) {                                          // 32 columns
-        const uint4 cc = *reinterpret_cast<const uint4*>(row + ((i ^ ((lane >> 1) & 3)) << 4));
-        const uint32_t pair = e4m3_to_f16((i < 2 ? sc.x : sc.y) >> (16 * (i & 1)));
-        const uint32_t w[4] = {cc.x, cc.y, cc.z, cc.w};
+        const uint32_t two = e4m3_to_f16((i < 2 ? sc.x : sc.y) >> (16 * (i & 1)));
+        const uint32_t w[4] = {cc[i].x, cc[i].y, cc[i].z, cc[i].w};
         uint32_t v[16];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           uint32_t h[4];
           e2m1_to_f16(w[j], h);
-          const uint32_t s = __byte_perm(pair, 0u, j < 2 ? 0x1010 : 0x3232);
+          const uint32_t s = __byte_perm(two, 0u, j < 2 ? 0x1010 : 0x3232);
 #pragma unroll
           for (int e = 0; e < 4; e++) v[4 * j + e] = f16x2_mul(h[e], s);
         }
@@ -331,40 +298,53 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) barrier_arrive(w_full + 8 * group);
+      if (lane == 0) barrier_arrive(full);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else if (warp == kB4MmaWarp) {
     // (the whole warp walks, and one lane issues: its operands are then uniform values. A single lane's walk took 1300 clocks a tile.)
     const uint32_t form = (1u << 4) | (static_cast<uint32_t>(P.n >> 3) << 17) | (static_cast<uint32_t>(kB4Tile >> 4) << 24);   // binary16 operands, FP32 accumulators
     const bool one = elected();
-    int group = 0, xs_ = 0;
+    const uint32_t operands = tmem + kB4SumColumns;
+    int pair = 0, x0 = 0;
     uint32_t wp = 0u, xp = 0u, ap = 1u;
     bool go = true;
     for (int first = begin; go && first < end; first += P.per_pass, ap ^= 1u) {
       const int count = min(P.per_pass, end - first);
-      for (int step = 0; go && step < steps; step++) {
-        go = barrier_wait(x_full + 8 * xs_, xp, given_up);
-        const uint64_t b = operand(smem_address(xs) + xs_ * x_bytes), b2 = b + static_cast<uint64_t>(P.n * 8);      // (64 columns on: n * 128 bytes)
-        const bool both = H - step * kB4Cols > 64, last = step == steps - 1;
-        for (int sum = 0; go && sum < count; sum++) {
-          if (step == 0) go = barrier_wait(acc_empty + 8 * sum, ap, given_up);             // (the first pass finds them empty)
-          go = go && barrier_wait(w_full + 8 * group, wp, given_up);
-          if (!go) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t d = tmem + static_cast<uint32_t>(sum * P.column_stride), a = tmem + kB4SumColumns + static_cast<uint32_t>(group * kB4OperandColumns);
+      for (int k0 = 0; go && k0 < H; k0 += kB4StepCols) {
+        const int quarters = min(4, (H - k0) / kB4XCols);
+        const bool last = k0 + kB4StepCols >= H;
+        uint64_t b[4];                                                       // the step's places of x
+        uint32_t x_bar[4], x_par[4];
 #pragma unroll
-          for (int k = 0; k < 4; k++) product_f16(one, d, a + 8 * k, b + 2 * k, form, k > 0 ? 1u : static_cast<uint32_t>(step));
-          if (both) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) product_f16(one, d, a + 32 + 8 * k, b2 + 2 * k, form, 1u);
-          }
-          if (one) products_commit(w_empty + 8 * group);
-          if (last && one) products_commit(acc_full + 8 * sum);
-          if (++group == kB4Groups) { group = 0; wp ^= 1u; }
+        for (int q = 0; q < 4; q++) {
+          const int x = x0 + q < P.x_stages ? x0 + q : x0 + q - P.x_stages;
+          b[q] = operand(smem_address(xs) + x * x_bytes); x_bar[q] = x_full + 8 * x; x_par[q] = x0 + q < P.x_stages ? xp : xp ^ 1u;
         }
-        if (one) products_commit(x_empty + 8 * xs_);
-        if (++xs_ == P.x_stages) { xs_ = 0; xp ^= 1u; }
+        uint32_t d = tmem;
+        for (int sum = 0; go && sum < count; sum++, d += static_cast<uint32_t>(P.column_stride)) {
+          if (k0 == 0) go = barrier_wait(acc_empty + 8 * sum, ap, given_up);               // (the first pass finds them empty)
+          go = go && barrier_wait(w_full + 8 * pair, wp, given_up);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t a = operands + static_cast<uint32_t>(pair * 2 * kB4OperandColumns);
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            if (q < quarters) {
+              if (sum == 0) go = go && barrier_wait(x_bar[q], x_par[q], given_up);
+              if (!go) break;
+#pragma unroll
+              for (int k = 0; k < 4; k++) product_f16(one, d, a + 32 * q + 8 * k, b[q] + 2 * k, form, q + k > 0 ? 1u : static_cast<uint32_t>(k0));
+              if (one && sum == count - 1) products_commit(x_bar[q] + 8 * kB4MaxXStages);   // (x_empty)
+            }
+          }
+          if (one) {
+            products_commit(w_empty + 8 * pair);
+            if (last) products_commit(acc_full + 8 * sum);
+          }
+          pair ^= 1;
+          wp ^= pair == 0 ? 1u : 0u;
+        }
+        x0 += quarters;
+        if (x0 >= P.x_stages) { x0 -= P.x_stages; xp ^= 1u; }
       }
     }
     if (!go && one) {                                                       // what is under way ends before the block does
@@ -376,12 +356,11 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
       int stage = 0, issued = 0; uint32_t phase = 0u;
       bool go = true;
       for (int first = begin; go && first < end; first += P.per_pass) {
-        for (int step = 0; step < steps; step++) {
+        for (int k = 0; k < H / kB4XCols; k++) {
           go = barrier_wait(x_empty + 8 * stage, phase ^ 1u, given_up);
           if (!go) break;
-          const uint32_t bytes = static_cast<uint32_t>(min(2, (H - step * kB4Cols) / 64) * P.n * 128);
-          barrier_expect(x_full + 8 * stage, bytes);
-          bulk_copy(smem_address(xs) + stage * x_bytes, P.xt + static_cast<size_t>(step) * x_bytes, bytes, x_full + 8 * stage);
+          barrier_expect(x_full + 8 * stage, static_cast<uint32_t>(x_bytes));
+          bulk_copy(smem_address(xs) + stage * x_bytes, P.xt + static_cast<size_t>(k) * x_bytes, static_cast<uint32_t>(x_bytes), x_full + 8 * stage);
           issued++;
           if (++stage == P.x_stages) { stage = 0; phase ^= 1u; }
         }
@@ -391,6 +370,33 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
           if (stage == 0) { stage = P.x_stages; phase ^= 1u; }
           stage--;
           for (uint32_t i = 0; i < kB4WaitLimit && !barrier_try(x_full + 8 * stage, phase); i++) {}
+        }
+    }
+  } else if (warp == kB4CodeWarp) {
+    if (lane == 0) {
+      bool go = true;
+      int issued = 0, slot = 0;
+      uint32_t phase = 0u;
+      for (int first = begin; go && first < end; first += P.per_pass) {
+        const int last = min(first + P.per_pass, end);
+        for (int step = 0; go && step < steps; step++) {
+          for (int tile = first; tile < last; tile++) {
+            const uint32_t bar = c_full + 8 * slot;
+            go = barrier_wait(c_empty + 8 * slot, phase ^ 1u, given_up);
+            if (!go) break;
+            barrier_expect(bar, kB4SlotBytes);
+            tile_copy(smem_address(cs) + slot * kB4CodeBytes, &code_map, step * (kB4StepCols / 2), tile * kB4Tile, bar);
+            tile_copy(smem_address(ss) + slot * (kB4SlotBytes - kB4CodeBytes), &scale_map, step * (kB4StepCols / kFp4Block), tile * kB4Tile, bar);
+            issued++;
+            if (++slot == P.code_slots) { slot = 0; phase ^= 1u; }
+          }
+        }
+      }
+      if (!go)                                                              // the copies under way
+        for (int k = 0; k < P.code_slots && k < issued; k++) {
+          if (slot == 0) { slot = P.code_slots; phase ^= 1u; }
+          slot--;
+          for (uint32_t i = 0; i < kB4WaitLimit && !barrier_try(c_full + 8 * slot, phase); i++) {}
         }
     }
   } else {

@@ -1,6 +1,9 @@
 // C ABI of the operators between the projection and the sampler: the microscaled 4-bit weight, the projection with it, and the logits' processing. As in
 // lithos_b200.cu: argument checks, launch geometry, kernel launches; no allocation, no synchronisation.
+#include <cuda.h>
 #include <cuda_runtime.h>
+
+#include <atomic>
 
 #include "common.cuh"
 #include "host.cuh"
@@ -80,6 +83,27 @@ size_t lm_head_nvfp4_workspace_bytes(int64_t rows, int64_t hidden_dim) {
   return batch4_workspace_bytes(rows, hidden_dim);
 }
 
+// A matrix of bytes that the copy engine reads in boxes of 128 rows by `width` bytes.
+static int byte_map(const uint8_t* p, int64_t rows, int64_t bytes, int64_t stride, uint32_t width, CUtensorMapSwizzle swizzle, CUtensorMap* map) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<Encode> known{nullptr};
+  Encode encode = known.load(std::memory_order_relaxed);
+  if (!encode) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found);
+    if (e != cudaSuccess) return cuda_fail(e);
+    if (found != cudaDriverEntryPointSuccess || !f) return cuda_fail(cudaErrorSymbolNotFound);
+    known.store(encode = reinterpret_cast<Encode>(f), std::memory_order_relaxed);
+  }
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(bytes), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(stride)};
+  const cuuint32_t box[2] = {width, kB4Tile}, steps[2] = {1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(p), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? LM_OK : cuda_fail(cudaErrorInvalidValue);
+}
+
 // More rows than a decode step has: the rows of x prepared once, then one launch for every 256 of them.
 static int head_nvfp4_batch(const lm_head_nvfp4_args* a, int sms) {
   if (!a->workspace || misaligned(a->workspace, 256) || a->workspace_bytes < batch4_workspace_bytes(a->rows, a->hidden_dim)) return LM_E_WORKSPACE;
@@ -100,6 +124,10 @@ static int head_nvfp4_batch(const lm_head_nvfp4_args* a, int sms) {
   P.hidden = R.hidden; P.vocab = static_cast<int>(a->vocab); P.logits_stride = a->logits_stride;
   rc = ensure_dynamic_smem(kSlotHeadNvfp4Batch, reinterpret_cast<const void*>(lm_head_nvfp4_batch_kernel), kB4SmemLimit);
   if (rc != LM_OK) return rc;
+  CUtensorMap code_map, scale_map;
+  rc = byte_map(a->codes, P.vocab, P.hidden / 2, a->codes_stride, kB4StepCols / 2, CU_TENSOR_MAP_SWIZZLE_128B, &code_map);
+  if (rc == LM_OK) rc = byte_map(a->scales, P.vocab, P.hidden / kFp4Block, a->scales_stride, kB4StepCols / kFp4Block, CU_TENSOR_MAP_SWIZZLE_NONE, &scale_map);
+  if (rc != LM_OK) return rc;
   const int tiles = (P.vocab + kB4Tile - 1) / kB4Tile;
   for (int64_t r = 0; r < a->rows; r += kB4MaxN) {
     P.rows = static_cast<int>(a->rows - r < kB4MaxN ? a->rows - r : kB4MaxN);
@@ -108,10 +136,12 @@ static int head_nvfp4_batch(const lm_head_nvfp4_args* a, int sms) {
     P.logits = static_cast<uint16_t*>(a->logits) + r * a->logits_stride;
     P.column_stride = P.n <= 32 ? 32 : P.n <= 64 ? 64 : P.n <= 128 ? 128 : 256;
     P.per_pass = kB4SumColumns / P.column_stride;
-    P.x_stages = P.n <= 96 ? 3 : 2;                                         // steps of x in shared memory, and as many tiles of codes as fit beside them
-    P.ahead = kB4Ahead;
-    while (batch4_smem_bytes(P.n, P.ahead, P.x_stages) > kB4SmemLimit) P.ahead--;
-    rc = launch_stream(true, lm_head_nvfp4_batch_kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), kB4Threads, batch4_smem_bytes(P.n, P.ahead, P.x_stages), 1, st, P);
+    // of x eight pieces in shared memory (a step's four and the next's, where tiles share them) or as many as fit beside three tiles of codes, and as many of these as fit then
+    P.x_stages = static_cast<int>((kB4SmemLimit - batch4_smem_bytes(P.n, 3, 0)) / static_cast<size_t>(batch4_x_stage_bytes(P.n)));
+    if (P.x_stages > kB4MaxXStages) P.x_stages = kB4MaxXStages;
+    P.code_slots = kB4MaxCodeSlots;
+    while (batch4_smem_bytes(P.n, P.code_slots, P.x_stages) > kB4SmemLimit) P.code_slots--;
+    rc = launch_stream(true, lm_head_nvfp4_batch_kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), kB4Threads, batch4_smem_bytes(P.n, P.code_slots, P.x_stages), 1, st, code_map, scale_map, P);
     if (rc != LM_OK) return rc;
   }
   return LM_OK;
@@ -126,7 +156,7 @@ int lm_head_nvfp4(const lm_head_nvfp4_args* a) {
   if (rc != LM_OK) return rc;
   if (a->rows > LM_HEAD_NVFP4_MAX_ROWS || a->vocab > LM_MAX_VOCAB || (a->hidden_dim % 64) != 0 || a->hidden_dim > kH4MaxHidden) return LM_E_UNSUPPORTED;
   if (a->codes_stride > 0x7FFFFFFF || a->scales_stride > 0x7FFFFFFF) return LM_E_UNSUPPORTED;
-  if (misaligned(a->codes, 16) || (a->codes_stride % 16) != 0 || misaligned(a->scales, 4) || (a->scales_stride % 4) != 0) return LM_E_UNSUPPORTED;   // 16- and 4-byte loads
+  if (misaligned(a->codes, 16) || (a->codes_stride % 16) != 0 || misaligned(a->scales, 16) || (a->scales_stride % 16) != 0) return LM_E_UNSUPPORTED;   // 16-byte copies
   Head4Dev P;
   P.x_stride = a->hidden_stride;
   P.codes = a->codes; P.codes_stride = a->codes_stride; P.scales = a->scales; P.scales_stride = a->scales_stride; P.scale = a->scale;

@@ -15,10 +15,15 @@ from .sampler import _dtype_code, _row_stride
 BLOCK = 16                               # columns that share a scale
 
 
+def _padded_scales(rows: int, blocks: int, device: torch.device) -> torch.Tensor:
+    """uint8 [rows, blocks] whose rows start at multiples of 16 bytes."""
+    return torch.empty(rows, (blocks + 15) // 16 * 16, dtype=torch.uint8, device=device)[:, :blocks]
+
+
 class Nvfp4Weight:
     """A matrix [rows, cols] in the 4-bit format: ``codes`` uint8 [rows, cols / 2] (the even column in the low nibble), ``scales`` float8_e4m3fn (or
     uint8, the same bytes) [rows, cols / 16], ``scale`` float32 with one element; CUDA tensors on one device, unit stride along a row. Element (r, c) is
-    e2m1(code) * scales[r, c // 16] * scale. A slice of rows, ``weight[lo:hi]``, is a view (a shard of a vocabulary)."""
+    e2m1(code) * scales[r, c // 16] * scale. (Scales whose rows do not start at multiples of 16 bytes are copied once, to rows padded to that.) A slice of rows, ``weight[lo:hi]``, is a view (a shard of a vocabulary)."""
 
     __slots__ = ("codes", "scales", "scale")
 
@@ -35,7 +40,10 @@ class Nvfp4Weight:
             raise ValueError("Nvfp4Weight: tensors on one device")
         if (codes.shape[1] > 1 and codes.stride(1) != 1) or (scales.shape[1] > 1 and scales.stride(1) != 1):
             raise ValueError("Nvfp4Weight: the rows must be contiguous")
-        self.codes, self.scales, self.scale = codes, scales.view(torch.uint8), scale
+        scales = scales.view(torch.uint8)
+        if scales.numel() and (scales.data_ptr() % 16 or (scales.shape[0] > 1 and scales.stride(0) % 16)):
+            scales = _padded_scales(*scales.shape, scales.device).copy_(scales)
+        self.codes, self.scales, self.scale = codes, scales, scale
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -84,7 +92,7 @@ def quantize_nvfp4(x: torch.Tensor, scale: Optional[torch.Tensor] = None) -> Nvf
         x = x.contiguous()
     with torch.cuda.device(x.device):
         codes = torch.empty(rows, cols // 2, dtype=torch.uint8, device=x.device)
-        scales = torch.empty(rows, cols // BLOCK, dtype=torch.uint8, device=x.device)
+        scales = _padded_scales(rows, cols // BLOCK, x.device)
         a = _lib.QuantizeNvfp4Args()
         a.struct_size = C.sizeof(a)
         if scale is None:
