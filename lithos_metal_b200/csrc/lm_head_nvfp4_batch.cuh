@@ -158,14 +158,17 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   return done != 0u;
 }
-// False when the limit ran out here or the block has given up.
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile uint32_t* given_up) {
+// False when the limit ran out here or the block has given up. (Out of line: the usual wait is over at the first or second look, and the roles' loops have to stay short.)
+__device__ __noinline__ bool barrier_wait_long(uint32_t bar, uint32_t parity, volatile uint32_t* given_up) {
   for (uint32_t i = 0; i < kB4WaitLimit; i++) {
     if (barrier_try(bar, parity)) return true;
     if ((i & 15u) == 15u && *given_up) return false;
   }
   *given_up = 1u;
   return false;
+}
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile uint32_t* given_up) {
+  return barrier_try(bar, parity) || barrier_wait_long(bar, parity, given_up);
 }
 __device__ __forceinline__ bool elected() {                                 // true in one lane of a warp that is together, always the same
   uint32_t p;
@@ -186,8 +189,8 @@ __device__ __forceinline__ void products_commit(uint32_t bar) {
 __device__ __forceinline__ uint64_t operand(uint32_t address) {
   return static_cast<uint64_t>((address >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ void product_f16(bool one, uint32_t d, uint32_t a, uint64_t b, uint32_t form, uint32_t add) {     // a: in tensor memory
-  if (one) asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(form), "r"(add) : "memory");
+__device__ __forceinline__ void product_f16(uint32_t d, uint32_t a, uint64_t b, uint32_t form, uint32_t add) {     // a: in tensor memory
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(form), "r"(add) : "memory");
 }
 __device__ __forceinline__ void operand16(uint32_t address, const uint32_t (&v)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
@@ -267,7 +270,7 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     int slot = pair;
     if (slot >= P.code_slots) { slot -= P.code_slots; slot_phase = 1u; }
     for (int left = (end - begin) * steps - pair; left > 0; left -= 2) {       // (which tile and step: the copies know)
-      bool go = barrier_wait(c_full + 8 * slot, slot_phase, given_up);
+      barrier_wait(c_full + 8 * slot, slot_phase, given_up);                 // (where a wait has run out, what follows is harmless and the block writes NaN)
       uint4 cc[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) cc[i] = *reinterpret_cast<const uint4*>(code_row + slot * kB4CodeBytes + piece[i]);
@@ -276,9 +279,9 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
       if (lane == 0) barrier_arrive(c_empty + 8 * slot);
       slot += 2;
       if (slot >= P.code_slots) { slot -= P.code_slots; slot_phase ^= 1u; }
-      go = __all_sync(kFull, go && barrier_wait(empty, phase, given_up));
+      barrier_wait(empty, phase, given_up);
       phase ^= 1u;
-      if (!go) break;
+      __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
       for (int i = 0; i < 4; i++) {                                          // 32 columns
@@ -304,13 +307,12 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     // (the whole warp walks, and one lane issues: its operands are then uniform values. A single lane's walk took 1300 clocks a tile.)
     const uint32_t form = (1u << 4) | (static_cast<uint32_t>(P.n >> 3) << 17) | (static_cast<uint32_t>(kB4Tile >> 4) << 24);   // binary16 operands, FP32 accumulators
     const bool one = elected();
-    const uint32_t operands = tmem + kB4SumColumns;
-    int pair = 0, x0 = 0;
-    uint32_t wp = 0u, xp = 0u, ap = 1u;
-    bool go = true;
-    for (int first = begin; go && first < end; first += P.per_pass, ap ^= 1u) {
+    int x0 = 0;
+    uint32_t a = tmem + kB4SumColumns, w_bar = w_full, wp = 0u, xp = 0u, ap = 1u;
+    const uint32_t other_a = a ^ (a + 2 * kB4OperandColumns), other_bar = w_full ^ (w_full + 8);    // (the two pairs in turn)
+    for (int first = begin; first < end; first += P.per_pass, ap ^= 1u) {
       const int count = min(P.per_pass, end - first);
-      for (int k0 = 0; go && k0 < H; k0 += kB4StepCols) {
+      for (int k0 = 0; k0 < H; k0 += kB4StepCols) {
         const int quarters = min(4, (H - k0) / kB4XCols);
         const bool last = k0 + kB4StepCols >= H;
         uint64_t b[4];                                                       // the step's places of x
@@ -321,33 +323,44 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
           b[q] = operand(smem_address(xs) + x * x_bytes); x_bar[q] = x_full + 8 * x; x_par[q] = x0 + q < P.x_stages ? xp : xp ^ 1u;
         }
         uint32_t d = tmem;
-        for (int sum = 0; go && sum < count; sum++, d += static_cast<uint32_t>(P.column_stride)) {
-          if (k0 == 0) go = barrier_wait(acc_empty + 8 * sum, ap, given_up);               // (the first pass finds them empty)
-          go = go && barrier_wait(w_full + 8 * pair, wp, given_up);
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t a = operands + static_cast<uint32_t>(pair * 2 * kB4OperandColumns);
+        for (int sum = 0; sum < count; sum++, d += static_cast<uint32_t>(P.column_stride)) {
+          if (k0 == 0) barrier_wait(acc_empty + 8 * sum, ap, given_up);                    // (the first pass finds them empty)
+          barrier_wait(w_bar, wp, given_up);
+          if (sum == 0 || sum == count - 1 || quarters < 4) {                // x arrives, or leaves
 #pragma unroll
-          for (int q = 0; q < 4; q++) {
-            if (q < quarters) {
-              if (sum == 0) go = go && barrier_wait(x_bar[q], x_par[q], given_up);
-              if (!go) break;
+            for (int q = 0; q < 4; q++) {
+              if (q < quarters) {
+                if (sum == 0) barrier_wait(x_bar[q], x_par[q], given_up);
+                __syncwarp();
+                if (one) {
+                  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-              for (int k = 0; k < 4; k++) product_f16(one, d, a + 32 * q + 8 * k, b[q] + 2 * k, form, q + k > 0 ? 1u : static_cast<uint32_t>(k0));
-              if (one && sum == count - 1) products_commit(x_bar[q] + 8 * kB4MaxXStages);   // (x_empty)
+                  for (int k = 0; k < 4; k++) product_f16(d, a + 32 * q + 8 * k, b[q] + 2 * k, form, q + k > 0 ? 1u : static_cast<uint32_t>(k0));
+                  if (sum == count - 1) products_commit(x_bar[q] + 8 * kB4MaxXStages);     // (x_empty)
+                }
+              }
+            }
+          } else if (one) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+#pragma unroll
+              for (int k = 0; k < 4; k++) product_f16(d, a + 32 * q + 8 * k, b[q] + 2 * k, form, q + k > 0 ? 1u : static_cast<uint32_t>(k0));
             }
           }
           if (one) {
-            products_commit(w_empty + 8 * pair);
+            products_commit(w_bar + 8 * kB4Pairs);                           // (w_empty)
             if (last) products_commit(acc_full + 8 * sum);
           }
-          pair ^= 1;
-          wp ^= pair == 0 ? 1u : 0u;
+          __syncwarp();
+          a ^= other_a; w_bar ^= other_bar;
+          wp ^= w_bar == w_full ? 1u : 0u;
         }
         x0 += quarters;
         if (x0 >= P.x_stages) { x0 -= P.x_stages; xp ^= 1u; }
       }
     }
-    if (!go && one) {                                                       // what is under way ends before the block does
+    if (*given_up && one) {                                                 // what is under way ends before the block does
       products_commit(drained);
       for (uint32_t i = 0; i < kB4WaitLimit && !barrier_try(drained, 0u); i++) {}
     }
