@@ -38,7 +38,8 @@ enum KernelSlot { kSlotFast, kSlotTopk, kSlotTopkOrdered, kSlotGeneric, kSlotVoc
                   kSlotDraftQ = kSlotArgmax + 2,    // (two instances)
                   kSlotVerify = kSlotDraftQ + 2,    // (twelve)
                   kSlotVerifyGiven = kSlotVerify + 12,   // (four)
-                  kSlotHeadNvfp4 = kSlotVerifyGiven + 4, kSlotHeadNvfp4Batch, kSlotLogits, kSlotLogitsF32,
+                  kSlotHeadNvfp4 = kSlotVerifyGiven + 4,     // (four)
+                  kSlotHeadNvfp4Batch = kSlotHeadNvfp4 + 4, kSlotLogits, kSlotLogitsF32,
                   kSlotCount };
 
 inline int ensure_dynamic_smem(KernelSlot slot, const void* func, size_t bytes, bool large_clusters = false) {

@@ -1,28 +1,32 @@
 // The vocabulary projection of a decode step with a 4-bit weight (nvfp4.cuh): logits[t, v] = bf16(g * sum_k x[t, k] * e2m1(c[v, k]) * e4m3(s[v, k / 16])),
-// FP32 accumulation, for up to 8 rows, the final RMSNorm fused on the input as in lm_head.cuh (the norm's output is rounded to BF16 by definition).
+// FP32 accumulation, for up to 8 NT rows (NT of 1 to 4), the final RMSNorm fused on the input as in lm_head.cuh (the norm's output is rounded to BF16 by definition).
 //
 // The weight is read once: 0.5625 bytes an element instead of 2 (350 MB for 151,936 x 4096: 53 us at the measured copy rate), so an SM has to take in
 // some 43 weights a clock. A code becomes binary16 by the conversion instruction (two codes each), times its block's scale by one packed multiplication:
 // exact, since e2m1 * e4m3 has 6 significant bits. The products and sums are those of mma.sync m16n8k16 (binary16 in, FP32 accumulate), 16 vocabulary rows to a
-// warp; measured alone, conversion, scale and mma together take in 57 weights a clock and SM, bit operations in the place of the conversion 34.
+// warp; measured alone, conversion, scale and mma together take in 57 weights a clock and SM, bit operations in the place of the conversion 34. (The operands go from registers to the
+// mma: on tcgen05 they pass through shared or tensor memory, which costs more than the products of so few rows: lm_head_nvfp4_batch.cuh.) A warp's loads run ahead in registers.
 //
 // x is BF16 and the mma wants binary16 on both sides. A row of x is multiplied by the power of two that brings its largest magnitude to 2^14 .. 2^15 (taken out
 // again behind the sum); BF16 values down to 2^-31 of the largest are then exact in binary16, subnormals included. Where some x is not (or is infinite or NaN),
 // every block sees it and takes the rows the slow way, in FP64 on the CUDA cores, whose range holds every product.
+//
+// A row's sum is (q0 + q1) + (q2 + q3) over four quarters of the hidden dimension, each in order: the same additions whether a warp walks the whole row or, for the tiles left over after
+// the last full round, four warps take a quarter each.
 #pragma once
 #include "common.cuh"
 #include "nvfp4.cuh"
 
 namespace lm {
 
-constexpr int kH4Threads = 256;
+constexpr int kH4Threads = 512;
 constexpr int kH4Warps = kH4Threads / 32;
-constexpr int kH4Rows = 8;                   // rows of x (the n dimension of the mma)
+constexpr int kH4Rows = 8;                   // rows of x to an mma (its n dimension)
+constexpr int kH4MaxNT = 4;
 constexpr int kH4Tile = 16;                  // vocabulary rows per warp tile (the m dimension)
 constexpr int kH4Step = 256;                 // columns per step: 32 bytes of codes per thread and row, a whole 128-byte line per row and quad
-constexpr int kH4Unroll = 4;                 // steps whose loads are in flight together: a batch
-constexpr int kH4MaxBatches = 13;            // batches of the longest row that fits (12,736 columns)
 constexpr int kH4MaxHidden = 12736;
+constexpr int kH4MaxSteps = (kH4MaxHidden + kH4Step - 1) / kH4Step;
 
 struct Head4Dev {
   const uint16_t* x; int64_t x_stride; int rows;
@@ -36,7 +40,7 @@ struct Head4Dev {
 // threads of a quad read 64 bytes in a row; rows 64 bytes out of step with each other's banks.
 __host__ __device__ inline int head4_steps(int hidden) { return (hidden + kH4Step - 1) / kH4Step; }
 __host__ __device__ inline int head4_row_bytes(int hidden) { return head4_steps(hidden) * 512 + 64; }
-__host__ __device__ inline size_t head4_smem_bytes(int hidden) { return static_cast<size_t>(kH4Rows) * head4_row_bytes(hidden); }
+__host__ __device__ inline size_t head4_smem_bytes(int hidden, int nt) { return static_cast<size_t>(kH4Rows * nt) * head4_row_bytes(hidden); }
 __device__ __forceinline__ int head4_x_offset(int k) { return (k >> 8) * 512 + ((((k >> 3) & 7) << 2) + ((k >> 6) & 3)) * 16 + (k & 7) * 2; }
 
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -59,202 +63,265 @@ __device__ __forceinline__ float head4_finish(double sum, float g, int n) {
   return __double2float_rn(sum * static_cast<double>(g) * __hiloint2double((1023 - n) << 20, 0));
 }
 
-static __global__ void __launch_bounds__(kH4Threads, 2) lm_head_nvfp4_kernel(Head4Dev P) {
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  __shared__ float s_part[kH4Rows][kH4Warps];
-  __shared__ uint32_t s_max[kH4Rows][kH4Warps];
-  __shared__ float part[kH4MaxBatches][32][4];
+// 16 vocabulary rows' codes and scales of a step, a thread's part: 64 columns of rows g and g + 8.
+struct Piece4 { uint4 a[2], b[2]; uint32_t fa, fb; };
+
+// kAhead: steps whose loads are in registers or on the way.
+template <int NT, int kAhead>
+static __global__ void __launch_bounds__(kH4Threads, 1) lm_head_nvfp4_kernel(Head4Dev P) {
+  constexpr int kRows = kH4Rows * NT;
+  extern __shared__ __align__(16) unsigned char smem_raw[];                 // [kRows][row_bytes]
+  __shared__ union {
+    struct { float sum[kRows * kH4MaxSteps]; uint32_t top[kRows * kH4MaxSteps]; } x;       // while x is prepared
+    float part[4][3][32][4 * NT];                                           // later: quarters of the tiles left over
+  } s_u;
+  float* s_sum = s_u.x.sum;
+  uint32_t* s_top = s_u.x.top;
+  __shared__ float s_factor[kRows];                                         // 1 / rms, then g * 2^-shift
+  __shared__ int s_shift[kRows];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int H = P.hidden, row_bytes = head4_row_bytes(H), steps = head4_steps(H), padded = steps * kH4Step;
+  const int H = P.hidden, row_bytes = head4_row_bytes(H), steps = head4_steps(H);
+  const int gq = lane >> 2, t = lane & 3;
+  const int n_tiles = (P.vocab + kH4Tile - 1) / kH4Tile, all_warps = gridDim.x * kH4Warps, full = n_tiles / all_warps * all_warps;
   after_predecessor();
-  // ---- the rows of x: normalised if a norm is fused, scaled, binary16
-  float inv_rms[kH4Rows];
-  if (P.gamma) {
-    float ss[kH4Rows];
-#pragma unroll
-    for (int r = 0; r < kH4Rows; r++) ss[r] = 0.0f;
-    for (int k = tid; k < H; k += kH4Threads) {
-#pragma unroll
-      for (int r = 0; r < kH4Rows; r++) if (r < P.rows) { const float v = __uint_as_float(static_cast<uint32_t>(P.x[r * P.x_stride + k]) << 16); ss[r] = __fmaf_rn(v, v, ss[r]); }
-    }
-#pragma unroll
-    for (int r = 0; r < kH4Rows; r++) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) ss[r] += __shfl_xor_sync(kFull, ss[r], o);
-      if (lane == 0) s_part[r][warp] = ss[r];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kH4Rows; r++) {
-      float s = 0.0f;
-#pragma unroll
-      for (int q = 0; q < kH4Warps; q++) s += s_part[r][q];
-      inv_rms[r] = __frsqrt_rn(__fadd_rn(__fdiv_rn(s, static_cast<float>(H)), P.eps));
-    }
-  }
-  // column k of the rows, as the BF16 values that are multiplied
-  auto column = [&](int k, uint16_t (&x)[kH4Rows]) {
-#pragma unroll
-    for (int r = 0; r < kH4Rows; r++) x[r] = (r < P.rows && k < H) ? P.x[r * P.x_stride + k] : static_cast<uint16_t>(0u);
-    if (P.gamma && k < H) {
-      const float gm = __uint_as_float(static_cast<uint32_t>(P.gamma[k]) << 16), scale = P.one_plus ? __fadd_rn(1.0f, gm) : gm;
-#pragma unroll
-      for (int r = 0; r < kH4Rows; r++) if (r < P.rows) x[r] = f32_to_bf16(__fmul_rn(__fmul_rn(__uint_as_float(static_cast<uint32_t>(x[r]) << 16), inv_rms[r]), scale));
-    }
+  const float g = __ldg(P.scale);
+  auto fetch = [&](Piece4& p, int tile, int s) {
+    const int v0 = tile * kH4Tile + gq, k = s * kH4Step + 64 * t;
+    if (k < H) {                                                            // (H is a multiple of 64: all of a thread's 64 columns or none)
+      const int64_t ra = min(v0, P.vocab - 1), rb = min(v0 + 8, P.vocab - 1);          // (rows beyond the vocabulary: loaded again, never stored)
+      const uint8_t *ca = P.codes + ra * P.codes_stride + (k >> 1), *cb = P.codes + rb * P.codes_stride + (k >> 1);
+      p.a[0] = __ldcs(reinterpret_cast<const uint4*>(ca)); p.a[1] = __ldcs(reinterpret_cast<const uint4*>(ca) + 1);
+      p.b[0] = __ldcs(reinterpret_cast<const uint4*>(cb)); p.b[1] = __ldcs(reinterpret_cast<const uint4*>(cb) + 1);
+      p.fa = __ldg(reinterpret_cast<const uint32_t*>(P.scales + ra * P.scales_stride + (k >> 4))); p.fb = __ldg(reinterpret_cast<const uint32_t*>(P.scales + rb * P.scales_stride + (k >> 4)));
+    } else { p.a[0] = p.a[1] = p.b[0] = p.b[1] = make_uint4(0u, 0u, 0u, 0u); p.fa = p.fb = 0u; }
   };
-  uint32_t top[kH4Rows];
+  // ---- the first steps' loads; they arrive while x is prepared
+  Piece4 ring[kAhead];
+  int load_tile = blockIdx.x * kH4Warps + warp, load_step = 0;
+  auto fetch_next = [&](Piece4& p) {
+    if (load_tile >= full) return;
+    fetch(p, load_tile, load_step);
+    if (++load_step == steps) { load_step = 0; load_tile += all_warps; }
+  };
 #pragma unroll
-  for (int r = 0; r < kH4Rows; r++) top[r] = 0u;
-  for (int k = tid; k < padded; k += kH4Threads) {
-    uint16_t x[kH4Rows];
-    column(k, x);
-#pragma unroll
-    for (int r = 0; r < kH4Rows; r++) { top[r] = max(top[r], static_cast<uint32_t>(x[r]) & 0x7FFFu); *reinterpret_cast<uint16_t*>(smem_raw + r * row_bytes + head4_x_offset(k)) = x[r]; }
-  }
-#pragma unroll
-  for (int r = 0; r < kH4Rows; r++) { const uint32_t m = warp_max_u32(top[r]); if (lane == 0) s_max[r][warp] = m; }
-  __syncthreads();
-  int shift[kH4Rows];                                                       // x is multiplied by 2^shift
-  bool bad = false;
-#pragma unroll
-  for (int r = 0; r < kH4Rows; r++) {
+  for (int d = 0; d < kAhead - 1; d++) fetch_next(ring[d]);
+  // ---- the rows of x: normalised if a norm is fused, scaled, binary16. A warp has 256 columns of a row at a time, a lane a chunk of 8.
+  const int items = kRows * steps;
+  auto chunk = [&](int item) -> uint4* { return reinterpret_cast<uint4*>(smem_raw + (item / steps) * row_bytes + (item % steps) * 512 + ((((lane & 7) << 2) + (lane >> 3)) << 4)); };
+  auto top_of = [](const uint32_t (&w)[4]) {
     uint32_t m = 0u;
 #pragma unroll
-    for (int q = 0; q < kH4Warps; q++) m = max(m, s_max[r][q]);
-    bad |= m >= 0x7F80u;                                                    // an infinity or a NaN
-    shift[r] = m == 0u ? 0 : 141 - static_cast<int>(max(m >> 7, 1u));       // (exponent of the largest to 14)
-  }
-  for (int k = tid; k < padded && !bad; k += kH4Threads) {
+    for (int e = 0; e < 4; e++) m = max(m, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));
+    return m;
+  };
+  for (int item = warp; item < items; item += kH4Warps) {
+    const int row = item / steps, k = (item % steps) * kH4Step + lane * 8;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    if (row < P.rows && k < H) {
+      const uint16_t* x = P.x + row * P.x_stride + k;
+      if ((reinterpret_cast<uintptr_t>(x) & 15u) == 0) { const uint4 q = *reinterpret_cast<const uint4*>(x); w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w; }
+      else {
 #pragma unroll
-    for (int r = 0; r < kH4Rows; r++) {
-      uint16_t* p = reinterpret_cast<uint16_t*>(smem_raw + r * row_bytes + head4_x_offset(k));
-      uint16_t h;
-      bad |= !scaled_f16(*p, shift[r], &h);
-      *p = h;
+        for (int e = 0; e < 4; e++) w[e] = static_cast<uint32_t>(x[2 * e]) | static_cast<uint32_t>(x[2 * e + 1]) << 16;
+      }
     }
-  }
-  const bool slow = __syncthreads_or(bad);
-  const float g = __ldg(P.scale);
-  auto put = [&](int r, int v, double sum, int n) { if (r < P.rows && v < P.vocab) P.logits[r * P.logits_stride + v] = f32_to_bf16(head4_finish(sum, g, n)); };
-  if (slow) {                                                               // some x is no binary16 after the scaling: BF16 in shared memory, FP64 arithmetic
-    for (int k = tid; k < padded; k += kH4Threads) {
-      uint16_t x[kH4Rows];
-      column(k, x);
+    *chunk(item) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (P.gamma) {
+      float ss = 0.0f;
 #pragma unroll
-      for (int r = 0; r < kH4Rows; r++) *reinterpret_cast<uint16_t*>(smem_raw + r * row_bytes + head4_x_offset(k)) = x[r];
+      for (int e = 0; e < 4; e++) { ss = __fmaf_rn(bf16_lo(w[e]), bf16_lo(w[e]), ss); ss = __fmaf_rn(bf16_hi(w[e]), bf16_hi(w[e]), ss); }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+      if (lane == 0) s_sum[item] = ss;
+    } else { const uint32_t m = warp_max_u32(top_of(w)); if (lane == 0) s_top[item] = m; }
+  }
+  __syncthreads();
+  if (P.gamma) {
+    if (tid < kRows) {
+      float ss = 0.0f;
+      for (int s = 0; s < steps; s++) ss += s_sum[tid * steps + s];
+      s_factor[tid] = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(H)), P.eps));
     }
     __syncthreads();
-    for (int v = blockIdx.x * kH4Warps + warp; v < P.vocab; v += gridDim.x * kH4Warps) {
-      double sum[kH4Rows];
-#pragma unroll
-      for (int r = 0; r < kH4Rows; r++) sum[r] = 0.0;
-      for (int w = lane; w < H / 8; w += 32) {
-        uint32_t h[4];
-        e2m1_to_f16(*reinterpret_cast<const uint32_t*>(P.codes + static_cast<int64_t>(v) * P.codes_stride + w * 4), h);
-        const float s = e4m3_value(P.scales[static_cast<int64_t>(v) * P.scales_stride + (w >> 1)]);
+    for (int item = warp; item < items; item += kH4Warps) {
+      const int row = item / steps, k = (item % steps) * kH4Step + lane * 8;
+      uint4 q = *chunk(item);
+      uint32_t w[4] = {q.x, q.y, q.z, q.w};
+      if (row < P.rows && k < H) {
+        const float inv_rms = s_factor[row];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const double w0 = f16_lo(h[e]) * s, w1 = f16_hi(h[e]) * s;
-#pragma unroll
-          for (int r = 0; r < kH4Rows; r++) {
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(smem_raw + r * row_bytes + head4_x_offset(8 * w + 2 * e));
-            sum[r] += static_cast<double>(bf16_lo(x)) * w0;
-            sum[r] += static_cast<double>(bf16_hi(x)) * w1;
-          }
+          const float g0 = __uint_as_float(static_cast<uint32_t>(__ldg(P.gamma + k + 2 * e)) << 16), g1 = __uint_as_float(static_cast<uint32_t>(__ldg(P.gamma + k + 2 * e + 1)) << 16);
+          const float s0 = P.one_plus ? __fadd_rn(1.0f, g0) : g0, s1 = P.one_plus ? __fadd_rn(1.0f, g1) : g1;
+          w[e] = static_cast<uint32_t>(f32_to_bf16(__fmul_rn(__fmul_rn(bf16_lo(w[e]), inv_rms), s0))) | static_cast<uint32_t>(f32_to_bf16(__fmul_rn(__fmul_rn(bf16_hi(w[e]), inv_rms), s1))) << 16;
         }
+        *chunk(item) = make_uint4(w[0], w[1], w[2], w[3]);
       }
+      const uint32_t m = warp_max_u32(top_of(w));
+      if (lane == 0) s_top[item] = m;
+    }
+    __syncthreads();
+  }
+  bool plain = true, bad = false;                                           // plain: every g * 2^-shift is a normal binary32, with room for the sum
+  if (tid < kRows) {
+    uint32_t m = 0u;
+    for (int s = 0; s < steps; s++) m = max(m, s_top[tid * steps + s]);
+    bad = m >= 0x7F80u;                                                     // an infinity or a NaN
+    const int shift = m == 0u ? 0 : 141 - static_cast<int>(max(m >> 7, 1u));      // x is multiplied by 2^shift (the exponent of the largest becomes 14)
+    const double f = static_cast<double>(g) * __hiloint2double((1023 - shift) << 20, 0);
+    plain = fabs(f) >= 0x1p-100 && fabs(f) <= 0x1p80;
+    s_shift[tid] = shift; s_factor[tid] = static_cast<float>(f);
+  }
+  plain = __syncthreads_and(plain);
+  for (int item = warp; item < items; item += kH4Warps) {
+    const int shift = s_shift[item / steps];
+    uint4 q = *chunk(item);
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-      for (int r = 0; r < kH4Rows; r++) {
+    for (int e = 0; e < 4; e++) {
+      uint16_t lo, hi;
+      bad |= !scaled_f16(static_cast<uint16_t>(w[e]), shift, &lo); bad |= !scaled_f16(static_cast<uint16_t>(w[e] >> 16), shift, &hi);
+      w[e] = static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
+    }
+    if (!bad) *chunk(item) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (__syncthreads_or(bad)) {
+    // some x is no binary16 after the scaling: FP64 on the values themselves
+    for (int v = blockIdx.x * kH4Warps + warp; v < P.vocab; v += all_warps) {
+      for (int r = 0; r < P.rows; r++) {
+        const uint16_t* x = P.x + r * P.x_stride;
+        float inv_rms = 1.0f;
+        if (P.gamma) {
+          float ss = 0.0f;
+          for (int s = 0; s < steps; s++) ss += s_sum[r * steps + s];
+          inv_rms = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(H)), P.eps));
+        }
+        double sum = 0.0;
+        for (int k = lane; k < H; k += 32) {
+          uint16_t xv = x[k];
+          if (P.gamma) {
+            const float gm = __uint_as_float(static_cast<uint32_t>(P.gamma[k]) << 16);
+            xv = f32_to_bf16(__fmul_rn(__fmul_rn(__uint_as_float(static_cast<uint32_t>(xv) << 16), inv_rms), P.one_plus ? __fadd_rn(1.0f, gm) : gm));
+          }
+          const uint32_t c = P.codes[static_cast<int64_t>(v) * P.codes_stride + (k >> 1)] >> (4 * (k & 1));
+          const float w = e2m1_value(c & 7u) * e4m3_value(P.scales[static_cast<int64_t>(v) * P.scales_stride + (k >> 4)]);
+          sum += static_cast<double>(__uint_as_float(static_cast<uint32_t>(xv) << 16)) * static_cast<double>(c & 8u ? -w : w);
+        }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum[r] += __shfl_xor_sync(kFull, sum[r], o);
-        if (lane == 0) put(r, v, sum[r], 0);
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+        if (lane == 0) P.logits[r * P.logits_stride + v] = f32_to_bf16(head4_finish(sum, g, 0));
       }
     }
     return;
   }
-  // ---- the tiles. A tile's sums are formed batch by batch (kH4Unroll steps into a fresh accumulator, then added to the total), the batches in order: the same
-  // additions whether one warp walks the whole row or, for the tiles left over after the last full round, the warps of a block take a batch each.
-  const int gq = lane >> 2, t = lane & 3;
-  const int n_tiles = (P.vocab + kH4Tile - 1) / kH4Tile;
-  const int batches = (steps + kH4Unroll - 1) / kH4Unroll;
-  const unsigned char* xrow = smem_raw + gq * row_bytes + t * 16;           // row gq of x, this thread's chunks
-  auto batch_sum = [&](int tile, int batch, float (&c)[4]) {
-    const int v0 = tile * kH4Tile;
-    const int64_t ra = min(v0 + gq, P.vocab - 1), rb = min(v0 + gq + 8, P.vocab - 1);      // (rows beyond the vocabulary: loaded again, never stored)
-    const int k0 = batch * kH4Unroll * kH4Step + 64 * t;
-    const uint8_t *ca = P.codes + ra * P.codes_stride + (k0 >> 1), *cb = P.codes + rb * P.codes_stride + (k0 >> 1);
-    const uint8_t *sa = P.scales + ra * P.scales_stride + (k0 >> 4), *sb = P.scales + rb * P.scales_stride + (k0 >> 4);
-    uint4 a[kH4Unroll][2], b[kH4Unroll][2];
-    uint32_t fa[kH4Unroll], fb[kH4Unroll];
+  // ---- products
+  const unsigned char* xrow = smem_raw + gq * row_bytes + t * 16;           // row gq of every eight of x, this thread's chunks
+  auto multiply = [&](const Piece4& p, int s, float (&c)[NT][4]) {
+    const uint32_t wa[8] = {p.a[0].x, p.a[0].y, p.a[0].z, p.a[0].w, p.a[1].x, p.a[1].y, p.a[1].z, p.a[1].w};
+    const uint32_t wb[8] = {p.b[0].x, p.b[0].y, p.b[0].z, p.b[0].w, p.b[1].x, p.b[1].y, p.b[1].z, p.b[1].w};
 #pragma unroll
-    for (int u = 0; u < kH4Unroll; u++) {
-      if (k0 + u * kH4Step < H) {                                           // (H is a multiple of 64: all of a thread's 64 columns or none)
-        a[u][0] = __ldcs(reinterpret_cast<const uint4*>(ca + u * 128)); a[u][1] = __ldcs(reinterpret_cast<const uint4*>(ca + u * 128) + 1);
-        b[u][0] = __ldcs(reinterpret_cast<const uint4*>(cb + u * 128)); b[u][1] = __ldcs(reinterpret_cast<const uint4*>(cb + u * 128) + 1);
-        fa[u] = __ldg(reinterpret_cast<const uint32_t*>(sa + u * 16)); fb[u] = __ldg(reinterpret_cast<const uint32_t*>(sb + u * 16));
-      } else { a[u][0] = a[u][1] = b[u][0] = b[u][1] = make_uint4(0u, 0u, 0u, 0u); fa[u] = fb[u] = 0u; }
-    }
-    c[0] = c[1] = c[2] = c[3] = 0.0f;
+    for (int h = 0; h < 2; h++) {                                           // two scales each
+      const uint32_t pa = e4m3_to_f16(p.fa >> (16 * h)), pb = e4m3_to_f16(p.fb >> (16 * h));
 #pragma unroll
-    for (int u = 0; u < kH4Unroll; u++) {
-      const int s = batch * kH4Unroll + u;
-      if (s >= steps) break;
-      const uint32_t wa[8] = {a[u][0].x, a[u][0].y, a[u][0].z, a[u][0].w, a[u][1].x, a[u][1].y, a[u][1].z, a[u][1].w};
-      const uint32_t wb[8] = {b[u][0].x, b[u][0].y, b[u][0].z, b[u][0].w, b[u][1].x, b[u][1].y, b[u][1].z, b[u][1].w};
+      for (int q = 0; q < 4; q++) {
+        const int j = 4 * h + q;
+        const uint32_t sa = __byte_perm(pa, 0u, q < 2 ? 0x1010 : 0x3232), sb = __byte_perm(pb, 0u, q < 2 ? 0x1010 : 0x3232);
+        uint32_t ha[4], hb[4];
+        e2m1_to_f16(wa[j], ha);
+        e2m1_to_f16(wb[j], hb);
 #pragma unroll
-      for (int p = 0; p < 2; p++) {                                         // two scales each
-        const uint32_t pa = e4m3_to_f16(fa[u] >> (16 * p)), pb = e4m3_to_f16(fb[u] >> (16 * p));
+        for (int e = 0; e < 4; e++) { ha[e] = f16x2_mul(ha[e], sa); hb[e] = f16x2_mul(hb[e], sb); }
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-          const int j = 4 * p + q;
-          const uint32_t sca = __byte_perm(pa, 0u, q < 2 ? 0x1010 : 0x3232), scb = __byte_perm(pb, 0u, q < 2 ? 0x1010 : 0x3232);
-          uint32_t ha[4], hb[4];
-          e2m1_to_f16(wa[j], ha);
-          e2m1_to_f16(wb[j], hb);
-#pragma unroll
-          for (int e = 0; e < 4; e++) { ha[e] = f16x2_mul(ha[e], sca); hb[e] = f16x2_mul(hb[e], scb); }
-          const uint4 x = *reinterpret_cast<const uint4*>(xrow + s * 512 + j * 64);
-          mma_f16_16816(c, ha[0], hb[0], ha[1], hb[1], x.x, x.y);
-          mma_f16_16816(c, ha[2], hb[2], ha[3], hb[3], x.z, x.w);
+        for (int n = 0; n < NT; n++) {
+          const uint4 x = *reinterpret_cast<const uint4*>(xrow + n * kH4Rows * row_bytes + s * 512 + j * 64);
+          mma_f16_16816(c[n], ha[0], hb[0], ha[1], hb[1], x.x, x.y);
+          mma_f16_16816(c[n], ha[2], hb[2], ha[3], hb[3], x.z, x.w);
         }
       }
     }
   };
-  auto store = [&](int tile, const float (&c)[4]) {
+  auto store = [&](int tile, const float (&c)[NT][4]) {
     const int v = tile * kH4Tile + gq;
 #pragma unroll
-    for (int r = 0; r < kH4Rows; r++) {
-      if (r >> 1 == t) { put(r, v, c[r & 1], shift[r]); put(r, v + 8, c[2 + (r & 1)], shift[r]); }
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int r = n * kH4Rows + 2 * t + (e & 1), vv = v + (e >> 1) * 8;
+        if (r < P.rows && vv < P.vocab) P.logits[r * P.logits_stride + vv] = f32_to_bf16(plain ? __fmul_rn(c[n][e], s_factor[r]) : head4_finish(c[n][e], g, s_shift[r]));
+      }
     }
   };
-  const int all_warps = gridDim.x * kH4Warps;
-  const int full = n_tiles / all_warps * all_warps;
-  for (int tile = blockIdx.x * kH4Warps + warp; tile < full; tile += all_warps) {
-    float total[4] = {0.0f, 0.0f, 0.0f, 0.0f}, c[4];
-    for (int batch = 0; batch < batches; batch++) {
-      batch_sum(tile, batch, c);
+  float c[NT][4], lo[NT][4], hi[NT][4];                                     // a quarter's sum; the first two quarters'; the third's
 #pragma unroll
-      for (int e = 0; e < 4; e++) total[e] = __fadd_rn(total[e], c[e]);
-    }
-    store(tile, total);
+  for (int n = 0; n < NT; n++) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) c[n][e] = lo[n][e] = hi[n][e] = 0.0f;
   }
-  for (int tile = full + blockIdx.x; tile < n_tiles; tile += gridDim.x) {
-    for (int batch = warp; batch < batches; batch += kH4Warps) {
-      float c[4];
-      batch_sum(tile, batch, c);
+  int s = 0, q = 0, bound = steps / 4;                                      // (a quarter: steps q * steps / 4 .. (q + 1) * steps / 4)
+  for (int tile = blockIdx.x * kH4Warps + warp; tile < full;) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) part[batch][lane][e] = c[e];
-    }
-    __syncthreads();
-    if (warp == 0) {
-      float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int batch = 0; batch < batches; batch++) {
+    for (int d = 0; d < kAhead; d++) {
+      if (tile >= full) break;
+      fetch_next(ring[(d + kAhead - 1) % kAhead]);
+      while (s == bound) {                                                  // the end of a quarter
 #pragma unroll
-        for (int e = 0; e < 4; e++) total[e] = __fadd_rn(total[e], part[batch][lane][e]);
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            if (q < 2) lo[n][e] = q == 0 ? c[n][e] : __fadd_rn(lo[n][e], c[n][e]); else hi[n][e] = c[n][e];
+            c[n][e] = 0.0f;
+          }
+        }
+        q++;
+        bound = (q + 1) * steps / 4;
       }
-      store(tile, total);
+      multiply(ring[d], s, c);
+      if (++s == steps) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) { c[n][e] = __fadd_rn(lo[n][e], __fadd_rn(hi[n][e], c[n][e])); lo[n][e] = hi[n][e] = 0.0f; }
+        }
+        store(tile, c);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) c[n][e] = 0.0f;
+        }
+        s = 0; q = 0; bound = steps / 4;
+        tile += all_warps;
+      }
     }
-    __syncthreads();
+  }
+  // ---- the tiles left over: four warps to a tile, a quarter each
+  const int group = warp >> 2, part = warp & 3, s0 = part * steps / 4, s1 = (part + 1) * steps / 4;
+  for (int tile = full + blockIdx.x + group * gridDim.x; tile < n_tiles; tile += 4 * gridDim.x) {
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) c[n][e] = 0.0f;
+    }
+    for (int b = s0; b < s1; b += kAhead) {
+#pragma unroll
+      for (int d = 0; d < kAhead; d++) if (b + d < s1) fetch(ring[d], tile, b + d);
+#pragma unroll
+      for (int d = 0; d < kAhead; d++) if (b + d < s1) multiply(ring[d], b + d, c);
+    }
+    if (part > 0) {
+#pragma unroll
+      for (int n = 0; n < NT; n++) *reinterpret_cast<float4*>(&s_u.part[group][part - 1][lane][4 * n]) = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
+    }
+    asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory");
+    if (part == 0) {
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          c[n][e] = __fadd_rn(__fadd_rn(c[n][e], s_u.part[group][0][lane][4 * n + e]), __fadd_rn(s_u.part[group][1][lane][4 * n + e], s_u.part[group][2][lane][4 * n + e]));
+      }
+      store(tile, c);
+    }
+    asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory");
   }
 }
 

@@ -78,8 +78,22 @@ int lm_dequantize_nvfp4(const lm_dequantize_nvfp4_args* a) {
   return launch_stream(false, nvfp4_dequantize_kernel, dim3(stride_grid(a->rows * (a->cols / 8), kQuantThreads, sms, 16)), kQuantThreads, 0, 1, static_cast<cudaStream_t>(a->stream), P);
 }
 
+// Rows of x that the mma.sync kernel takes: as many eights as its shared memory holds, four at most.
+static bool head4_few_rows(int64_t rows, int64_t hidden) {
+  const int64_t nt = (rows + kH4Rows - 1) / kH4Rows;
+  return nt <= 1 || (nt <= kH4MaxNT && head4_smem_bytes(static_cast<int>(hidden), static_cast<int>(nt)) <= 200 * 1024);
+}
+
+static int head_nvfp4_few(void (*kernel)(Head4Dev), const Head4Dev& P, int nt, int sms, cudaStream_t st) {
+  const size_t smem = head4_smem_bytes(P.hidden, nt);
+  const int rc = ensure_dynamic_smem(static_cast<KernelSlot>(kSlotHeadNvfp4 + nt - 1), reinterpret_cast<const void*>(kernel), smem);
+  if (rc != LM_OK) return rc;
+  const int tiles = (P.vocab + kH4Tile - 1) / kH4Tile;
+  return launch_beside(kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), kH4Threads, smem, 1, st, P);
+}
+
 size_t lm_head_nvfp4_workspace_bytes(int64_t rows, int64_t hidden_dim) {
-  if (rows <= kH4Rows || hidden_dim < 1 || rows > LM_HEAD_NVFP4_MAX_ROWS || hidden_dim > kH4MaxHidden) return 0;
+  if (hidden_dim < 1 || head4_few_rows(rows, hidden_dim) || rows > LM_HEAD_NVFP4_MAX_ROWS || hidden_dim > kH4MaxHidden) return 0;
   return batch4_workspace_bytes(rows, hidden_dim);
 }
 
@@ -165,16 +179,15 @@ int lm_head_nvfp4(const lm_head_nvfp4_args* a) {
   int sms = 0;
   rc = sm_count(&sms);
   if (rc != LM_OK) return rc;
-  if (a->rows > kH4Rows) return head_nvfp4_batch(a, sms);
-  const size_t smem = head4_smem_bytes(P.hidden);
-  rc = ensure_dynamic_smem(kSlotHeadNvfp4, reinterpret_cast<const void*>(lm_head_nvfp4_kernel), smem);
-  if (rc != LM_OK) return rc;
-  int per_sm = 1;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, lm_head_nvfp4_kernel, kH4Threads, smem) != cudaSuccess || per_sm < 1) per_sm = 1;
-  const long long tiles = (a->vocab + kH4Tile - 1) / kH4Tile, most = static_cast<long long>(per_sm) * sms;
-  const unsigned grid = static_cast<unsigned>(tiles < most ? tiles : most);
+  if (!head4_few_rows(a->rows, P.hidden)) return head_nvfp4_batch(a, sms);
   P.x = static_cast<const uint16_t*>(a->hidden); P.logits = static_cast<uint16_t*>(a->logits); P.rows = static_cast<int>(a->rows);
-  return launch_beside(lm_head_nvfp4_kernel, dim3(grid), kH4Threads, smem, 1, static_cast<cudaStream_t>(a->stream), P);
+  cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  switch ((a->rows + kH4Rows - 1) / kH4Rows) {
+    case 1: return head_nvfp4_few(lm_head_nvfp4_kernel<1, 4>, P, 1, sms, st);
+    case 2: return head_nvfp4_few(lm_head_nvfp4_kernel<2, 3>, P, 2, sms, st);
+    case 3: return head_nvfp4_few(lm_head_nvfp4_kernel<3, 2>, P, 3, sms, st);
+    default: return head_nvfp4_few(lm_head_nvfp4_kernel<4, 2>, P, 4, sms, st);
+  }
 }
 
 // Whether writing `out` can change what is read of `in` (both [rows, vocab] in elements of `size` bytes): same place and strides is in place, sharing nothing is fine.
