@@ -52,11 +52,58 @@ __device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b) { uint32_t
 __device__ __forceinline__ uint16_t f32_to_f16(float f) { uint16_t r; asm("cvt.rn.f16.f32 %0, %1;" : "=h"(r) : "f"(f)); return r; }
 __device__ __forceinline__ uint16_t f32_to_bf16(float f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f)); }
 
-// A BF16 value times 2^shift as binary16; false where that is not exact (a product that vanishes in binary32 included).
-__device__ __forceinline__ bool scaled_f16(uint16_t bf16, int shift, uint16_t* h) {
-  const float f = ldexpf(__uint_as_float(static_cast<uint32_t>(bf16) << 16), shift);
+// 2^shift in two factors (each a normal binary32 for every shift that occurs), and a BF16 value times that as binary16; false where it is not exact (a product that vanishes in
+// binary32 included). The first product is exact, the second one rounds at most where it falls below the normal numbers.
+struct Scale4 { float a, b; };
+__device__ __forceinline__ Scale4 scale_of(int shift) {
+  const int h = shift / 2;
+  return Scale4{__int_as_float((127 + h) << 23), __int_as_float((127 + shift - h) << 23)};
+}
+__device__ __forceinline__ bool scaled_f16(float x, Scale4 s, uint16_t* h) {
+  const float f = __fmul_rn(__fmul_rn(x, s.a), s.b);
   *h = f32_to_f16(f);
-  return f16_lo(*h) == f && (f != 0.0f || (bf16 & 0x7FFFu) == 0u);
+  return f16_lo(*h) == f && (f != 0.0f || x == 0.0f);
+}
+// The power of two that brings a row whose largest magnitude has these BF16 bits to 2^14 .. 2^15.
+__device__ __forceinline__ int shift_of(uint32_t top) { return top == 0u ? 0 : 141 - static_cast<int>(max(top >> 7, 1u)); }
+__device__ __forceinline__ uint32_t top_of(const uint32_t (&w)[4]) {         // the largest magnitude of eight BF16
+  uint32_t m = 0u;
+#pragma unroll
+  for (int e = 0; e < 4; e++) m = max(m, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));
+  return m;
+}
+// Eight BF16 from any address.
+__device__ __forceinline__ void load8(const uint16_t* p, uint32_t (&w)[4]) {
+  if ((reinterpret_cast<uintptr_t>(p) & 15u) == 0) { const uint4 q = *reinterpret_cast<const uint4*>(p); w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w; }
+  else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = static_cast<uint32_t>(p[2 * e]) | static_cast<uint32_t>(p[2 * e + 1]) << 16;
+  }
+}
+// Eight elements of a row normalised: bf16(x * inv_rms * scale).
+__device__ __forceinline__ void normalise8(uint32_t (&w)[4], const uint32_t (&gamma)[4], float inv_rms, int one_plus) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const float g0 = bf16_lo(gamma[e]), g1 = bf16_hi(gamma[e]);
+    const float lo = __fmul_rn(__fmul_rn(bf16_lo(w[e]), inv_rms), one_plus ? __fadd_rn(1.0f, g0) : g0), hi = __fmul_rn(__fmul_rn(bf16_hi(w[e]), inv_rms), one_plus ? __fadd_rn(1.0f, g1) : g1);
+    w[e] = static_cast<uint32_t>(f32_to_bf16(lo)) | static_cast<uint32_t>(f32_to_bf16(hi)) << 16;
+  }
+}
+__device__ __forceinline__ float squares8(const uint32_t (&w)[4]) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; e++) { ss = __fmaf_rn(bf16_lo(w[e]), bf16_lo(w[e]), ss); ss = __fmaf_rn(bf16_hi(w[e]), bf16_hi(w[e]), ss); }
+  return ss;
+}
+__device__ __forceinline__ bool scaled8(uint32_t (&w)[4], Scale4 s) {         // in place, BF16 to binary16; false where one is not exact
+  bool exact = true;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    uint16_t lo, hi;
+    exact &= scaled_f16(bf16_lo(w[e]), s, &lo); exact &= scaled_f16(bf16_hi(w[e]), s, &hi);
+    w[e] = static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
+  }
+  return exact;
 }
 // The sum of a logit times g and 2^-n (n: what x was multiplied by), in binary64 so that no intermediate leaves the range.
 __device__ __forceinline__ float head4_finish(double sum, float g, int n) {
@@ -82,7 +129,8 @@ static __global__ void __launch_bounds__(kH4Threads, 1) lm_head_nvfp4_kernel(Hea
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int H = P.hidden, row_bytes = head4_row_bytes(H), steps = head4_steps(H);
   const int gq = lane >> 2, t = lane & 3;
-  const int n_tiles = (P.vocab + kH4Tile - 1) / kH4Tile, all_warps = gridDim.x * kH4Warps, full = n_tiles / all_warps * all_warps;
+  // A round: a tile to a warp. What is left over after the full rounds takes another one, or (two quarters of a round or less) four warps to a tile.
+  const int n_tiles = (P.vocab + kH4Tile - 1) / kH4Tile, all_warps = gridDim.x * kH4Warps, left = n_tiles % all_warps, full = left > all_warps / 2 ? n_tiles : n_tiles - left;
   after_predecessor();
   const float g = __ldg(P.scale);
   auto fetch = [&](Piece4& p, int tile, int s) {
@@ -105,107 +153,97 @@ static __global__ void __launch_bounds__(kH4Threads, 1) lm_head_nvfp4_kernel(Hea
   };
 #pragma unroll
   for (int d = 0; d < kAhead - 1; d++) fetch_next(ring[d]);
-  // ---- the rows of x: normalised if a norm is fused, scaled, binary16. A warp has 256 columns of a row at a time, a lane a chunk of 8.
-  const int items = kRows * steps;
-  auto chunk = [&](int item) -> uint4* { return reinterpret_cast<uint4*>(smem_raw + (item / steps) * row_bytes + (item % steps) * 512 + ((((lane & 7) << 2) + (lane >> 3)) << 4)); };
-  auto top_of = [](const uint32_t (&w)[4]) {
-    uint32_t m = 0u;
+  // ---- the rows of x: normalised if a norm is fused, scaled, binary16. `per` warps to a row, 256 columns at a time, a lane a chunk of 8. (Rows of the mma beyond P.rows hold whatever
+  // is there: they reach no other row's sums.)
+  int per = kH4Warps;
+  while (per > 1 && per * P.rows > kH4Warps) per >>= 1;
+  const int my_row = warp / per, my_part = warp % per, row_step = kH4Warps / per;
+  constexpr int kTogether = 4;                                              // chunks a lane has under way
+  auto chunk = [&](int row, int s) -> uint4* { return reinterpret_cast<uint4*>(smem_raw + row * row_bytes + s * 512 + ((((lane & 7) << 2) + (lane >> 3)) << 4)); };
+  // f(row, s, w): the chunk's eight elements, changed or not; the chunks of a batch are asked for together
+  auto each = [&](auto get, auto f) {
+    for (int row = my_row; row < P.rows; row += row_step) {
+      for (int base = my_part; base < steps; base += kTogether * per) {
+        uint32_t w[kTogether][4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) m = max(m, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));
-    return m;
-  };
-  for (int item = warp; item < items; item += kH4Warps) {
-    const int row = item / steps, k = (item % steps) * kH4Step + lane * 8;
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-    if (row < P.rows && k < H) {
-      const uint16_t* x = P.x + row * P.x_stride + k;
-      if ((reinterpret_cast<uintptr_t>(x) & 15u) == 0) { const uint4 q = *reinterpret_cast<const uint4*>(x); w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w; }
-      else {
+        for (int u = 0; u < kTogether; u++) if (base + u * per < steps) get(row, base + u * per, w[u]);
 #pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = static_cast<uint32_t>(x[2 * e]) | static_cast<uint32_t>(x[2 * e + 1]) << 16;
+        for (int u = 0; u < kTogether; u++) if (base + u * per < steps) f(row, base + u * per, w[u]);
       }
     }
-    *chunk(item) = make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  auto from_memory = [&](int row, int s, uint32_t (&w)[4]) {
+    const int k = s * kH4Step + lane * 8;
+    w[0] = w[1] = w[2] = w[3] = 0u;
+    if (k < H) load8(P.x + row * P.x_stride + k, w);
+  };
+  auto from_shared = [&](int row, int s, uint32_t (&w)[4]) { const uint4 q = *chunk(row, s); w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w; };
+  auto to_shared = [&](int row, int s, const uint32_t (&w)[4]) { *chunk(row, s) = make_uint4(w[0], w[1], w[2], w[3]); };
+  auto mean_square = [&](int row) {
+    float ss = 0.0f;
+    for (int s = 0; s < steps; s++) ss += s_sum[row * kH4MaxSteps + s];
+    return __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(H)), P.eps));
+  };
+  each(from_memory, [&](int row, int s, uint32_t (&w)[4]) {
+    to_shared(row, s, w);
     if (P.gamma) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 4; e++) { ss = __fmaf_rn(bf16_lo(w[e]), bf16_lo(w[e]), ss); ss = __fmaf_rn(bf16_hi(w[e]), bf16_hi(w[e]), ss); }
+      float ss = squares8(w);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-      if (lane == 0) s_sum[item] = ss;
-    } else { const uint32_t m = warp_max_u32(top_of(w)); if (lane == 0) s_top[item] = m; }
-  }
-  __syncthreads();
+      if (lane == 0) s_sum[row * kH4MaxSteps + s] = ss;
+    } else { const uint32_t m = warp_max_u32(top_of(w)); if (lane == 0) s_top[row * kH4MaxSteps + s] = m; }
+  });
   if (P.gamma) {
-    if (tid < kRows) {
-      float ss = 0.0f;
-      for (int s = 0; s < steps; s++) ss += s_sum[tid * steps + s];
-      s_factor[tid] = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(H)), P.eps));
-    }
     __syncthreads();
-    for (int item = warp; item < items; item += kH4Warps) {
-      const int row = item / steps, k = (item % steps) * kH4Step + lane * 8;
-      uint4 q = *chunk(item);
-      uint32_t w[4] = {q.x, q.y, q.z, q.w};
-      if (row < P.rows && k < H) {
-        const float inv_rms = s_factor[row];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float g0 = __uint_as_float(static_cast<uint32_t>(__ldg(P.gamma + k + 2 * e)) << 16), g1 = __uint_as_float(static_cast<uint32_t>(__ldg(P.gamma + k + 2 * e + 1)) << 16);
-          const float s0 = P.one_plus ? __fadd_rn(1.0f, g0) : g0, s1 = P.one_plus ? __fadd_rn(1.0f, g1) : g1;
-          w[e] = static_cast<uint32_t>(f32_to_bf16(__fmul_rn(__fmul_rn(bf16_lo(w[e]), inv_rms), s0))) | static_cast<uint32_t>(f32_to_bf16(__fmul_rn(__fmul_rn(bf16_hi(w[e]), inv_rms), s1))) << 16;
-        }
-        *chunk(item) = make_uint4(w[0], w[1], w[2], w[3]);
+    float inv_rms = 0.0f;
+    int known = -1;
+    each(from_shared, [&](int row, int s, uint32_t (&w)[4]) {
+      if (row != known) { inv_rms = mean_square(row); known = row; }
+      const int k = s * kH4Step + lane * 8;
+      if (k < H) {
+        uint32_t gamma[4];
+        load8(P.gamma + k, gamma);
+        normalise8(w, gamma, inv_rms, P.one_plus);
+        to_shared(row, s, w);
       }
       const uint32_t m = warp_max_u32(top_of(w));
-      if (lane == 0) s_top[item] = m;
-    }
-    __syncthreads();
+      if (lane == 0) s_top[row * kH4MaxSteps + s] = m;
+    });
   }
+  __syncthreads();
   bool plain = true, bad = false;                                           // plain: every g * 2^-shift is a normal binary32, with room for the sum
-  if (tid < kRows) {
+  if (tid < P.rows) {
     uint32_t m = 0u;
-    for (int s = 0; s < steps; s++) m = max(m, s_top[tid * steps + s]);
+    for (int s = 0; s < steps; s++) m = max(m, s_top[tid * kH4MaxSteps + s]);
     bad = m >= 0x7F80u;                                                     // an infinity or a NaN
-    const int shift = m == 0u ? 0 : 141 - static_cast<int>(max(m >> 7, 1u));      // x is multiplied by 2^shift (the exponent of the largest becomes 14)
+    const int shift = shift_of(m);
     const double f = static_cast<double>(g) * __hiloint2double((1023 - shift) << 20, 0);
     plain = fabs(f) >= 0x1p-100 && fabs(f) <= 0x1p80;
     s_shift[tid] = shift; s_factor[tid] = static_cast<float>(f);
   }
   plain = __syncthreads_and(plain);
-  for (int item = warp; item < items; item += kH4Warps) {
-    const int shift = s_shift[item / steps];
-    uint4 q = *chunk(item);
-    uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      uint16_t lo, hi;
-      bad |= !scaled_f16(static_cast<uint16_t>(w[e]), shift, &lo); bad |= !scaled_f16(static_cast<uint16_t>(w[e] >> 16), shift, &hi);
-      w[e] = static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
-    }
-    if (!bad) *chunk(item) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+  each(from_shared, [&](int row, int s, uint32_t (&w)[4]) { bad |= !scaled8(w, scale_of(s_shift[row])); to_shared(row, s, w); });
   if (__syncthreads_or(bad)) {
     // some x is no binary16 after the scaling: FP64 on the values themselves
     for (int v = blockIdx.x * kH4Warps + warp; v < P.vocab; v += all_warps) {
       for (int r = 0; r < P.rows; r++) {
-        const uint16_t* x = P.x + r * P.x_stride;
-        float inv_rms = 1.0f;
-        if (P.gamma) {
-          float ss = 0.0f;
-          for (int s = 0; s < steps; s++) ss += s_sum[r * steps + s];
-          inv_rms = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(H)), P.eps));
-        }
+        const float inv_rms = P.gamma ? mean_square(r) : 1.0f;
         double sum = 0.0;
-        for (int k = lane; k < H; k += 32) {
-          uint16_t xv = x[k];
+        for (int k = lane * 8; k < H; k += 256) {
+          uint32_t x[4], h[4];
+          load8(P.x + r * P.x_stride + k, x);
           if (P.gamma) {
-            const float gm = __uint_as_float(static_cast<uint32_t>(P.gamma[k]) << 16);
-            xv = f32_to_bf16(__fmul_rn(__fmul_rn(__uint_as_float(static_cast<uint32_t>(xv) << 16), inv_rms), P.one_plus ? __fadd_rn(1.0f, gm) : gm));
+            uint32_t gamma[4];
+            load8(P.gamma + k, gamma);
+            normalise8(x, gamma, inv_rms, P.one_plus);
           }
-          const uint32_t c = P.codes[static_cast<int64_t>(v) * P.codes_stride + (k >> 1)] >> (4 * (k & 1));
-          const float w = e2m1_value(c & 7u) * e4m3_value(P.scales[static_cast<int64_t>(v) * P.scales_stride + (k >> 4)]);
-          sum += static_cast<double>(__uint_as_float(static_cast<uint32_t>(xv) << 16)) * static_cast<double>(c & 8u ? -w : w);
+          e2m1_to_f16(*reinterpret_cast<const uint32_t*>(P.codes + static_cast<int64_t>(v) * P.codes_stride + (k >> 1)), h);
+          const float sc = e4m3_value(P.scales[static_cast<int64_t>(v) * P.scales_stride + (k >> 4)]);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            sum += static_cast<double>(bf16_lo(x[e])) * static_cast<double>(f16_lo(h[e]) * sc);
+            sum += static_cast<double>(bf16_hi(x[e])) * static_cast<double>(f16_hi(h[e]) * sc);
+          }
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);

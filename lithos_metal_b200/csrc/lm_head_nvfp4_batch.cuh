@@ -63,87 +63,70 @@ struct Rows4Dev {
   uint8_t* xt; uint16_t* xb; int* shift; int* bad;
 };
 
-// One block: one (padded) row.
+// One block: one (padded) row, a thread up to kB4Chunks chunks of 8 columns.
+constexpr int kB4Chunks = (kH4MaxHidden / 8 + kB4RowsThreads - 1) / kB4RowsThreads;
 static __global__ void __launch_bounds__(kB4RowsThreads) nvfp4_rows_kernel(Rows4Dev P) {
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  uint16_t* xs = reinterpret_cast<uint16_t*>(smem_raw);                     // [hidden]
   __shared__ float s_sum[kB4RowsThreads / 32];
-  __shared__ uint32_t s_max[kB4RowsThreads / 32];
+  __shared__ uint32_t s_top[kB4RowsThreads / 32];
   after_predecessor();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x, H = P.hidden;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x, chunks = P.hidden / 8;
   const int group = row / kB4MaxN, in_group = row % kB4MaxN;
   const int n = min(kB4MaxN, batch4_padded(P.rows) - group * kB4MaxN);
-  unsigned char* out = P.xt + static_cast<size_t>(group) * kB4MaxN * H * 2;
-  auto place = [&](int chunk) { return out + (static_cast<size_t>(chunk >> 3) * n + in_group) * 128 + (((chunk & 7) ^ (in_group & 7)) << 4); };   // 8 columns: 16 bytes
+  unsigned char* out = P.xt + static_cast<size_t>(group) * kB4MaxN * P.hidden * 2;
+  auto place = [&](int c) { return reinterpret_cast<uint4*>(out + (static_cast<size_t>(c >> 3) * n + in_group) * 128 + (((c & 7) ^ (in_group & 7)) << 4)); };   // 8 columns: 16 bytes
   if (row >= P.rows) {
-    for (int c = tid; c < H / 8; c += kB4RowsThreads) *reinterpret_cast<uint4*>(place(c)) = make_uint4(0u, 0u, 0u, 0u);
+    for (int c = tid; c < chunks; c += kB4RowsThreads) *place(c) = make_uint4(0u, 0u, 0u, 0u);
     if (tid == 0) { P.shift[row] = 0; P.bad[row] = 0; }
     return;
   }
-  const uint16_t* x = P.x + row * P.x_stride;
-  const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
+  uint32_t w[kB4Chunks][4];
   float ss = 0.0f;
-  for (int c = tid; c < H / 8; c += kB4RowsThreads) {
-    uint4 q;
-    if (aligned) q = *reinterpret_cast<const uint4*>(x + 8 * c);
-    else {
-      uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) w[e] = static_cast<uint32_t>(x[8 * c + 2 * e]) | static_cast<uint32_t>(x[8 * c + 2 * e + 1]) << 16;
-      q = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int e = 0; e < 4; e++) { ss = __fmaf_rn(bf16_lo(w[e]), bf16_lo(w[e]), ss); ss = __fmaf_rn(bf16_hi(w[e]), bf16_hi(w[e]), ss); }
-    *reinterpret_cast<uint4*>(xs + 8 * c) = q;
+  for (int u = 0; u < kB4Chunks; u++) {
+    w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
+    if (tid + u * kB4RowsThreads < chunks) load8(P.x + row * P.x_stride + 8 * (tid + u * kB4RowsThreads), w[u]);
   }
-  float inv_rms = 1.0f;
   if (P.gamma) {
+#pragma unroll
+    for (int u = 0; u < kB4Chunks; u++) ss += squares8(w[u]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
     if (lane == 0) s_sum[warp] = ss;
     __syncthreads();
-    float s = 0.0f;
+    ss = 0.0f;
 #pragma unroll
-    for (int q = 0; q < kB4RowsThreads / 32; q++) s += s_sum[q];
-    inv_rms = __frsqrt_rn(__fadd_rn(__fdiv_rn(s, static_cast<float>(H)), P.eps));
+    for (int q = 0; q < kB4RowsThreads / 32; q++) ss += s_sum[q];
+    const float inv_rms = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(P.hidden)), P.eps));
+#pragma unroll
+    for (int u = 0; u < kB4Chunks; u++) {
+      if (tid + u * kB4RowsThreads < chunks) {
+        uint32_t gamma[4];
+        load8(P.gamma + 8 * (tid + u * kB4RowsThreads), gamma);
+        normalise8(w[u], gamma, inv_rms, P.one_plus);
+      }
+    }
   }
   uint32_t top = 0u;
-  for (int c = tid; c < H / 8; c += kB4RowsThreads) {                        // (a thread's own columns: no barrier)
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      uint16_t v = xs[8 * c + e];
-      if (P.gamma) {
-        const float gm = __uint_as_float(static_cast<uint32_t>(P.gamma[8 * c + e]) << 16);
-        v = f32_to_bf16(__fmul_rn(__fmul_rn(__uint_as_float(static_cast<uint32_t>(v) << 16), inv_rms), P.one_plus ? __fadd_rn(1.0f, gm) : gm));
-        xs[8 * c + e] = v;
-      }
-      top = max(top, static_cast<uint32_t>(v) & 0x7FFFu);
-    }
-  }
+  for (int u = 0; u < kB4Chunks; u++) top = max(top, top_of(w[u]));
   top = warp_max_u32(top);
-  if (lane == 0) s_max[warp] = top;
+  if (lane == 0) s_top[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int q = 0; q < kB4RowsThreads / 32; q++) top = max(top, s_max[q]);
-  const int shift = top == 0u ? 0 : 141 - static_cast<int>(max(top >> 7, 1u));
+  for (int q = 0; q < kB4RowsThreads / 32; q++) top = max(top, s_top[q]);
+  const int shift = shift_of(top);
   bool bad = top >= 0x7F80u;
-  for (int c = tid; c < H / 8; c += kB4RowsThreads) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) { uint16_t h; bad |= !scaled_f16(xs[8 * c + e], shift, &h); }
+  for (int u = 0; u < kB4Chunks; u++) {
+    if (tid + u * kB4RowsThreads < chunks) {
+      *reinterpret_cast<uint4*>(P.xb + static_cast<size_t>(row) * P.hidden + 8 * (tid + u * kB4RowsThreads)) = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
+      bad |= !scaled8(w[u], scale_of(shift));
+    }
   }
   bad = __syncthreads_or(bad);
-  for (int c = tid; c < H / 8; c += kB4RowsThreads) {
-    uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      uint16_t lo, hi;
-      scaled_f16(xs[8 * c + 2 * e], shift, &lo); scaled_f16(xs[8 * c + 2 * e + 1], shift, &hi);
-      w[e] = bad ? 0u : static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
-    }
-    *reinterpret_cast<uint4*>(place(c)) = make_uint4(w[0], w[1], w[2], w[3]);
-    *reinterpret_cast<uint4*>(P.xb + static_cast<size_t>(row) * H + 8 * c) = *reinterpret_cast<const uint4*>(xs + 8 * c);
-  }
+  for (int u = 0; u < kB4Chunks; u++)
+    if (tid + u * kB4RowsThreads < chunks) *place(tid + u * kB4RowsThreads) = bad ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
   if (tid == 0) { P.shift[row] = shift; P.bad[row] = bad ? 1 : 0; }
 }
 

@@ -131,7 +131,7 @@ static int head_nvfp4_batch(const lm_head_nvfp4_args* a, int sms) {
   ws = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~static_cast<uintptr_t>(255));
   R.xb = reinterpret_cast<uint16_t*>(ws); ws += batch4_xb_bytes(a->rows, a->hidden_dim);
   R.shift = reinterpret_cast<int*>(ws); R.bad = R.shift + padded;
-  int rc = launch_beside(nvfp4_rows_kernel, dim3(static_cast<unsigned>(padded)), kB4RowsThreads, static_cast<size_t>(R.hidden) * 2, 1, st, R);
+  int rc = launch_beside(nvfp4_rows_kernel, dim3(static_cast<unsigned>(padded)), kB4RowsThreads, 0, 1, st, R);
   if (rc != LM_OK) return rc;
   Batch4Dev P;
   P.codes = a->codes; P.codes_stride = a->codes_stride; P.scales = a->scales; P.scales_stride = a->scales_stride; P.scale = a->scale;
