@@ -8,14 +8,17 @@
 // mma: on tcgen05 they pass through shared or tensor memory, which costs more than the products of so few rows: lm_head_nvfp4_batch.cuh.) A warp's loads run ahead in registers.
 //
 // x is BF16 and the mma wants binary16 on both sides. A row of x is multiplied by the power of two that brings its largest magnitude to 2^14 .. 2^15 (taken out
-// again behind the sum); BF16 values down to 2^-31 of the largest are then exact in binary16, subnormals included. Where some x is not (or is infinite or NaN),
-// every block sees it and takes the rows the slow way, in FP64 on the CUDA cores, whose range holds every product.
+// again behind the sum); BF16 values down to 2^-31 of the largest are then exact in binary16, subnormals included. A row where some x is not (or is infinite or NaN) is
+// done over at the end, in FP64 on the CUDA cores, whose range holds every product. All this is nvfp4_rows_kernel's work, once per call; this kernel's blocks copy its result. (Every block
+// preparing x for itself took 13 us of a call of 8 rows of 4096.)
 //
 // A row's sum is (q0 + q1) + (q2 + q3) over four quarters of the hidden dimension, each in order: the same additions whether a warp walks the whole row or, for the tiles left over after
 // the last full round, four warps take a quarter each.
 #pragma once
 #include "common.cuh"
 #include "nvfp4.cuh"
+
+#include <climits>
 
 namespace lm {
 
@@ -26,13 +29,12 @@ constexpr int kH4MaxNT = 4;
 constexpr int kH4Tile = 16;                  // vocabulary rows per warp tile (the m dimension)
 constexpr int kH4Step = 256;                 // columns per step: 32 bytes of codes per thread and row, a whole 128-byte line per row and quad
 constexpr int kH4MaxHidden = 12736;
-constexpr int kH4MaxSteps = (kH4MaxHidden + kH4Step - 1) / kH4Step;
 
 struct Head4Dev {
-  const uint16_t* x; int64_t x_stride; int rows;
+  int rows;
   const uint8_t* codes; int64_t codes_stride; const uint8_t* scales; int64_t scales_stride; const float* scale;
   int hidden; int vocab;
-  const uint16_t* gamma; float eps; int one_plus;
+  const uint8_t* xt; const uint16_t* xb; const int* shift; const int* bad;
   uint16_t* logits; int64_t logits_stride;
 };
 
@@ -110,6 +112,142 @@ __device__ __forceinline__ float head4_finish(double sum, float g, int n) {
   return __double2float_rn(sum * static_cast<double>(g) * __hiloint2double((1023 - n) << 20, 0));
 }
 
+// ---- the rows of x, once per call: normalised if a norm is fused, scaled, binary16 --------------------------------------------------------------------
+
+// Workspace: x in binary16, for few rows as they lie in shared memory (head4_x_offset), otherwise by pieces of 64 columns, [group of 256 rows][hidden / 64][rows of the group, padded to 16]
+// [128 bytes, swizzled]; x in BF16 [rows][hidden]; shift and bad [padded rows].
+constexpr int kX4Threads = 256;
+constexpr int kX4Group = 256;
+constexpr uint32_t kWait4Limit = 1u << 20;
+__host__ __device__ inline int x4_padded(int64_t rows) { return static_cast<int>((rows + 15) / 16 * 16); }
+__host__ inline size_t x4_xt_bytes(int64_t rows, int64_t hidden) { return (static_cast<size_t>(x4_padded(rows)) * head4_row_bytes(static_cast<int>(hidden)) + 255) / 256 * 256; }
+__host__ inline size_t x4_xb_bytes(int64_t rows, int64_t hidden) { return (static_cast<size_t>(rows) * hidden * 2 + 255) / 256 * 256; }
+__host__ inline size_t x4_workspace_bytes(int64_t rows, int64_t hidden) { return x4_xt_bytes(rows, hidden) + x4_xb_bytes(rows, hidden) + static_cast<size_t>(x4_padded(rows)) * 8; }
+
+struct Rows4Dev {
+  const uint16_t* x; int64_t x_stride; int rows; int hidden;
+  const uint16_t* gamma; float eps; int one_plus;
+  int few;                                  // the layout of the mma.sync kernel
+  uint8_t* xt; uint16_t* xb; int* shift; int* bad;
+};
+
+// One block: one (padded) row, a thread up to kX4Chunks chunks of 8 columns.
+constexpr int kX4Chunks = (kH4MaxHidden / 8 + kX4Threads - 1) / kX4Threads;
+static __global__ void __launch_bounds__(kX4Threads) nvfp4_rows_kernel(Rows4Dev P) {
+  __shared__ float s_sum[kX4Threads / 32];
+  __shared__ uint32_t s_top[kX4Threads / 32];
+  after_predecessor();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x, chunks = P.hidden / 8;
+  // where the 16 bytes of 8 columns go
+  const int group = row / kX4Group, in_group = row % kX4Group, n = min(kX4Group, x4_padded(P.rows) - group * kX4Group);
+  unsigned char* out = P.few ? P.xt + static_cast<size_t>(row) * head4_row_bytes(P.hidden) : P.xt + static_cast<size_t>(group) * kX4Group * P.hidden * 2;
+  auto place = [&](int c) {
+    return reinterpret_cast<uint4*>(P.few ? out + head4_x_offset(8 * c) : out + (static_cast<size_t>(c >> 3) * n + in_group) * 128 + (((c & 7) ^ (in_group & 7)) << 4));
+  };
+  if (row >= P.rows) {
+    for (int c = tid; c < chunks; c += kX4Threads) *place(c) = make_uint4(0u, 0u, 0u, 0u);
+    if (tid == 0) { P.shift[row] = 0; P.bad[row] = 0; }
+    return;
+  }
+  uint32_t w[kX4Chunks][4];
+  float ss = 0.0f;
+#pragma unroll
+  for (int u = 0; u < kX4Chunks; u++) {
+    w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
+    if (tid + u * kX4Threads < chunks) load8(P.x + row * P.x_stride + 8 * (tid + u * kX4Threads), w[u]);
+  }
+  if (P.gamma) {
+#pragma unroll
+    for (int u = 0; u < kX4Chunks; u++) ss += squares8(w[u]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+    if (lane == 0) s_sum[warp] = ss;
+    __syncthreads();
+    ss = 0.0f;
+#pragma unroll
+    for (int q = 0; q < kX4Threads / 32; q++) ss += s_sum[q];
+    const float inv_rms = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(P.hidden)), P.eps));
+#pragma unroll
+    for (int u = 0; u < kX4Chunks; u++) {
+      if (tid + u * kX4Threads < chunks) {
+        uint32_t gamma[4];
+        load8(P.gamma + 8 * (tid + u * kX4Threads), gamma);
+        normalise8(w[u], gamma, inv_rms, P.one_plus);
+      }
+    }
+  }
+  uint32_t top = 0u;
+#pragma unroll
+  for (int u = 0; u < kX4Chunks; u++) top = max(top, top_of(w[u]));
+  top = warp_max_u32(top);
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kX4Threads / 32; q++) top = max(top, s_top[q]);
+  const int shift = shift_of(top);
+  bool bad = top >= 0x7F80u;
+#pragma unroll
+  for (int u = 0; u < kX4Chunks; u++) {
+    if (tid + u * kX4Threads < chunks) {
+      *reinterpret_cast<uint4*>(P.xb + static_cast<size_t>(row) * P.hidden + 8 * (tid + u * kX4Threads)) = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
+      bad |= !scaled8(w[u], scale_of(shift));
+    }
+  }
+  bad = __syncthreads_or(bad);
+#pragma unroll
+  for (int u = 0; u < kX4Chunks; u++)
+    if (tid + u * kX4Threads < chunks) *place(tid + u * kX4Threads) = bad ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
+  if (P.few && tid < head4_steps(P.hidden) * 32 - chunks) *place(chunks + tid) = make_uint4(0u, 0u, 0u, 0u);     // (the last step's columns beyond the row)
+  if (tid == 0) { P.shift[row] = shift; P.bad[row] = bad ? 1 : 0; }
+}
+
+// ---- barriers and copies -------------------------------------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t smem_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void barrier_arrive(uint32_t bar, uint32_t count = 1u) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0u;
+}
+// False when the limit ran out here or the block has given up. (Out of line: the usual wait is over at the first or second look, and the roles' loops have to stay short.)
+__device__ __noinline__ bool barrier_wait_long(uint32_t bar, uint32_t parity, volatile uint32_t* given_up) {
+  for (uint32_t i = 0; i < kWait4Limit; i++) {
+    if (barrier_try(bar, parity)) return true;
+    if ((i & 15u) == 15u && *given_up) return false;
+  }
+  *given_up = 1u;
+  return false;
+}
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile uint32_t* given_up) {
+  return barrier_try(bar, parity) || barrier_wait_long(bar, parity, given_up);
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+constexpr int kBad4 = INT_MIN;               // in the place of a shift: the row is done over
+
+// The sum of a logit in FP64, by a warp: x [hidden] in BF16, a row's codes and scales.
+__device__ __noinline__ double exact_sum(const uint16_t* x, const uint8_t* codes, const uint8_t* scales, int hidden, int lane) {
+  double sum = 0.0;
+  for (int k = lane * 8; k < hidden; k += 256) {
+    uint32_t xw[4], h[4];
+    load8(x + k, xw);
+    e2m1_to_f16(*reinterpret_cast<const uint32_t*>(codes + (k >> 1)), h);
+    const float sc = e4m3_value(scales[k >> 4]);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      sum += static_cast<double>(bf16_lo(xw[e])) * static_cast<double>(f16_lo(h[e]) * sc);
+      sum += static_cast<double>(bf16_hi(xw[e])) * static_cast<double>(f16_hi(h[e]) * sc);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+  return sum;
+}
+
 // 16 vocabulary rows' codes and scales of a step, a thread's part: 64 columns of rows g and g + 8.
 struct Piece4 { uint4 a[2], b[2]; uint32_t fa, fb; };
 
@@ -118,20 +256,16 @@ template <int NT, int kAhead>
 static __global__ void __launch_bounds__(kH4Threads, 1) lm_head_nvfp4_kernel(Head4Dev P) {
   constexpr int kRows = kH4Rows * NT;
   extern __shared__ __align__(16) unsigned char smem_raw[];                 // [kRows][row_bytes]
-  __shared__ union {
-    struct { float sum[kRows * kH4MaxSteps]; uint32_t top[kRows * kH4MaxSteps]; } x;       // while x is prepared
-    float part[4][3][32][4 * NT];                                           // later: quarters of the tiles left over
-  } s_u;
-  float* s_sum = s_u.x.sum;
-  uint32_t* s_top = s_u.x.top;
-  __shared__ float s_factor[kRows];                                         // 1 / rms, then g * 2^-shift
+  __shared__ float s_part[4][3][32][4 * NT];                                // quarters of the tiles left over
+  __shared__ float s_factor[kRows];                                         // g * 2^-shift
   __shared__ int s_shift[kRows];
+  __shared__ uint64_t s_bar;
+  __shared__ uint32_t s_gave_up;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int H = P.hidden, row_bytes = head4_row_bytes(H), steps = head4_steps(H);
   const int gq = lane >> 2, t = lane & 3;
   // A round: a tile to a warp. What is left over after the full rounds takes another one, or (two quarters of a round or less) four warps to a tile.
   const int n_tiles = (P.vocab + kH4Tile - 1) / kH4Tile, all_warps = gridDim.x * kH4Warps, left = n_tiles % all_warps, full = left > all_warps / 2 ? n_tiles : n_tiles - left;
-  after_predecessor();
   const float g = __ldg(P.scale);
   auto fetch = [&](Piece4& p, int tile, int s) {
     const int v0 = tile * kH4Tile + gq, k = s * kH4Step + 64 * t;
@@ -143,7 +277,8 @@ static __global__ void __launch_bounds__(kH4Threads, 1) lm_head_nvfp4_kernel(Hea
       p.fa = __ldg(reinterpret_cast<const uint32_t*>(P.scales + ra * P.scales_stride + (k >> 4))); p.fb = __ldg(reinterpret_cast<const uint32_t*>(P.scales + rb * P.scales_stride + (k >> 4)));
     } else { p.a[0] = p.a[1] = p.b[0] = p.b[1] = make_uint4(0u, 0u, 0u, 0u); p.fa = p.fb = 0u; }
   };
-  // ---- the first steps' loads; they arrive while x is prepared
+  // ---- the first steps' loads; they arrive while x is prepared. (The launch in front is the preparation of x, which begins to let this one in when all before it is complete: the weight
+  // may be read at once.)
   Piece4 ring[kAhead];
   int load_tile = blockIdx.x * kH4Warps + warp, load_step = 0;
   auto fetch_next = [&](Piece4& p) {
@@ -153,105 +288,29 @@ static __global__ void __launch_bounds__(kH4Threads, 1) lm_head_nvfp4_kernel(Hea
   };
 #pragma unroll
   for (int d = 0; d < kAhead - 1; d++) fetch_next(ring[d]);
-  // ---- the rows of x: normalised if a norm is fused, scaled, binary16. `per` warps to a row, 256 columns at a time, a lane a chunk of 8. (Rows of the mma beyond P.rows hold whatever
-  // is there: they reach no other row's sums.)
-  int per = kH4Warps;
-  while (per > 1 && per * P.rows > kH4Warps) per >>= 1;
-  const int my_row = warp / per, my_part = warp % per, row_step = kH4Warps / per;
-  constexpr int kTogether = 4;                                              // chunks a lane has under way
-  auto chunk = [&](int row, int s) -> uint4* { return reinterpret_cast<uint4*>(smem_raw + row * row_bytes + s * 512 + ((((lane & 7) << 2) + (lane >> 3)) << 4)); };
-  // f(row, s, w): the chunk's eight elements, changed or not; the chunks of a batch are asked for together
-  auto each = [&](auto get, auto f) {
-    for (int row = my_row; row < P.rows; row += row_step) {
-      for (int base = my_part; base < steps; base += kTogether * per) {
-        uint32_t w[kTogether][4];
-#pragma unroll
-        for (int u = 0; u < kTogether; u++) if (base + u * per < steps) get(row, base + u * per, w[u]);
-#pragma unroll
-        for (int u = 0; u < kTogether; u++) if (base + u * per < steps) f(row, base + u * per, w[u]);
-      }
-    }
-  };
-  auto from_memory = [&](int row, int s, uint32_t (&w)[4]) {
-    const int k = s * kH4Step + lane * 8;
-    w[0] = w[1] = w[2] = w[3] = 0u;
-    if (k < H) load8(P.x + row * P.x_stride + k, w);
-  };
-  auto from_shared = [&](int row, int s, uint32_t (&w)[4]) { const uint4 q = *chunk(row, s); w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w; };
-  auto to_shared = [&](int row, int s, const uint32_t (&w)[4]) { *chunk(row, s) = make_uint4(w[0], w[1], w[2], w[3]); };
-  auto mean_square = [&](int row) {
-    float ss = 0.0f;
-    for (int s = 0; s < steps; s++) ss += s_sum[row * kH4MaxSteps + s];
-    return __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(H)), P.eps));
-  };
-  each(from_memory, [&](int row, int s, uint32_t (&w)[4]) {
-    to_shared(row, s, w);
-    if (P.gamma) {
-      float ss = squares8(w);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-      if (lane == 0) s_sum[row * kH4MaxSteps + s] = ss;
-    } else { const uint32_t m = warp_max_u32(top_of(w)); if (lane == 0) s_top[row * kH4MaxSteps + s] = m; }
-  });
-  if (P.gamma) {
-    __syncthreads();
-    float inv_rms = 0.0f;
-    int known = -1;
-    each(from_shared, [&](int row, int s, uint32_t (&w)[4]) {
-      if (row != known) { inv_rms = mean_square(row); known = row; }
-      const int k = s * kH4Step + lane * 8;
-      if (k < H) {
-        uint32_t gamma[4];
-        load8(P.gamma + k, gamma);
-        normalise8(w, gamma, inv_rms, P.one_plus);
-        to_shared(row, s, w);
-      }
-      const uint32_t m = warp_max_u32(top_of(w));
-      if (lane == 0) s_top[row * kH4MaxSteps + s] = m;
-    });
+  // ---- x
+  if (tid == 0) {
+    barrier_init(smem_address(&s_bar), 1);
+    s_gave_up = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  __syncthreads();
-  bool plain = true, bad = false;                                           // plain: every g * 2^-shift is a normal binary32, with room for the sum
+  after_predecessor();
+  bool plain = true;                                                        // every g * 2^-shift is a normal binary32, with room for the sum
+  if (tid == 0) {
+    barrier_expect(smem_address(&s_bar), static_cast<uint32_t>(P.rows * row_bytes));
+    bulk_copy(smem_address(smem_raw), P.xt, static_cast<uint32_t>(P.rows * row_bytes), smem_address(&s_bar));       // (rows of the mma beyond P.rows reach no other row's sums)
+  }
+  bool any_bad = false;
   if (tid < P.rows) {
-    uint32_t m = 0u;
-    for (int s = 0; s < steps; s++) m = max(m, s_top[tid * kH4MaxSteps + s]);
-    bad = m >= 0x7F80u;                                                     // an infinity or a NaN
-    const int shift = shift_of(m);
+    const int shift = P.shift[tid];
     const double f = static_cast<double>(g) * __hiloint2double((1023 - shift) << 20, 0);
     plain = fabs(f) >= 0x1p-100 && fabs(f) <= 0x1p80;
-    s_shift[tid] = shift; s_factor[tid] = static_cast<float>(f);
+    any_bad = P.bad[tid] != 0;
+    s_shift[tid] = any_bad ? kBad4 : shift; s_factor[tid] = static_cast<float>(f);
   }
   plain = __syncthreads_and(plain);
-  each(from_shared, [&](int row, int s, uint32_t (&w)[4]) { bad |= !scaled8(w, scale_of(s_shift[row])); to_shared(row, s, w); });
-  if (__syncthreads_or(bad)) {
-    // some x is no binary16 after the scaling: FP64 on the values themselves
-    for (int v = blockIdx.x * kH4Warps + warp; v < P.vocab; v += all_warps) {
-      for (int r = 0; r < P.rows; r++) {
-        const float inv_rms = P.gamma ? mean_square(r) : 1.0f;
-        double sum = 0.0;
-        for (int k = lane * 8; k < H; k += 256) {
-          uint32_t x[4], h[4];
-          load8(P.x + r * P.x_stride + k, x);
-          if (P.gamma) {
-            uint32_t gamma[4];
-            load8(P.gamma + k, gamma);
-            normalise8(x, gamma, inv_rms, P.one_plus);
-          }
-          e2m1_to_f16(*reinterpret_cast<const uint32_t*>(P.codes + static_cast<int64_t>(v) * P.codes_stride + (k >> 1)), h);
-          const float sc = e4m3_value(P.scales[static_cast<int64_t>(v) * P.scales_stride + (k >> 4)]);
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            sum += static_cast<double>(bf16_lo(x[e])) * static_cast<double>(f16_lo(h[e]) * sc);
-            sum += static_cast<double>(bf16_hi(x[e])) * static_cast<double>(f16_hi(h[e]) * sc);
-          }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-        if (lane == 0) P.logits[r * P.logits_stride + v] = f32_to_bf16(head4_finish(sum, g, 0));
-      }
-    }
-    return;
-  }
+  any_bad = __syncthreads_or(any_bad);
+  barrier_wait(smem_address(&s_bar), 0u, &s_gave_up);
   // ---- products
   const unsigned char* xrow = smem_raw + gq * row_bytes + t * 16;           // row gq of every eight of x, this thread's chunks
   auto multiply = [&](const Piece4& p, int s, float (&c)[NT][4]) {
@@ -285,7 +344,7 @@ static __global__ void __launch_bounds__(kH4Threads, 1) lm_head_nvfp4_kernel(Hea
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const int r = n * kH4Rows + 2 * t + (e & 1), vv = v + (e >> 1) * 8;
-        if (r < P.rows && vv < P.vocab) P.logits[r * P.logits_stride + vv] = f32_to_bf16(plain ? __fmul_rn(c[n][e], s_factor[r]) : head4_finish(c[n][e], g, s_shift[r]));
+        if (r < P.rows && vv < P.vocab && s_shift[r] != kBad4) P.logits[r * P.logits_stride + vv] = f32_to_bf16(plain ? __fmul_rn(c[n][e], s_factor[r]) : head4_finish(c[n][e], g, s_shift[r]));
       }
     }
   };
@@ -347,7 +406,7 @@ static __global__ void __launch_bounds__(kH4Threads, 1) lm_head_nvfp4_kernel(Hea
     }
     if (part > 0) {
 #pragma unroll
-      for (int n = 0; n < NT; n++) *reinterpret_cast<float4*>(&s_u.part[group][part - 1][lane][4 * n]) = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
+      for (int n = 0; n < NT; n++) *reinterpret_cast<float4*>(&s_part[group][part - 1][lane][4 * n]) = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
     }
     asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory");
     if (part == 0) {
@@ -355,11 +414,20 @@ static __global__ void __launch_bounds__(kH4Threads, 1) lm_head_nvfp4_kernel(Hea
       for (int n = 0; n < NT; n++) {
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          c[n][e] = __fadd_rn(__fadd_rn(c[n][e], s_u.part[group][0][lane][4 * n + e]), __fadd_rn(s_u.part[group][1][lane][4 * n + e], s_u.part[group][2][lane][4 * n + e]));
+          c[n][e] = __fadd_rn(__fadd_rn(c[n][e], s_part[group][0][lane][4 * n + e]), __fadd_rn(s_part[group][1][lane][4 * n + e], s_part[group][2][lane][4 * n + e]));
       }
       store(tile, c);
     }
     asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory");
+  }
+  // ---- rows whose x is no binary16 after the scaling, or x that never came
+  __syncthreads();
+  for (int r = 0; r < P.rows && (any_bad || s_gave_up); r++) {
+    if (s_shift[r] != kBad4 && !s_gave_up) continue;
+    for (int v = blockIdx.x * kH4Warps + warp; v < P.vocab; v += all_warps) {
+      const float z = s_gave_up ? __int_as_float(0x7FC00000) : head4_finish(exact_sum(P.xb + static_cast<size_t>(r) * H, P.codes + v * P.codes_stride, P.scales + v * P.scales_stride, H, lane), g, 0);
+      if (lane == 0) P.logits[r * P.logits_stride + v] = f32_to_bf16(z);
+    }
   }
 }
 

@@ -20,7 +20,7 @@
 namespace lm {
 
 constexpr int kB4Tile = 128;                 // vocabulary rows per tile (M)
-constexpr int kB4MaxN = 256;                 // rows of x per launch
+constexpr int kB4MaxN = kX4Group;            // rows of x per launch
 constexpr int kB4StepCols = 256;             // columns of a tile's codes that come together: 128 bytes a row, and 16 of scales
 constexpr int kB4Cols = 128;                 // columns of an operand: two a step
 constexpr int kB4XCols = 64;                 // columns of x that come together
@@ -33,8 +33,6 @@ constexpr int kB4MaxSums = kB4SumColumns / 32;
 constexpr int kB4DequantWarps = 8 * kB4Pairs, kB4DoneWarps = 4;
 constexpr int kB4MmaWarp = kB4DequantWarps, kB4CopyWarp = kB4MmaWarp + 1, kB4CodeWarp = kB4CopyWarp + 1, kB4FirstDoneWarp = kB4CodeWarp + 1;
 constexpr int kB4Threads = 32 * (kB4FirstDoneWarp + kB4DoneWarps);
-constexpr int kB4RowsThreads = 256;
-constexpr uint32_t kB4WaitLimit = 1u << 20;
 constexpr int kB4SmemLimit = 232448;
 
 struct Batch4Dev {
@@ -45,121 +43,17 @@ struct Batch4Dev {
   int per_pass; int column_stride; int code_slots; int x_stages;
 };
 
-// Workspace: x in binary16 by steps of 64 columns, [group][hidden / 64][rows of the group, padded][128 bytes, swizzled]; x in BF16 [rows][hidden]; shift and bad [padded rows].
-__host__ __device__ inline int batch4_padded(int64_t rows) { return static_cast<int>((rows + 15) / 16 * 16); }
-__host__ inline size_t batch4_xt_bytes(int64_t rows, int64_t hidden) { return static_cast<size_t>(batch4_padded(rows)) * hidden * 2; }
-__host__ inline size_t batch4_xb_bytes(int64_t rows, int64_t hidden) { return (static_cast<size_t>(rows) * hidden * 2 + 255) / 256 * 256; }
-__host__ inline size_t batch4_workspace_bytes(int64_t rows, int64_t hidden) {
-  return batch4_xt_bytes(rows, hidden) + batch4_xb_bytes(rows, hidden) + 2 * (static_cast<size_t>(batch4_padded(rows)) * 4 + 255) / 256 * 256 + 512;
-}
 __host__ __device__ inline int batch4_x_stage_bytes(int n) { return n * kB4XCols * 2; }
 __host__ inline size_t batch4_smem_bytes(int n, int code_slots, int x_stages) {
   return 1024 + static_cast<size_t>(code_slots) * kB4SlotBytes + static_cast<size_t>(x_stages) * batch4_x_stage_bytes(n) + kB4MaxN * 4 + 512;
 }
 
-struct Rows4Dev {
-  const uint16_t* x; int64_t x_stride; int rows; int hidden;
-  const uint16_t* gamma; float eps; int one_plus;
-  uint8_t* xt; uint16_t* xb; int* shift; int* bad;
-};
+// ---- copies and products -------------------------------------------------------------------------------------------------------------------------------
 
-// One block: one (padded) row, a thread up to kB4Chunks chunks of 8 columns.
-constexpr int kB4Chunks = (kH4MaxHidden / 8 + kB4RowsThreads - 1) / kB4RowsThreads;
-static __global__ void __launch_bounds__(kB4RowsThreads) nvfp4_rows_kernel(Rows4Dev P) {
-  __shared__ float s_sum[kB4RowsThreads / 32];
-  __shared__ uint32_t s_top[kB4RowsThreads / 32];
-  after_predecessor();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x, chunks = P.hidden / 8;
-  const int group = row / kB4MaxN, in_group = row % kB4MaxN;
-  const int n = min(kB4MaxN, batch4_padded(P.rows) - group * kB4MaxN);
-  unsigned char* out = P.xt + static_cast<size_t>(group) * kB4MaxN * P.hidden * 2;
-  auto place = [&](int c) { return reinterpret_cast<uint4*>(out + (static_cast<size_t>(c >> 3) * n + in_group) * 128 + (((c & 7) ^ (in_group & 7)) << 4)); };   // 8 columns: 16 bytes
-  if (row >= P.rows) {
-    for (int c = tid; c < chunks; c += kB4RowsThreads) *place(c) = make_uint4(0u, 0u, 0u, 0u);
-    if (tid == 0) { P.shift[row] = 0; P.bad[row] = 0; }
-    return;
-  }
-  uint32_t w[kB4Chunks][4];
-  float ss = 0.0f;
-#pragma unroll
-  for (int u = 0; u < kB4Chunks; u++) {
-    w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
-    if (tid + u * kB4RowsThreads < chunks) load8(P.x + row * P.x_stride + 8 * (tid + u * kB4RowsThreads), w[u]);
-  }
-  if (P.gamma) {
-#pragma unroll
-    for (int u = 0; u < kB4Chunks; u++) ss += squares8(w[u]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-    if (lane == 0) s_sum[warp] = ss;
-    __syncthreads();
-    ss = 0.0f;
-#pragma unroll
-    for (int q = 0; q < kB4RowsThreads / 32; q++) ss += s_sum[q];
-    const float inv_rms = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(P.hidden)), P.eps));
-#pragma unroll
-    for (int u = 0; u < kB4Chunks; u++) {
-      if (tid + u * kB4RowsThreads < chunks) {
-        uint32_t gamma[4];
-        load8(P.gamma + 8 * (tid + u * kB4RowsThreads), gamma);
-        normalise8(w[u], gamma, inv_rms, P.one_plus);
-      }
-    }
-  }
-  uint32_t top = 0u;
-#pragma unroll
-  for (int u = 0; u < kB4Chunks; u++) top = max(top, top_of(w[u]));
-  top = warp_max_u32(top);
-  if (lane == 0) s_top[warp] = top;
-  __syncthreads();
-#pragma unroll
-  for (int q = 0; q < kB4RowsThreads / 32; q++) top = max(top, s_top[q]);
-  const int shift = shift_of(top);
-  bool bad = top >= 0x7F80u;
-#pragma unroll
-  for (int u = 0; u < kB4Chunks; u++) {
-    if (tid + u * kB4RowsThreads < chunks) {
-      *reinterpret_cast<uint4*>(P.xb + static_cast<size_t>(row) * P.hidden + 8 * (tid + u * kB4RowsThreads)) = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
-      bad |= !scaled8(w[u], scale_of(shift));
-    }
-  }
-  bad = __syncthreads_or(bad);
-#pragma unroll
-  for (int u = 0; u < kB4Chunks; u++)
-    if (tid + u * kB4RowsThreads < chunks) *place(tid + u * kB4RowsThreads) = bad ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
-  if (tid == 0) { P.shift[row] = shift; P.bad[row] = bad ? 1 : 0; }
-}
-
-// ---- barriers, copies and products --------------------------------------------------------------------------------------------------------------
-
-__device__ __forceinline__ uint32_t smem_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
-__device__ __forceinline__ void barrier_arrive(uint32_t bar, uint32_t count = 1u) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
-__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
-__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-  return done != 0u;
-}
-// False when the limit ran out here or the block has given up. (Out of line: the usual wait is over at the first or second look, and the roles' loops have to stay short.)
-__device__ __noinline__ bool barrier_wait_long(uint32_t bar, uint32_t parity, volatile uint32_t* given_up) {
-  for (uint32_t i = 0; i < kB4WaitLimit; i++) {
-    if (barrier_try(bar, parity)) return true;
-    if ((i & 15u) == 15u && *given_up) return false;
-  }
-  *given_up = 1u;
-  return false;
-}
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile uint32_t* given_up) {
-  return barrier_try(bar, parity) || barrier_wait_long(bar, parity, given_up);
-}
 __device__ __forceinline__ bool elected() {                                 // true in one lane of a warp that is together, always the same
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0u;
-}
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 // A box of 128 rows: 128 bytes of codes in the 128-byte swizzle, or 16 bytes of scales (columns a multiple of that; what lies beyond the matrix arrives as zeros).
 __device__ __forceinline__ void tile_copy(uint32_t dst, const CUtensorMap* map, int column, int row, uint32_t bar) {
@@ -226,16 +120,8 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     words[1] = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  after_predecessor();
-  const float g = __ldg(P.scale);
-  bool plain = true;                                                        // every g * 2^-shift is a normal binary32, with room for the sum
-  for (int r = tid; r < P.n; r += kB4Threads) {
-    const double f = static_cast<double>(g) * __hiloint2double((1023 - P.shift[r]) << 20, 0);
-    plain &= fabs(f) >= 0x1p-100 && fabs(f) <= 0x1p80;
-    factor[r] = static_cast<float>(f);
-  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  plain = __syncthreads_and(plain);
+  __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = words[0];
 
@@ -345,9 +231,10 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     }
     if (*given_up && one) {                                                 // what is under way ends before the block does
       products_commit(drained);
-      for (uint32_t i = 0; i < kB4WaitLimit && !barrier_try(drained, 0u); i++) {}
+      for (uint32_t i = 0; i < kWait4Limit && !barrier_try(drained, 0u); i++) {}
     }
   } else if (warp == kB4CopyWarp) {
+    after_predecessor();                                                    // (the weight's copies do not wait for the preparation of x: see lm_head_nvfp4_kernel)
     if (lane == 0) {
       int stage = 0, issued = 0; uint32_t phase = 0u;
       bool go = true;
@@ -365,7 +252,7 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
         for (int k = 0; k < P.x_stages && k < issued; k++) {
           if (stage == 0) { stage = P.x_stages; phase ^= 1u; }
           stage--;
-          for (uint32_t i = 0; i < kB4WaitLimit && !barrier_try(x_full + 8 * stage, phase); i++) {}
+          for (uint32_t i = 0; i < kWait4Limit && !barrier_try(x_full + 8 * stage, phase); i++) {}
         }
     }
   } else if (warp == kB4CodeWarp) {
@@ -392,13 +279,21 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
         for (int k = 0; k < P.code_slots && k < issued; k++) {
           if (slot == 0) { slot = P.code_slots; phase ^= 1u; }
           slot--;
-          for (uint32_t i = 0; i < kB4WaitLimit && !barrier_try(c_full + 8 * slot, phase); i++) {}
+          for (uint32_t i = 0; i < kWait4Limit && !barrier_try(c_full + 8 * slot, phase); i++) {}
         }
     }
   } else {
     // ---- finished accumulators: a warp has 32 vocabulary rows of every tile; a column is a row of logits
+    after_predecessor();
     const int part = warp & 3;
-    bool go = true;
+    const float g = __ldg(P.scale);
+    bool go = true, plain = true;                                           // plain: every g * 2^-shift is a normal binary32, with room for the sum
+    for (int r = lane; r < P.n; r += 32) {                                  // (each of these warps the same values)
+      const double f = static_cast<double>(g) * __hiloint2double((1023 - P.shift[r]) << 20, 0);
+      plain &= fabs(f) >= 0x1p-100 && fabs(f) <= 0x1p80;
+      factor[r] = static_cast<float>(f);
+    }
+    plain = __all_sync(kFull, plain);
     uint32_t phase = 0u;
     for (int first = begin; go && first < end; first += P.per_pass, phase ^= 1u) {
       const int last = min(first + P.per_pass, end);
@@ -432,6 +327,7 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     }
   }
   __syncwarp();
+  after_predecessor();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -447,22 +343,8 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     if (!P.bad[r]) continue;
     const uint16_t* x = P.xb + static_cast<size_t>(r) * H;
     for (int v = v0 + warp; v < v1; v += kB4Threads / 32) {
-      double sum = 0.0;
-      for (int w = lane; w < H / 8; w += 32) {
-        uint32_t h[4];
-        e2m1_to_f16(*reinterpret_cast<const uint32_t*>(P.codes + static_cast<int64_t>(v) * P.codes_stride + w * 4), h);
-        const float s = e4m3_value(P.scales[static_cast<int64_t>(v) * P.scales_stride + (w >> 1)]);
-        const uint4 xq = *reinterpret_cast<const uint4*>(x + 8 * w);
-        const uint32_t xw[4] = {xq.x, xq.y, xq.z, xq.w};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          sum += static_cast<double>(bf16_lo(xw[e])) * static_cast<double>(f16_lo(h[e]) * s);
-          sum += static_cast<double>(bf16_hi(xw[e])) * static_cast<double>(f16_hi(h[e]) * s);
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-      if (lane == 0) P.logits[r * P.logits_stride + v] = f32_to_bf16(head4_finish(sum, g, 0));
+      const double sum = exact_sum(x, P.codes + v * P.codes_stride, P.scales + v * P.scales_stride, H, lane);
+      if (lane == 0) P.logits[r * P.logits_stride + v] = f32_to_bf16(head4_finish(sum, __ldg(P.scale), 0));
     }
   }
 }

@@ -84,17 +84,21 @@ static bool head4_few_rows(int64_t rows, int64_t hidden) {
   return nt <= 1 || (nt <= kH4MaxNT && head4_smem_bytes(static_cast<int>(hidden), static_cast<int>(nt)) <= 200 * 1024);
 }
 
-static int head_nvfp4_few(void (*kernel)(Head4Dev), const Head4Dev& P, int nt, int sms, cudaStream_t st) {
+size_t lm_head_nvfp4_workspace_bytes(int64_t rows, int64_t hidden_dim) {
+  if (rows < 1 || hidden_dim < 1 || rows > LM_HEAD_NVFP4_MAX_ROWS || hidden_dim > kH4MaxHidden) return 0;
+  return x4_workspace_bytes(rows, hidden_dim);
+}
+
+static int head_nvfp4_few(void (*kernel)(Head4Dev), const lm_head_nvfp4_args* a, const Rows4Dev& R, int nt, int sms) {
+  Head4Dev P;
+  P.rows = R.rows; P.codes = a->codes; P.codes_stride = a->codes_stride; P.scales = a->scales; P.scales_stride = a->scales_stride; P.scale = a->scale;
+  P.hidden = R.hidden; P.vocab = static_cast<int>(a->vocab);
+  P.xt = R.xt; P.xb = R.xb; P.shift = R.shift; P.bad = R.bad; P.logits = static_cast<uint16_t*>(a->logits); P.logits_stride = a->logits_stride;
   const size_t smem = head4_smem_bytes(P.hidden, nt);
   const int rc = ensure_dynamic_smem(static_cast<KernelSlot>(kSlotHeadNvfp4 + nt - 1), reinterpret_cast<const void*>(kernel), smem);
   if (rc != LM_OK) return rc;
   const int tiles = (P.vocab + kH4Tile - 1) / kH4Tile;
-  return launch_beside(kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), kH4Threads, smem, 1, st, P);
-}
-
-size_t lm_head_nvfp4_workspace_bytes(int64_t rows, int64_t hidden_dim) {
-  if (hidden_dim < 1 || head4_few_rows(rows, hidden_dim) || rows > LM_HEAD_NVFP4_MAX_ROWS || hidden_dim > kH4MaxHidden) return 0;
-  return batch4_workspace_bytes(rows, hidden_dim);
+  return launch_stream(true, kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), kH4Threads, smem, 1, static_cast<cudaStream_t>(a->stream), P);
 }
 
 // A matrix of bytes that the copy engine reads in boxes of 128 rows by `width` bytes.
@@ -118,25 +122,13 @@ static int byte_map(const uint8_t* p, int64_t rows, int64_t bytes, int64_t strid
   return r == CUDA_SUCCESS ? LM_OK : cuda_fail(cudaErrorInvalidValue);
 }
 
-// More rows than a decode step has: the rows of x prepared once, then one launch for every 256 of them.
-static int head_nvfp4_batch(const lm_head_nvfp4_args* a, int sms) {
-  if (!a->workspace || misaligned(a->workspace, 256) || a->workspace_bytes < batch4_workspace_bytes(a->rows, a->hidden_dim)) return LM_E_WORKSPACE;
+// More rows: a launch for every 256 of them.
+static int head_nvfp4_batch(const lm_head_nvfp4_args* a, const Rows4Dev& R, int sms) {
   cudaStream_t st = static_cast<cudaStream_t>(a->stream);
-  unsigned char* ws = static_cast<unsigned char*>(a->workspace);
-  const int padded = batch4_padded(a->rows);
-  Rows4Dev R;
-  R.x = static_cast<const uint16_t*>(a->hidden); R.x_stride = a->hidden_stride; R.rows = static_cast<int>(a->rows); R.hidden = static_cast<int>(a->hidden_dim);
-  R.gamma = static_cast<const uint16_t*>(a->norm_weight); R.eps = a->eps; R.one_plus = a->one_plus;
-  R.xt = ws; ws += batch4_xt_bytes(a->rows, a->hidden_dim);
-  ws = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~static_cast<uintptr_t>(255));
-  R.xb = reinterpret_cast<uint16_t*>(ws); ws += batch4_xb_bytes(a->rows, a->hidden_dim);
-  R.shift = reinterpret_cast<int*>(ws); R.bad = R.shift + padded;
-  int rc = launch_beside(nvfp4_rows_kernel, dim3(static_cast<unsigned>(padded)), kB4RowsThreads, 0, 1, st, R);
-  if (rc != LM_OK) return rc;
   Batch4Dev P;
   P.codes = a->codes; P.codes_stride = a->codes_stride; P.scales = a->scales; P.scales_stride = a->scales_stride; P.scale = a->scale;
   P.hidden = R.hidden; P.vocab = static_cast<int>(a->vocab); P.logits_stride = a->logits_stride;
-  rc = ensure_dynamic_smem(kSlotHeadNvfp4Batch, reinterpret_cast<const void*>(lm_head_nvfp4_batch_kernel), kB4SmemLimit);
+  int rc = ensure_dynamic_smem(kSlotHeadNvfp4Batch, reinterpret_cast<const void*>(lm_head_nvfp4_batch_kernel), kB4SmemLimit);
   if (rc != LM_OK) return rc;
   CUtensorMap code_map, scale_map;
   rc = byte_map(a->codes, P.vocab, P.hidden / 2, a->codes_stride, kB4StepCols / 2, CU_TENSOR_MAP_SWIZZLE_128B, &code_map);
@@ -145,7 +137,7 @@ static int head_nvfp4_batch(const lm_head_nvfp4_args* a, int sms) {
   const int tiles = (P.vocab + kB4Tile - 1) / kB4Tile;
   for (int64_t r = 0; r < a->rows; r += kB4MaxN) {
     P.rows = static_cast<int>(a->rows - r < kB4MaxN ? a->rows - r : kB4MaxN);
-    P.n = batch4_padded(P.rows);
+    P.n = x4_padded(P.rows);
     P.xt = R.xt + static_cast<size_t>(r) * R.hidden * 2; P.xb = R.xb + static_cast<size_t>(r) * R.hidden; P.shift = R.shift + r; P.bad = R.bad + r;
     P.logits = static_cast<uint16_t*>(a->logits) + r * a->logits_stride;
     P.column_stride = P.n <= 32 ? 32 : P.n <= 64 ? 64 : P.n <= 128 ? 128 : 256;
@@ -171,22 +163,26 @@ int lm_head_nvfp4(const lm_head_nvfp4_args* a) {
   if (a->rows > LM_HEAD_NVFP4_MAX_ROWS || a->vocab > LM_MAX_VOCAB || (a->hidden_dim % 64) != 0 || a->hidden_dim > kH4MaxHidden) return LM_E_UNSUPPORTED;
   if (a->codes_stride > 0x7FFFFFFF || a->scales_stride > 0x7FFFFFFF) return LM_E_UNSUPPORTED;
   if (misaligned(a->codes, 16) || (a->codes_stride % 16) != 0 || misaligned(a->scales, 16) || (a->scales_stride % 16) != 0) return LM_E_UNSUPPORTED;   // 16-byte copies
-  Head4Dev P;
-  P.x_stride = a->hidden_stride;
-  P.codes = a->codes; P.codes_stride = a->codes_stride; P.scales = a->scales; P.scales_stride = a->scales_stride; P.scale = a->scale;
-  P.hidden = static_cast<int>(a->hidden_dim); P.vocab = static_cast<int>(a->vocab);
-  P.gamma = static_cast<const uint16_t*>(a->norm_weight); P.eps = a->eps; P.one_plus = a->one_plus; P.logits_stride = a->logits_stride;
+  if (!a->workspace || misaligned(a->workspace, 256) || a->workspace_bytes < x4_workspace_bytes(a->rows, a->hidden_dim)) return LM_E_WORKSPACE;
   int sms = 0;
   rc = sm_count(&sms);
   if (rc != LM_OK) return rc;
-  if (!head4_few_rows(a->rows, P.hidden)) return head_nvfp4_batch(a, sms);
-  P.x = static_cast<const uint16_t*>(a->hidden); P.logits = static_cast<uint16_t*>(a->logits); P.rows = static_cast<int>(a->rows);
-  cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  Rows4Dev R;
+  unsigned char* ws = static_cast<unsigned char*>(a->workspace);
+  const int padded = x4_padded(a->rows);
+  R.x = static_cast<const uint16_t*>(a->hidden); R.x_stride = a->hidden_stride; R.rows = static_cast<int>(a->rows); R.hidden = static_cast<int>(a->hidden_dim);
+  R.gamma = static_cast<const uint16_t*>(a->norm_weight); R.eps = a->eps; R.one_plus = a->one_plus; R.few = head4_few_rows(a->rows, a->hidden_dim) ? 1 : 0;
+  R.xt = ws; ws += x4_xt_bytes(a->rows, a->hidden_dim);
+  R.xb = reinterpret_cast<uint16_t*>(ws); ws += x4_xb_bytes(a->rows, a->hidden_dim);
+  R.shift = reinterpret_cast<int*>(ws); R.bad = R.shift + padded;
+  rc = launch_beside(nvfp4_rows_kernel, dim3(static_cast<unsigned>(R.few ? R.rows : padded)), kX4Threads, 0, 1, static_cast<cudaStream_t>(a->stream), R);
+  if (rc != LM_OK) return rc;
+  if (!R.few) return head_nvfp4_batch(a, R, sms);
   switch ((a->rows + kH4Rows - 1) / kH4Rows) {
-    case 1: return head_nvfp4_few(lm_head_nvfp4_kernel<1, 4>, P, 1, sms, st);
-    case 2: return head_nvfp4_few(lm_head_nvfp4_kernel<2, 3>, P, 2, sms, st);
-    case 3: return head_nvfp4_few(lm_head_nvfp4_kernel<3, 2>, P, 3, sms, st);
-    default: return head_nvfp4_few(lm_head_nvfp4_kernel<4, 2>, P, 4, sms, st);
+    case 1: return head_nvfp4_few(lm_head_nvfp4_kernel<1, 4>, a, R, 1, sms);
+    case 2: return head_nvfp4_few(lm_head_nvfp4_kernel<2, 3>, a, R, 2, sms);
+    case 3: return head_nvfp4_few(lm_head_nvfp4_kernel<3, 2>, a, R, 3, sms);
+    default: return head_nvfp4_few(lm_head_nvfp4_kernel<4, 2>, a, R, 4, sms);
   }
 }
 
