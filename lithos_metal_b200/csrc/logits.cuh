@@ -3,18 +3,18 @@
 // Per row r, with c_all the occurrences of a token in history[r, :len] and c_out those from position prompt_len on:
 //   z = float(logit); c_all > 0: z = z > 0 ? z / rho : z * rho; c_out > 0: z = (z - pi) - phi * c_out; z += the token's biases, in list order; masked: -inf.
 // The penalties touch as many logits as the history has tokens, the biases as many as their list; a mask usually touches most. So a row is cut into slices, a block
-// each. A block streams its slice once (16 bytes a load; out of place: copy and mask; in place: only words of the mask that are not all ones or all zeros are read,
-// without a mask nothing is) and then sets the few logits of its slice that a list names. Which those are, and how often, is counted in shared memory
-// addressed by the token (nothing can overflow, no order matters): words are cleared only where a list names them. The first thread to claim a token sets it.
+// each. Which of its slice's tokens the history holds, and how often, a block counts in shared memory addressed by the token (nothing can overflow, no order matters): a bit per token, and a word
+// of counts that is cleared only where a bit is set. It streams its slice once, 16 bytes a load, several under way per thread since before the counting: copied, masked and penalised on the way
+// (in place: only what changes is written, and read where a mask keeps some of eight). A token with a bias is set behind that by its (first) entry of the list. In place without a mask only the
+// tokens the lists name are touched.
 #pragma once
 #include "common.cuh"
 
 namespace lm {
 
 constexpr int kLogitsThreads = 512;
-constexpr int kLogitsMaxSlice = 12288;       // logits per slice at most: 48 KB of counts (96 with biases)
+constexpr int kLogitsMaxSlice = 24576;       // logits per slice at most: 96 KB of counts, two blocks to an SM
 constexpr int kLogitsMinSlice = 1024;
-
 struct LogitsDev {
   const void* in; int64_t in_stride; void* out; int64_t out_stride; int in_place;
   int rows; int vocab;
@@ -41,38 +41,55 @@ template <bool F32> __device__ __forceinline__ void set_logit(void* row, int64_t
   if (F32) static_cast<float*>(row)[i] = z; else static_cast<uint16_t*>(row)[i] = __bfloat16_as_ushort(__float2bfloat16_rn(z));
 }
 
-// Eight logits under the bits of `keep`.
+// Eight logits; those whose bit of `keep` is clear become -inf.
+__device__ __forceinline__ uint32_t two_kept(uint32_t w, uint32_t keep) {    // of two BF16: bytes of w or of two -inf
+  return __byte_perm(w, 0xFF80FF80u, 0x7654u - (keep & 1u) * 0x44u - (keep & 2u) * 0x2200u);
+}
 template <bool F32> struct Chunk;
 template <> struct Chunk<false> {
   uint4 q;
   __device__ __forceinline__ void load(const void* p) { q = __ldcs(static_cast<const uint4*>(p)); }
   __device__ __forceinline__ void store(void* p) const { *static_cast<uint4*>(p) = q; }
-  static __device__ __forceinline__ uint32_t two(uint32_t w, uint32_t keep) {
-    return (keep & 1u ? w & 0xFFFFu : 0xFF80u) | (keep & 2u ? w & 0xFFFF0000u : 0xFF800000u);
+  __device__ __forceinline__ void apply(uint32_t keep) { q.x = two_kept(q.x, keep); q.y = two_kept(q.y, keep >> 2); q.z = two_kept(q.z, keep >> 4); q.w = two_kept(q.w, keep >> 6); }
+  __device__ __forceinline__ float get(int e) const {
+    const uint32_t w = e & 4 ? (e & 2 ? q.w : q.z) : (e & 2 ? q.y : q.x);
+    return e & 1 ? bf16_hi(w) : bf16_lo(w);
   }
-  __device__ __forceinline__ void apply(uint32_t keep) {
-    if (keep == 0xFFu) return;
-    q.x = two(q.x, keep); q.y = two(q.y, keep >> 2); q.z = two(q.z, keep >> 4); q.w = two(q.w, keep >> 6);
+  __device__ __forceinline__ void set(int e, float z) {
+    const uint32_t h = __bfloat16_as_ushort(__float2bfloat16_rn(z)), sel = e & 1 ? 0x5410u : 0x3254u;      // h in the upper or the lower half
+    const int i = e >> 1;
+    q.x = i == 0 ? __byte_perm(q.x, h, sel) : q.x; q.y = i == 1 ? __byte_perm(q.y, h, sel) : q.y; q.z = i == 2 ? __byte_perm(q.z, h, sel) : q.z; q.w = i == 3 ? __byte_perm(q.w, h, sel) : q.w;
   }
 };
 template <> struct Chunk<true> {
-  uint4 a, b;
-  __device__ __forceinline__ void load(const void* p) { a = __ldcs(static_cast<const uint4*>(p)); b = __ldcs(static_cast<const uint4*>(p) + 1); }
-  __device__ __forceinline__ void store(void* p) const { static_cast<uint4*>(p)[0] = a; static_cast<uint4*>(p)[1] = b; }
+  uint32_t v[8];
+  __device__ __forceinline__ void load(const void* p) {
+    const uint4 a = __ldcs(static_cast<const uint4*>(p)), b = __ldcs(static_cast<const uint4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  __device__ __forceinline__ void store(void* p) const { static_cast<uint4*>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]); static_cast<uint4*>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]); }
   __device__ __forceinline__ void apply(uint32_t keep) {
-    if (keep == 0xFFu) return;
-    const uint32_t m = 0xFF800000u;
-    if (!(keep & 1u)) a.x = m; if (!(keep & 2u)) a.y = m; if (!(keep & 4u)) a.z = m; if (!(keep & 8u)) a.w = m;
-    if (!(keep & 16u)) b.x = m; if (!(keep & 32u)) b.y = m; if (!(keep & 64u)) b.z = m; if (!(keep & 128u)) b.w = m;
+#pragma unroll
+    for (int e = 0; e < 8; e++) if (!((keep >> e) & 1u)) v[e] = 0xFF800000u;
+  }
+  __device__ __forceinline__ float get(int e) const {
+    uint32_t r = v[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) r = i == e ? v[i] : r;
+    return __uint_as_float(r);
+  }
+  __device__ __forceinline__ void set(int e, float z) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = i == e ? __float_as_uint(z) : v[i];
   }
 };
 
 template <bool F32>
-static __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(LogitsDev P) {
+static __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(LogitsDev P) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   uint32_t* counts = reinterpret_cast<uint32_t*>(smem_raw);                // [slice]
-  uint32_t* first = counts + P.slice;                                       // [slice], with biases: the token's first entry
-  constexpr int kSize = F32 ? 4 : 2;
+  uint32_t* named = counts + P.slice;                                       // [slice / 32 + 1] a bit for every token of the history
+  constexpr int kSize = F32 ? 4 : 2, kAhead = F32 ? 4 : 6;
   const int tid = threadIdx.x;
   after_predecessor();
   const long long items = static_cast<long long>(P.rows) * P.slices;
@@ -80,101 +97,143 @@ static __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(LogitsDev
     const int row = static_cast<int>(item / P.slices), lo = static_cast<int>(item % P.slices) * P.slice, hi = min(lo + P.slice, P.vocab);
     const unsigned char* in = static_cast<const unsigned char*>(P.in) + row * P.in_stride * kSize;
     unsigned char* out = static_cast<unsigned char*>(P.out) + row * P.out_stride * kSize;
-    const uint32_t* mask = nullptr;                                         // the row's words, or none
-    bool nothing = false;                                                   // the row's mask does not exist: everything is masked
-    if (P.mask) {
-      const int m = P.mask_rows ? P.mask_rows[row] : row;
-      if (m >= P.mask_count) nothing = true; else if (m >= 0) mask = P.mask + m * P.mask_stride;
-    }
+    const int which = P.mask ? (P.mask_rows ? P.mask_rows[row] : row) : -1;
     const int n_hist = P.history ? min(P.lengths ? max(P.lengths[row], 0) : P.hist_len, P.hist_len) : 0;
-    const int n_bias = P.bias_len;
+    const int n_bias = P.bias_len, prompt = P.prompts ? P.prompts[row] : 0;
+    const float rho = P.rho ? P.rho[row] : P.rho_s, pi = P.pi ? P.pi[row] : P.pi_s, phi = P.phi ? P.phi[row] : P.phi_s;
+    const bool nothing = which >= P.mask_count && which >= 0;               // the row's mask does not exist: everything is masked
+    const uint8_t* mask = which >= 0 && !nothing ? reinterpret_cast<const uint8_t*>(P.mask + which * P.mask_stride) : nullptr;     // the row's bits, or none
+    const bool stream = !P.in_place || mask || nothing;
+    const uint32_t width = static_cast<uint32_t>(hi - lo);
+    auto keeps = [&](int v) { return !nothing && (!mask || ((mask[v >> 3] >> (v & 7)) & 1u)); };
+    // ---- the slice: [lo, head) singly, then chunks of 8 from 16-byte boundaries, then the rest singly
+    int head = lo, chunks = 0;
+    if (stream && ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(out) + static_cast<uintptr_t>(lo) * kSize;
+      head = min(lo + static_cast<int>(((16u - (at & 15u)) & 15u) / kSize), hi);
+      chunks = (hi - head) / 8;
+    }
+    const int shift = head & 7;                                              // of a chunk's bits in their byte (lo is a multiple of 32)
+    // chunk c: its logits at in8 + c * 8 * kSize, its bits from mask8[c] on
+    const unsigned char* in8 = in + static_cast<int64_t>(head) * kSize;
+    unsigned char* out8 = out + static_cast<int64_t>(head) * kSize;
+    const uint8_t* mask8 = mask ? mask + (head >> 3) : nullptr;
+    auto bits_of = [&](const uint8_t* p, int c) -> uint32_t { return shift == 0 ? p[c] : ((p[c] | static_cast<uint32_t>(p[c + 1]) << 8) >> shift) & 0xFFu; };
+    Chunk<F32> x[kAhead];
+    uint32_t keep[kAhead];
+    auto load_bits = [&](int c0) {
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) {
+        keep[u] = nothing ? 0u : 0xFFu;
+        if (mask8 && c0 + u * kLogitsThreads < chunks) keep[u] = bits_of(mask8, c0 + u * kLogitsThreads);
+      }
+    };
+    auto load = [&](int c0) {
+      const unsigned char* p = in8 + static_cast<int64_t>(c0) * (8 * kSize);
+#pragma unroll
+      for (int u = 0; u < kAhead; u++)
+        if (c0 + u * kLogitsThreads < chunks && keep[u] != 0u && !(P.in_place && keep[u] == 0xFFu)) x[u].load(p + u * (kLogitsThreads * 8 * kSize));
+    };
+    load_bits(tid);
+    load(tid);
+    // ---- counts, while the first chunks are on their way
     const int32_t* hist = P.history + row * P.hist_stride;
     const int32_t* ids = P.bias_ids + row * P.bias_ids_stride;
-    const uint32_t width = static_cast<uint32_t>(hi - lo);
-    auto keeps = [&](int v) { return !nothing && (!mask || ((mask[v >> 5] >> (v & 31)) & 1u)); };
-    // ---- counts
-    if (!nothing) {
-      for (int i = tid; i < n_hist; i += kLogitsThreads) { const uint32_t v = static_cast<uint32_t>(hist[i]) - lo; if (v < width) { counts[v] = 0u; if (n_bias) first[v] = 0xFFFFFFFFu; } }
-      for (int i = tid; i < n_bias; i += kLogitsThreads) { const uint32_t v = static_cast<uint32_t>(ids[i]) - lo; if (v < width) { counts[v] = 0u; first[v] = 0xFFFFFFFFu; } }
+    const bool lists = !nothing && (n_hist || n_bias);
+    // f(token in the slice, behind the prompt) for the history's tokens in the slice
+    auto each_token = [&](auto f) {
+      const bool fours = (reinterpret_cast<uintptr_t>(hist) & 15u) == 0;
+      for (int i = 4 * tid; i < n_hist; i += 4 * kLogitsThreads) {
+        int t[4];
+        if (fours && i + 4 <= n_hist) { const int4 q = __ldg(reinterpret_cast<const int4*>(hist + i)); t[0] = q.x; t[1] = q.y; t[2] = q.z; t[3] = q.w; }
+        else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) t[e] = i + e < n_hist ? hist[i + e] : -1;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) { const uint32_t v = static_cast<uint32_t>(t[e]) - static_cast<uint32_t>(lo); if (v < width) f(v, i + e >= prompt); }     // (-1, padding: never below a width)
+      }
+    };
+    auto penalised = [&](float z, uint32_t n) {
+      if (n & (kSeen | kOutMask)) z = (z > 0.0f) ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
+      if (n & kOutMask) z = __fsub_rn(__fsub_rn(z, pi), __fmul_rn(phi, static_cast<float>(n & kOutMask)));
+      return z;
+    };
+    if (lists) {
+      for (int i = tid; i < P.slice / 32 + 1; i += kLogitsThreads) named[i] = 0u;
+      if (n_hist) each_token([&](uint32_t v, bool) { counts[v] = 0u; });
+      for (int i = tid; i < n_bias; i += kLogitsThreads) { const uint32_t v = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(lo); if (v < width) counts[v] = 0u; }
       __syncthreads();
-      const int prompt = P.prompts ? P.prompts[row] : 0;
-      for (int i = tid; i < n_hist; i += kLogitsThreads) {
-        const uint32_t v = static_cast<uint32_t>(hist[i]) - lo;
-        if (v < width) { atomicOr(&counts[v], kSeen); if (i >= prompt) atomicAdd(&counts[v], 1u); }
-      }
-      for (int i = tid; i < n_bias; i += kLogitsThreads) {
-        const uint32_t v = static_cast<uint32_t>(ids[i]) - lo;
-        if (v < width) { atomicAdd(&counts[v], kBiasOne); atomicMin(&first[v], static_cast<uint32_t>(i)); }
-      }
+      if (n_hist) each_token([&](uint32_t v, bool behind) {
+        if (behind) atomicAdd(&counts[v], 1u); else atomicOr(&counts[v], kSeen);
+        atomicOr(&named[v >> 5], 1u << (v & 31));
+      });
+      for (int i = tid; i < n_bias; i += kLogitsThreads) { const uint32_t v = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(lo); if (v < width) atomicAdd(&counts[v], kBiasOne); }
+      __syncthreads();
     }
-    // ---- the slice
-    if (!P.in_place || mask || nothing) {
-      const bool together = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0 && (reinterpret_cast<uintptr_t>(in) & (kSize - 1)) == 0;
-      int head = lo, chunks = 0;                                            // [lo, head) singly, then chunks of 8 from 16-byte boundaries, then the rest singly
-      if (together) {
-        const uintptr_t at = reinterpret_cast<uintptr_t>(out) + static_cast<uintptr_t>(lo) * kSize;
-        head = min(lo + static_cast<int>(((16u - (at & 15u)) & 15u) / kSize), hi);
-        chunks = (hi - head) / 8;
-      }
+    const bool penalise_here = lists && n_hist;
+    if (stream) {
       const int tail = head + 8 * chunks, singles = (head - lo) + (hi - tail);
       for (int i = tid; i < singles; i += kLogitsThreads) {
         const int v = i < head - lo ? lo + i : tail + (i - (head - lo));
         if (!keeps(v)) set_logit<F32>(out, v, -INFINITY);
+        else if (penalise_here && ((named[(v - lo) >> 5] >> ((v - lo) & 31)) & 1u) && !(counts[v - lo] & kBiasMask)) set_logit<F32>(out, v, penalised(logit_at<F32>(in, v), counts[v - lo]));
         else if (!P.in_place) {
           if (F32) reinterpret_cast<uint32_t*>(out)[v] = reinterpret_cast<const uint32_t*>(in)[v]; else reinterpret_cast<uint16_t*>(out)[v] = reinterpret_cast<const uint16_t*>(in)[v];
         }
       }
-      const int last = (P.vocab - 1) >> 5;
-      auto bits8 = [&](int v) -> uint32_t {                                  // the mask's bits of v .. v + 7
-        if (nothing) return 0u;
-        if (!mask) return 0xFFu;
-        const int w = v >> 5;
-        return __funnelshift_r(__ldg(mask + w), __ldg(mask + min(w + 1, last)), v & 31) & 0xFFu;
-      };
-      constexpr int kAhead = F32 ? 2 : 4;
-      for (int c0 = tid; c0 < chunks; c0 += kLogitsThreads * kAhead) {
-        Chunk<F32> x[kAhead];
-        uint32_t keep[kAhead];
+      const uint8_t* named8 = reinterpret_cast<const uint8_t*>(named) + ((head - lo) >> 3);
+      const uint32_t* counts8 = counts + (head - lo);
+      for (int c0 = tid; c0 < chunks;) {
+        unsigned char* p = out8 + static_cast<int64_t>(c0) * (8 * kSize);
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
           const int c = c0 + u * kLogitsThreads;
-          keep[u] = c < chunks ? bits8(head + 8 * c) : 0u;
-          if (c < chunks && keep[u] != 0u && !(P.in_place && keep[u] == 0xFFu)) x[u].load(in + static_cast<int64_t>(head + 8 * c) * kSize);
+          if (c >= chunks) break;
+          uint32_t touched = penalise_here ? bits_of(named8, c) & keep[u] : 0u;
+          if (P.in_place && keep[u] == 0xFFu) {                             // (not loaded: what is named is set singly)
+            for (; touched; touched &= touched - 1u) {
+              const int v = 8 * c + __ffs(static_cast<int>(touched)) - 1;
+              if (!(counts8[v] & kBiasMask)) set_logit<F32>(out8, v, penalised(logit_at<F32>(in8, v), counts8[v]));
+            }
+            continue;
+          }
+          for (; touched; touched &= touched - 1u) {
+            const int e = __ffs(static_cast<int>(touched)) - 1;
+            const uint32_t n = counts8[8 * c + e];
+            if (!(n & kBiasMask)) x[u].set(e, penalised(x[u].get(e), n));    // (with a bias: set below, from the logit itself)
+          }
+          if (keep[u] != 0xFFu) x[u].apply(keep[u]);
+          x[u].store(p + u * (kLogitsThreads * 8 * kSize));
         }
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-          const int c = c0 + u * kLogitsThreads;
-          if (c >= chunks || (P.in_place && keep[u] == 0xFFu)) continue;
-          x[u].apply(keep[u]);
-          x[u].store(out + static_cast<int64_t>(head + 8 * c) * kSize);
-        }
+        c0 += kLogitsThreads * kAhead;
+        if (c0 < chunks) { load_bits(c0); load(c0); }
       }
     }
-    __syncthreads();
-    // ---- the logits that the lists name
-    if (!nothing && (n_hist || n_bias)) {
-      const float rho = P.rho ? P.rho[row] : P.rho_s, pi = P.pi ? P.pi[row] : P.pi_s, phi = P.phi ? P.phi[row] : P.phi_s;
-      for (int i = tid; i < n_hist + n_bias; i += kLogitsThreads) {
-        const uint32_t v = static_cast<uint32_t>(i < n_hist ? hist[i] : ids[i - n_hist]) - lo;
-        if (v >= width) continue;
-        const uint32_t n = atomicOr(&counts[v], kClaimed);
-        if (n & kClaimed) continue;
+    // ---- tokens of the history where nothing was streamed, and those with a bias
+    if (lists && (!stream || n_bias)) {
+      __syncthreads();
+      if (!stream && n_hist) each_token([&](uint32_t v, bool) {
+        const uint32_t n = atomicOr(&counts[v], kClaimed);                  // (the first thread to claim a token sets it)
         const int id = lo + static_cast<int>(v);
-        if (!keeps(id)) continue;
-        float z = logit_at<F32>(in, id);
-        if (n & kSeen) z = (z > 0.0f) ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
-        if (n & kOutMask) z = __fsub_rn(__fsub_rn(z, pi), __fmul_rn(phi, static_cast<float>(n & kOutMask)));
-        if (n & kBiasMask) {
-          const float* values = P.bias_values + row * P.bias_values_stride;
-          int e = static_cast<int>(first[v]);
-          z = __fadd_rn(z, values[e]);
-          for (int left = static_cast<int>((n & kBiasMask) / kBiasOne) - 1; left > 0;)           // (a token listed more than once: its values in list order)
-            if (++e < n_bias) { if (ids[e] == id) { z = __fadd_rn(z, values[e]); left--; } } else break;
-        }
+        if (!(n & (kClaimed | kBiasMask))) set_logit<F32>(out, id, penalised(logit_at<F32>(in, id), n));
+      });
+      const float* values = P.bias_values + row * P.bias_values_stride;
+      for (int i = tid; i < n_bias; i += kLogitsThreads) {
+        const int id = ids[i];
+        const uint32_t v = static_cast<uint32_t>(id) - static_cast<uint32_t>(lo);
+        if (v >= width || !keeps(id)) continue;
+        const uint32_t n = counts[v];
+        int others = static_cast<int>((n & kBiasMask) / kBiasOne) - 1;       // (a token listed more than once: the first entry adds all values in list order)
+        bool first = true;
+        for (int e = 0; others > 0 && first && e < i; e++) first = ids[e] != id;
+        if (!first) continue;
+        float z = __fadd_rn(penalised(logit_at<F32>(in, id), n), values[i]);
+        for (int e = i + 1; others > 0 && e < n_bias; e++) if (ids[e] == id) { z = __fadd_rn(z, values[e]); others--; }
         set_logit<F32>(out, id, z);
       }
     }
-    __syncthreads();                                                        // the tables are the next slice's
+    if (lists) __syncthreads();                                             // the tables are the next slice's
   }
 }
 

@@ -226,15 +226,15 @@ int lm_process_logits(const lm_logits_args* a) {
   P.rho = a->repetition; P.rho_s = a->repetition_s; P.pi = a->presence; P.pi_s = a->presence_s; P.phi = a->frequency; P.phi_s = a->frequency_s;
   P.bias_ids = a->bias_ids; P.bias_ids_stride = a->bias_ids_stride; P.bias_values = a->bias_values; P.bias_values_stride = a->bias_values_stride; P.bias_len = static_cast<int>(a->bias_len);
   P.mask = a->mask; P.mask_stride = a->mask_stride; P.mask_rows = a->mask_rows; P.mask_count = static_cast<int>(a->mask_count);
-  // slices: as many as give every SM four blocks, within the bounds of the tables
+  // slices: as few as give every SM two blocks of work, within the bounds of the table
   const long long total = static_cast<long long>(a->rows) * a->vocab;
-  long long per = (total / (4LL * sms) + 255) / 256 * 256;
+  long long per = (total / (2LL * sms) + 255) / 256 * 256;
   if (per < kLogitsMinSlice) per = kLogitsMinSlice;
   if (per > kLogitsMaxSlice) per = kLogitsMaxSlice;
   P.slices = static_cast<int>((a->vocab + per - 1) / per);
   P.slice = static_cast<int>(((a->vocab + P.slices - 1) / P.slices + 31) / 32 * 32);
   P.slices = static_cast<int>((a->vocab + P.slice - 1) / P.slice);
-  const size_t smem = lists ? static_cast<size_t>(P.slice) * 4 * (a->bias_len > 0 ? 2 : 1) : 0;
+  const size_t smem = lists ? static_cast<size_t>(P.slice) * 4 + P.slice / 8 + 16 : 0;
   const bool f32 = a->dtype == LM_DTYPE_F32;
   rc = ensure_dynamic_smem(f32 ? kSlotLogitsF32 : kSlotLogits, f32 ? reinterpret_cast<const void*>(logits_kernel<true>) : reinterpret_cast<const void*>(logits_kernel<false>), smem);
   if (rc != LM_OK) return rc;
