@@ -2,19 +2,22 @@
 //
 // Per row r, with c_all the occurrences of a token in history[r, :len] and c_out those from position prompt_len on:
 //   z = float(logit); c_all > 0: z = z > 0 ? z / rho : z * rho; c_out > 0: z = (z - pi) - phi * c_out; z += the token's biases, in list order; masked: -inf.
-// The penalties touch as many logits as the history has tokens, the biases as many as their list; a mask usually touches most. So a row is cut into slices, a block
-// each. Which of its slice's tokens the history holds, and how often, a block counts in shared memory addressed by the token (nothing can overflow, no order matters): a bit per token, and a word
-// of counts that is cleared only where a bit is set. It streams its slice once, 16 bytes a load, several under way per thread since before the counting: copied, masked and penalised on the way
-// (in place: only what changes is written, and read where a mask keeps some of eight). A token with a bias is set behind that by its (first) entry of the list. In place without a mask only the
-// tokens the lists name are touched.
+// The penalties touch as many logits as the history has tokens, the biases as many as their list; a mask usually touches most. A block has a row, or a slice of one where there are few. It
+// looks through the row's lists once: a bit in shared memory for every token of the history in its slice, and a hash table of these and the biased tokens with their counts (its size is given by
+// the lists' lengths, or by the slice's width: it never fills up). Then it streams the slice, 16 bytes a load, four under way per thread: copied and masked (in place: only what changes is
+// written, and read where a mask keeps some of eight), and logits whose bit is set are looked up and penalised in the registers that hold them. Tokens with a bias are set behind that, by their
+// (first) entry of the list. In place without a mask only the tokens that the lists name are touched.
 #pragma once
 #include "common.cuh"
 
 namespace lm {
 
 constexpr int kLogitsThreads = 512;
-constexpr int kLogitsMaxSlice = 24576;       // logits per slice at most: 96 KB of counts, two blocks to an SM
+constexpr int kLogitsPerSM = 3;              // blocks
 constexpr int kLogitsMinSlice = 1024;
+constexpr int kLogitsMaxTable = 16384;       // entries of the hash table, 8 bytes each
+constexpr int kLogitsMaxNamed = 12288;       // tokens in it at most
+
 struct LogitsDev {
   const void* in; int64_t in_stride; void* out; int64_t out_stride; int in_place;
   int rows; int vocab;
@@ -22,15 +25,14 @@ struct LogitsDev {
   const float* rho; float rho_s; const float* pi; float pi_s; const float* phi; float phi_s;
   const int32_t* bias_ids; int64_t bias_ids_stride; const float* bias_values; int64_t bias_values_stride; int bias_len;
   const uint32_t* mask; int64_t mask_stride; const int32_t* mask_rows; int mask_count;
-  int slice; int slices;
+  int slice; int slices; int table_log2;     // the table has 2^table_log2 entries
 };
 
-// a token's word of counts
+// a token's counts
 constexpr uint32_t kOutMask = 0x1FFFFu;      // bits 0..16: occurrences behind the prompt
 constexpr uint32_t kBiasOne = 1u << 17;      // bits 17..29: its biases (8191 at most)
 constexpr uint32_t kBiasMask = 0x1FFFu << 17;
 constexpr uint32_t kSeen = 1u << 30;         // it occurs
-constexpr uint32_t kClaimed = 1u << 31;
 constexpr int kLogitsMaxHistory = 65536;
 constexpr int kLogitsMaxBias = 8191;
 
@@ -84,12 +86,31 @@ template <> struct Chunk<true> {
   }
 };
 
-template <bool F32>
-static __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(LogitsDev P) {
+// A hash table of tokens in shared memory, linear probing.
+constexpr uint32_t kNoToken = 0xFFFFFFFFu;
+struct TokenTable {
+  uint32_t* key; uint32_t* count; int log2;
+  __device__ __forceinline__ uint32_t home(uint32_t v) const { return (v * 2654435769u) >> (32 - log2); }     // (2^32 over the golden ratio: neighbours lie apart)
+  __device__ __forceinline__ uint32_t insert(uint32_t v) const {
+    for (uint32_t i = home(v);; i = (i + 1u) & ((1u << log2) - 1u)) {
+      const uint32_t k = atomicCAS(&key[i], kNoToken, v);
+      if (k == kNoToken || k == v) return i;
+    }
+  }
+  __device__ __forceinline__ uint32_t find(uint32_t v) const {               // (of a token that is there)
+    uint32_t i = home(v);
+    while (key[i] != v) i = (i + 1u) & ((1u << log2) - 1u);
+    return i;
+  }
+};
+
+// kLists: there is a history or a bias list.
+template <bool F32, bool kLists>
+static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_kernel(LogitsDev P) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  uint32_t* counts = reinterpret_cast<uint32_t*>(smem_raw);                // [slice]
-  uint32_t* named = counts + P.slice;                                       // [slice / 32 + 1] a bit for every token of the history
-  constexpr int kSize = F32 ? 4 : 2, kAhead = F32 ? 4 : 6;
+  const TokenTable table{reinterpret_cast<uint32_t*>(smem_raw), reinterpret_cast<uint32_t*>(smem_raw) + (1 << P.table_log2), P.table_log2};
+  uint32_t* named = table.count + (1 << P.table_log2);                      // [slice / 32 + 1] a bit for every token of the history
+  constexpr int kSize = F32 ? 4 : 2, kAhead = F32 ? 2 : 4;
   const int tid = threadIdx.x;
   after_predecessor();
   const long long items = static_cast<long long>(P.rows) * P.slices;
@@ -98,132 +119,137 @@ static __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(Logits
     const unsigned char* in = static_cast<const unsigned char*>(P.in) + row * P.in_stride * kSize;
     unsigned char* out = static_cast<unsigned char*>(P.out) + row * P.out_stride * kSize;
     const int which = P.mask ? (P.mask_rows ? P.mask_rows[row] : row) : -1;
-    const int n_hist = P.history ? min(P.lengths ? max(P.lengths[row], 0) : P.hist_len, P.hist_len) : 0;
-    const int n_bias = P.bias_len, prompt = P.prompts ? P.prompts[row] : 0;
-    const float rho = P.rho ? P.rho[row] : P.rho_s, pi = P.pi ? P.pi[row] : P.pi_s, phi = P.phi ? P.phi[row] : P.phi_s;
     const bool nothing = which >= P.mask_count && which >= 0;               // the row's mask does not exist: everything is masked
     const uint8_t* mask = which >= 0 && !nothing ? reinterpret_cast<const uint8_t*>(P.mask + which * P.mask_stride) : nullptr;     // the row's bits, or none
     const bool stream = !P.in_place || mask || nothing;
-    const uint32_t width = static_cast<uint32_t>(hi - lo);
     auto keeps = [&](int v) { return !nothing && (!mask || ((mask[v >> 3] >> (v & 7)) & 1u)); };
-    // ---- the slice: [lo, head) singly, then chunks of 8 from 16-byte boundaries, then the rest singly
-    int head = lo, chunks = 0;
-    if (stream && ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0) {
-      const uintptr_t at = reinterpret_cast<uintptr_t>(out) + static_cast<uintptr_t>(lo) * kSize;
-      head = min(lo + static_cast<int>(((16u - (at & 15u)) & 15u) / kSize), hi);
-      chunks = (hi - head) / 8;
-    }
-    const int shift = head & 7;                                              // of a chunk's bits in their byte (lo is a multiple of 32)
-    // chunk c: its logits at in8 + c * 8 * kSize, its bits from mask8[c] on
-    const unsigned char* in8 = in + static_cast<int64_t>(head) * kSize;
-    unsigned char* out8 = out + static_cast<int64_t>(head) * kSize;
-    const uint8_t* mask8 = mask ? mask + (head >> 3) : nullptr;
-    auto bits_of = [&](const uint8_t* p, int c) -> uint32_t { return shift == 0 ? p[c] : ((p[c] | static_cast<uint32_t>(p[c + 1]) << 8) >> shift) & 0xFFu; };
-    Chunk<F32> x[kAhead];
-    uint32_t keep[kAhead];
-    auto load_bits = [&](int c0) {
-#pragma unroll
-      for (int u = 0; u < kAhead; u++) {
-        keep[u] = nothing ? 0u : 0xFFu;
-        if (mask8 && c0 + u * kLogitsThreads < chunks) keep[u] = bits_of(mask8, c0 + u * kLogitsThreads);
-      }
-    };
-    auto load = [&](int c0) {
-      const unsigned char* p = in8 + static_cast<int64_t>(c0) * (8 * kSize);
-#pragma unroll
-      for (int u = 0; u < kAhead; u++)
-        if (c0 + u * kLogitsThreads < chunks && keep[u] != 0u && !(P.in_place && keep[u] == 0xFFu)) x[u].load(p + u * (kLogitsThreads * 8 * kSize));
-    };
-    load_bits(tid);
-    load(tid);
-    // ---- counts, while the first chunks are on their way
+    // ---- the lists
+    const int n_hist = kLists && P.history && !nothing ? min(P.lengths ? max(P.lengths[row], 0) : P.hist_len, P.hist_len) : 0;
+    const int n_bias = kLists && !nothing ? P.bias_len : 0;
     const int32_t* hist = P.history + row * P.hist_stride;
     const int32_t* ids = P.bias_ids + row * P.bias_ids_stride;
-    const bool lists = !nothing && (n_hist || n_bias);
-    // f(token in the slice, behind the prompt) for the history's tokens in the slice
-    auto each_token = [&](auto f) {
-      const bool fours = (reinterpret_cast<uintptr_t>(hist) & 15u) == 0;
-      for (int i = 4 * tid; i < n_hist; i += 4 * kLogitsThreads) {
-        int t[4];
-        if (fours && i + 4 <= n_hist) { const int4 q = __ldg(reinterpret_cast<const int4*>(hist + i)); t[0] = q.x; t[1] = q.y; t[2] = q.z; t[3] = q.w; }
-        else {
-#pragma unroll
-          for (int e = 0; e < 4; e++) t[e] = i + e < n_hist ? hist[i + e] : -1;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) { const uint32_t v = static_cast<uint32_t>(t[e]) - static_cast<uint32_t>(lo); if (v < width) f(v, i + e >= prompt); }     // (-1, padding: never below a width)
-      }
-    };
     auto penalised = [&](float z, uint32_t n) {
-      if (n & (kSeen | kOutMask)) z = (z > 0.0f) ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
-      if (n & kOutMask) z = __fsub_rn(__fsub_rn(z, pi), __fmul_rn(phi, static_cast<float>(n & kOutMask)));
+      if (n & (kSeen | kOutMask)) { const float rho = P.rho ? __ldg(P.rho + row) : P.rho_s; z = (z > 0.0f) ? __fdiv_rn(z, rho) : __fmul_rn(z, rho); }
+      if (n & kOutMask) {
+        const float pi = P.pi ? __ldg(P.pi + row) : P.pi_s, phi = P.phi ? __ldg(P.phi + row) : P.phi_s;
+        z = __fsub_rn(__fsub_rn(z, pi), __fmul_rn(phi, static_cast<float>(n & kOutMask)));
+      }
       return z;
     };
-    if (lists) {
+    if (n_hist || n_bias) {
+      const uint32_t width = static_cast<uint32_t>(hi - lo);
+      for (int i = tid; i < 1 << P.table_log2; i += kLogitsThreads) { table.key[i] = kNoToken; table.count[i] = 0u; }
       for (int i = tid; i < P.slice / 32 + 1; i += kLogitsThreads) named[i] = 0u;
-      if (n_hist) each_token([&](uint32_t v, bool) { counts[v] = 0u; });
-      for (int i = tid; i < n_bias; i += kLogitsThreads) { const uint32_t v = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(lo); if (v < width) counts[v] = 0u; }
       __syncthreads();
-      if (n_hist) each_token([&](uint32_t v, bool behind) {
-        if (behind) atomicAdd(&counts[v], 1u); else atomicOr(&counts[v], kSeen);
-        atomicOr(&named[v >> 5], 1u << (v & 31));
-      });
-      for (int i = tid; i < n_bias; i += kLogitsThreads) { const uint32_t v = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(lo); if (v < width) atomicAdd(&counts[v], kBiasOne); }
+      const int prompt = P.prompts ? P.prompts[row] : 0;
+      for (int i = tid; i < n_hist; i += kLogitsThreads) {
+        const uint32_t v = static_cast<uint32_t>(hist[i]) - static_cast<uint32_t>(lo);
+        if (v < width) {
+          uint32_t* n = &table.count[table.insert(v)];
+          if (i >= prompt) atomicAdd(n, 1u); else atomicOr(n, kSeen);
+          atomicOr(&named[v >> 5], 1u << (v & 31));
+        }
+      }
+      for (int i = tid; i < n_bias; i += kLogitsThreads) {
+        const uint32_t v = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(lo);
+        if (v < width) atomicAdd(&table.count[table.insert(v)], kBiasOne);
+      }
       __syncthreads();
     }
-    const bool penalise_here = lists && n_hist;
+    // ---- the slice: [lo, head) singly, then chunks of 8 from 16-byte boundaries, then the rest singly
     if (stream) {
+      int head = lo, chunks = 0;
+      if (((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(out) + static_cast<uintptr_t>(lo) * kSize;
+        head = min(lo + static_cast<int>(((16u - (at & 15u)) & 15u) / kSize), hi);
+        chunks = (hi - head) / 8;
+      }
       const int tail = head + 8 * chunks, singles = (head - lo) + (hi - tail);
       for (int i = tid; i < singles; i += kLogitsThreads) {
         const int v = i < head - lo ? lo + i : tail + (i - (head - lo));
-        if (!keeps(v)) set_logit<F32>(out, v, -INFINITY);
-        else if (penalise_here && ((named[(v - lo) >> 5] >> ((v - lo) & 31)) & 1u) && !(counts[v - lo] & kBiasMask)) set_logit<F32>(out, v, penalised(logit_at<F32>(in, v), counts[v - lo]));
-        else if (!P.in_place) {
+        if (!keeps(v)) { set_logit<F32>(out, v, -INFINITY); continue; }
+        if (n_hist && ((named[(v - lo) >> 5] >> ((v - lo) & 31)) & 1u)) {
+          const uint32_t n = table.count[table.find(static_cast<uint32_t>(v - lo))];
+          if (!(n & kBiasMask)) { set_logit<F32>(out, v, penalised(logit_at<F32>(in, v), n)); continue; }
+        }
+        if (!P.in_place) {
           if (F32) reinterpret_cast<uint32_t*>(out)[v] = reinterpret_cast<const uint32_t*>(in)[v]; else reinterpret_cast<uint16_t*>(out)[v] = reinterpret_cast<const uint16_t*>(in)[v];
         }
       }
-      const uint8_t* named8 = reinterpret_cast<const uint8_t*>(named) + ((head - lo) >> 3);
-      const uint32_t* counts8 = counts + (head - lo);
-      for (int c0 = tid; c0 < chunks;) {
-        unsigned char* p = out8 + static_cast<int64_t>(c0) * (8 * kSize);
+      const int shift = head & 7;                                            // of a chunk's bits in their byte (lo is a multiple of 32)
+      for (int c0 = tid; c0 < chunks; c0 += kLogitsThreads * kAhead) {
+        const unsigned char* from = in + static_cast<int64_t>(head + 8 * c0) * kSize;
+        unsigned char* to = out + static_cast<int64_t>(head + 8 * c0) * kSize;
+        Chunk<F32> x[kAhead];
+        uint32_t keep = nothing ? 0u : 0xFFFFFFFFu, touched = 0u;            // 8 bits for each chunk
+        if (mask) {
+          const uint8_t* p = mask + (head >> 3) + c0;
+          keep = 0u;
+#pragma unroll
+          for (int u = 0; u < kAhead; u++) {
+            if (c0 + u * kLogitsThreads < chunks) {
+              uint32_t k = __ldg(p + u * kLogitsThreads);
+              if (shift) k = ((k | static_cast<uint32_t>(__ldg(p + u * kLogitsThreads + 1)) << 8) >> shift) & 0xFFu;     // (v + 7 is in the row, and so is its byte)
+              keep |= k << (8 * u);
+            }
+          }
+        }
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
-          const int c = c0 + u * kLogitsThreads;
-          if (c >= chunks) break;
-          uint32_t touched = penalise_here ? bits_of(named8, c) & keep[u] : 0u;
-          if (P.in_place && keep[u] == 0xFFu) {                             // (not loaded: what is named is set singly)
-            for (; touched; touched &= touched - 1u) {
-              const int v = 8 * c + __ffs(static_cast<int>(touched)) - 1;
-              if (!(counts8[v] & kBiasMask)) set_logit<F32>(out8, v, penalised(logit_at<F32>(in8, v), counts8[v]));
-            }
-            continue;
-          }
-          for (; touched; touched &= touched - 1u) {
-            const int e = __ffs(static_cast<int>(touched)) - 1;
-            const uint32_t n = counts8[8 * c + e];
-            if (!(n & kBiasMask)) x[u].set(e, penalised(x[u].get(e), n));    // (with a bias: set below, from the logit itself)
-          }
-          if (keep[u] != 0xFFu) x[u].apply(keep[u]);
-          x[u].store(p + u * (kLogitsThreads * 8 * kSize));
+          const uint32_t k = (keep >> (8 * u)) & 0xFFu;
+          if (c0 + u * kLogitsThreads < chunks && k != 0u && !(P.in_place && k == 0xFFu)) x[u].load(from + u * (kLogitsThreads * 8 * kSize));
         }
-        c0 += kLogitsThreads * kAhead;
-        if (c0 < chunks) { load_bits(c0); load(c0); }
+        if (n_hist) {
+          const uint8_t* p = reinterpret_cast<const uint8_t*>(named) + ((head - lo) >> 3) + c0;
+#pragma unroll
+          for (int u = 0; u < kAhead; u++) {
+            if (c0 + u * kLogitsThreads < chunks) {
+              uint32_t k = p[u * kLogitsThreads];
+              if (shift) k = ((k | static_cast<uint32_t>(p[u * kLogitsThreads + 1]) << 8) >> shift) & 0xFFu;
+              touched |= k << (8 * u);
+            }
+          }
+          touched &= keep;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+          const uint32_t k = (keep >> (8 * u)) & 0xFFu;
+          if (c0 + u * kLogitsThreads < chunks && !(P.in_place && k == 0xFFu)) {
+            if (k != 0xFFu) x[u].apply(k);
+            x[u].store(to + u * (kLogitsThreads * 8 * kSize));
+          }
+        }
+        for (; touched; touched &= touched - 1u) {                           // (behind the stores of their chunks, by the same thread)
+          const int b = __ffs(static_cast<int>(touched)) - 1, u = b >> 3, v = (c0 + u * kLogitsThreads) * 8 + (b & 7);     // from head on
+          const uint32_t n = table.count[table.find(static_cast<uint32_t>(head - lo + v))];
+          if (n & kBiasMask) continue;                                       // (set below, from the logit itself)
+          float z;
+          if (P.in_place && ((keep >> (8 * u)) & 0xFFu) == 0xFFu) z = logit_at<F32>(in, head + v);     // (not loaded)
+          else {
+            z = x[0].get(b & 7);
+#pragma unroll
+            for (int q = 1; q < kAhead; q++) { const float zq = x[q].get(b & 7); z = q == u ? zq : z; }
+          }
+          set_logit<F32>(out, head + v, penalised(z, n));
+        }
       }
     }
     // ---- tokens of the history where nothing was streamed, and those with a bias
-    if (lists && (!stream || n_bias)) {
+    if ((n_hist || n_bias) && (!stream || n_bias)) {
       __syncthreads();
-      if (!stream && n_hist) each_token([&](uint32_t v, bool) {
-        const uint32_t n = atomicOr(&counts[v], kClaimed);                  // (the first thread to claim a token sets it)
-        const int id = lo + static_cast<int>(v);
-        if (!(n & (kClaimed | kBiasMask))) set_logit<F32>(out, id, penalised(logit_at<F32>(in, id), n));
-      });
+      const uint32_t width = static_cast<uint32_t>(hi - lo);
+      if (!stream) {
+        for (int i = tid; i < 1 << P.table_log2; i += kLogitsThreads) {
+          const uint32_t v = table.key[i], n = table.count[i];
+          if (v != kNoToken && !(n & kBiasMask)) set_logit<F32>(out, lo + static_cast<int>(v), penalised(logit_at<F32>(in, lo + static_cast<int>(v)), n));
+        }
+      }
       const float* values = P.bias_values + row * P.bias_values_stride;
       for (int i = tid; i < n_bias; i += kLogitsThreads) {
         const int id = ids[i];
         const uint32_t v = static_cast<uint32_t>(id) - static_cast<uint32_t>(lo);
         if (v >= width || !keeps(id)) continue;
-        const uint32_t n = counts[v];
+        const uint32_t n = table.count[table.find(v)];
         int others = static_cast<int>((n & kBiasMask) / kBiasOne) - 1;       // (a token listed more than once: the first entry adds all values in list order)
         bool first = true;
         for (int e = 0; others > 0 && first && e < i; e++) first = ids[e] != id;
@@ -233,7 +259,7 @@ static __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(Logits
         set_logit<F32>(out, id, z);
       }
     }
-    if (lists) __syncthreads();                                             // the tables are the next slice's
+    if (kLists) __syncthreads();                                            // the tables are the next slice's
   }
 }
 

@@ -226,22 +226,37 @@ int lm_process_logits(const lm_logits_args* a) {
   P.rho = a->repetition; P.rho_s = a->repetition_s; P.pi = a->presence; P.pi_s = a->presence_s; P.phi = a->frequency; P.phi_s = a->frequency_s;
   P.bias_ids = a->bias_ids; P.bias_ids_stride = a->bias_ids_stride; P.bias_values = a->bias_values; P.bias_values_stride = a->bias_values_stride; P.bias_len = static_cast<int>(a->bias_len);
   P.mask = a->mask; P.mask_stride = a->mask_stride; P.mask_rows = a->mask_rows; P.mask_count = static_cast<int>(a->mask_count);
-  // slices: as few as give every SM two blocks of work, within the bounds of the table
-  const long long total = static_cast<long long>(a->rows) * a->vocab;
-  long long per = (total / (2LL * sms) + 255) / 256 * 256;
-  if (per < kLogitsMinSlice) per = kLogitsMinSlice;
-  if (per > kLogitsMaxSlice) per = kLogitsMaxSlice;
-  P.slices = static_cast<int>((a->vocab + per - 1) / per);
-  P.slice = static_cast<int>(((a->vocab + P.slices - 1) / P.slices + 31) / 32 * 32);
+  // A block to a row, or to a slice of one: one block to an SM while the slices are short (the launch is then made ready beside its predecessor), otherwise rounds of kLogitsPerSM blocks to an SM
+  // that are as full as they can be. Lists that are longer than the table takes: slices no wider than that.
+  const long long names = (P.history ? P.hist_len : 0) + P.bias_len, total = static_cast<long long>(a->rows) * a->vocab;
+  long long slices = 1;
+  if (total <= 16384LL * sms) slices = sms / a->rows;
+  else {
+    double best = 0.0;
+    const long long at_once = static_cast<long long>(kLogitsPerSM) * sms;
+    for (int rounds = 1; rounds <= 4; rounds++) {
+      const long long n = rounds * at_once / a->rows > 1 ? rounds * at_once / a->rows : 1, items = n * a->rows;
+      const double full = static_cast<double>(items) / static_cast<double>((items + at_once - 1) / at_once * at_once);
+      if (full > best + 0.02) { best = full; slices = n; }
+    }
+  }
+  if (slices < 1) slices = 1;
+  if (slices > (a->vocab + kLogitsMinSlice - 1) / kLogitsMinSlice) slices = (a->vocab + kLogitsMinSlice - 1) / kLogitsMinSlice;
+  if (names > kLogitsMaxNamed && slices < (a->vocab + kLogitsMaxNamed - 32) / (kLogitsMaxNamed - 31)) slices = (a->vocab + kLogitsMaxNamed - 32) / (kLogitsMaxNamed - 31);
+  P.slice = static_cast<int>(((a->vocab + slices - 1) / slices + 31) / 32 * 32);
   P.slices = static_cast<int>((a->vocab + P.slice - 1) / P.slice);
-  const size_t smem = lists ? static_cast<size_t>(P.slice) * 4 + P.slice / 8 + 16 : 0;
+  const long long named = names < P.slice ? names : P.slice;
+  P.table_log2 = 8;
+  while ((3LL << P.table_log2) < 4 * named) P.table_log2++;                 // three quarters full at most
+  const size_t smem = lists ? (size_t{8} << P.table_log2) + static_cast<size_t>(P.slice) / 8 + 16 : 0;
   const bool f32 = a->dtype == LM_DTYPE_F32;
-  rc = ensure_dynamic_smem(f32 ? kSlotLogitsF32 : kSlotLogits, f32 ? reinterpret_cast<const void*>(logits_kernel<true>) : reinterpret_cast<const void*>(logits_kernel<false>), smem);
-  if (rc != LM_OK) return rc;
+  void (*const kernel)(LogitsDev) = f32 ? (lists ? logits_kernel<true, true> : logits_kernel<true, false>) : (lists ? logits_kernel<false, true> : logits_kernel<false, false>);
+  if (lists) {
+    rc = ensure_dynamic_smem(f32 ? kSlotLogitsF32 : kSlotLogits, reinterpret_cast<const void*>(kernel), smem);
+    if (rc != LM_OK) return rc;
+  }
   const long long items = static_cast<long long>(P.rows) * P.slices;
-  const unsigned grid = static_cast<unsigned>(items < 0x7FFFFFFF ? items : 0x7FFFFFFF);
-  cudaStream_t st = static_cast<cudaStream_t>(a->stream);
-  return f32 ? launch_beside(logits_kernel<true>, dim3(grid), kLogitsThreads, smem, 1, st, P) : launch_beside(logits_kernel<false>, dim3(grid), kLogitsThreads, smem, 1, st, P);
+  return launch_beside(kernel, dim3(static_cast<unsigned>(items < 0x7FFFFFFF ? items : 0x7FFFFFFF)), kLogitsThreads, smem, 1, static_cast<cudaStream_t>(a->stream), P);
 }
 
 }  // extern "C"
