@@ -3,8 +3,8 @@
 // Per row r, with c_all the occurrences of a token in history[r, :len] and c_out those from position prompt_len on:
 //   z = float(logit); c_all > 0: z = z > 0 ? z / rho : z * rho; c_out > 0: z = (z - pi) - phi * c_out; z += the token's biases, in list order; masked: -inf.
 // The penalties touch as many logits as the history has tokens, the biases as many as their list; a mask usually touches most. A block has a row, or a slice of one where there are few. It
-// looks through the row's lists once: a bit in shared memory for every token of the history in its slice, and a hash table of these and the biased tokens with their counts (its size is given by
-// the lists' lengths, or by the slice's width: it never fills up). Then it streams the slice, 16 bytes a load, four under way per thread: copied and masked (in place: only what changes is
+// looks through the row's lists once: a bit in shared memory for every token of the history in its slice, and a table of these and the biased tokens with their counts: a word for every token of
+// the slice, or where that is smaller a hash table (its size is given by the lists' lengths: it never fills up). Then it streams the slice, 16 bytes a load, four under way per thread: copied and masked (in place: only what changes is
 // written, and read where a mask keeps some of eight), and logits whose bit is set are looked up and penalised in the registers that hold them. Tokens with a bias are set behind that, by their
 // (first) entry of the list. In place without a mask only the tokens that the lists name are touched.
 #pragma once
@@ -15,8 +15,9 @@ namespace lm {
 constexpr int kLogitsThreads = 512;
 constexpr int kLogitsPerSM = 3;              // blocks
 constexpr int kLogitsMinSlice = 1024;
-constexpr int kLogitsMaxTable = 16384;       // entries of the hash table, 8 bytes each
-constexpr int kLogitsMaxNamed = 12288;       // tokens in it at most
+constexpr int kLogitsMaxNamed = 12288;       // tokens in a hash table at most (16384 entries, 128 KB); longer lists: slices of
+constexpr int kLogitsMaxDirect = 24576;      // at most so many tokens (96 KB)
+constexpr int kLogitsMaxSlice = 524288;      // and never wider than this (64 KB of bits)
 
 struct LogitsDev {
   const void* in; int64_t in_stride; void* out; int64_t out_stride; int in_place;
@@ -25,7 +26,7 @@ struct LogitsDev {
   const float* rho; float rho_s; const float* pi; float pi_s; const float* phi; float phi_s;
   const int32_t* bias_ids; int64_t bias_ids_stride; const float* bias_values; int64_t bias_values_stride; int bias_len;
   const uint32_t* mask; int64_t mask_stride; const int32_t* mask_rows; int mask_count;
-  int slice; int slices; int table_log2;     // the table has 2^table_log2 entries
+  int slice; int slices; int table_log2;     // the hash table has 2^table_log2 entries; 0: a word for every token of the slice
 };
 
 // a token's counts
@@ -86,18 +87,28 @@ template <> struct Chunk<true> {
   }
 };
 
-// A hash table of tokens in shared memory, linear probing.
+// The tokens' counts in shared memory: a hash table with linear probing, or (log2 = 0) a word per token of the slice.
 constexpr uint32_t kNoToken = 0xFFFFFFFFu;
 struct TokenTable {
-  uint32_t* key; uint32_t* count; int log2;
+  uint32_t* key; uint32_t* count; int log2; int slice;
+  __device__ __forceinline__ TokenTable(unsigned char* smem, int log2_, int slice_)
+      : key(reinterpret_cast<uint32_t*>(smem)), count(reinterpret_cast<uint32_t*>(smem) + (log2_ ? 1 << log2_ : 0)), log2(log2_), slice(slice_) {}
+  __device__ __forceinline__ int words() const { return log2 ? 1 << log2 : slice; }     // of counts (a multiple of 32)
+  __device__ __forceinline__ uint32_t* end() const { return count + words(); }
   __device__ __forceinline__ uint32_t home(uint32_t v) const { return (v * 2654435769u) >> (32 - log2); }     // (2^32 over the golden ratio: neighbours lie apart)
+  __device__ __forceinline__ void clear() const {                            // and the bits behind the counts
+    const int keys = log2 ? 1 << log2 : 0, all = keys + words() + slice / 32;      // (slice / 32 + 1 words of bits; the last one is never used, only read)
+    for (int i = 4 * threadIdx.x; i < all; i += 4 * kLogitsThreads) { const uint32_t z = i < keys ? kNoToken : 0u; *reinterpret_cast<uint4*>(key + i) = make_uint4(z, z, z, z); }
+  }
   __device__ __forceinline__ uint32_t insert(uint32_t v) const {
+    if (!log2) return v;
     for (uint32_t i = home(v);; i = (i + 1u) & ((1u << log2) - 1u)) {
       const uint32_t k = atomicCAS(&key[i], kNoToken, v);
       if (k == kNoToken || k == v) return i;
     }
   }
   __device__ __forceinline__ uint32_t find(uint32_t v) const {               // (of a token that is there)
+    if (!log2) return v;
     uint32_t i = home(v);
     while (key[i] != v) i = (i + 1u) & ((1u << log2) - 1u);
     return i;
@@ -108,8 +119,8 @@ struct TokenTable {
 template <bool F32, bool kLists>
 static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_kernel(LogitsDev P) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  const TokenTable table{reinterpret_cast<uint32_t*>(smem_raw), reinterpret_cast<uint32_t*>(smem_raw) + (1 << P.table_log2), P.table_log2};
-  uint32_t* named = table.count + (1 << P.table_log2);                      // [slice / 32 + 1] a bit for every token of the history
+  const TokenTable table(smem_raw, P.table_log2, P.slice);
+  uint32_t* named = table.end();                                            // [slice / 32 + 1] a bit for every token of the history
   constexpr int kSize = F32 ? 4 : 2, kAhead = F32 ? 2 : 4;
   const int tid = threadIdx.x;
   after_predecessor();
@@ -138,16 +149,21 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
     };
     if (n_hist || n_bias) {
       const uint32_t width = static_cast<uint32_t>(hi - lo);
-      for (int i = tid; i < 1 << P.table_log2; i += kLogitsThreads) { table.key[i] = kNoToken; table.count[i] = 0u; }
-      for (int i = tid; i < P.slice / 32 + 1; i += kLogitsThreads) named[i] = 0u;
+      table.clear();
       __syncthreads();
       const int prompt = P.prompts ? P.prompts[row] : 0;
-      for (int i = tid; i < n_hist; i += kLogitsThreads) {
-        const uint32_t v = static_cast<uint32_t>(hist[i]) - static_cast<uint32_t>(lo);
-        if (v < width) {
-          uint32_t* n = &table.count[table.insert(v)];
-          if (i >= prompt) atomicAdd(n, 1u); else atomicOr(n, kSeen);
-          atomicOr(&named[v >> 5], 1u << (v & 31));
+      for (int base = tid; base < n_hist; base += 4 * kLogitsThreads) {
+        uint32_t t[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) t[e] = base + e * kLogitsThreads < n_hist ? static_cast<uint32_t>(hist[base + e * kLogitsThreads]) - static_cast<uint32_t>(lo) : kNoToken;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint32_t v = t[e];
+          if (v < width) {
+            uint32_t* n = &table.count[table.insert(v)];
+            if (base + e * kLogitsThreads >= prompt) atomicAdd(n, 1u); else atomicOr(n, kSeen);
+            atomicOr(&named[v >> 5], 1u << (v & 31));
+          }
         }
       }
       for (int i = tid; i < n_bias; i += kLogitsThreads) {
@@ -177,11 +193,9 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
         }
       }
       const int shift = head & 7;                                            // of a chunk's bits in their byte (lo is a multiple of 32)
-      for (int c0 = tid; c0 < chunks; c0 += kLogitsThreads * kAhead) {
-        const unsigned char* from = in + static_cast<int64_t>(head + 8 * c0) * kSize;
-        unsigned char* to = out + static_cast<int64_t>(head + 8 * c0) * kSize;
-        Chunk<F32> x[kAhead];
-        uint32_t keep = nothing ? 0u : 0xFFFFFFFFu, touched = 0u;            // 8 bits for each chunk
+      // the mask's bits of kAhead chunks, 8 for each
+      auto kept = [&](int c0) {
+        uint32_t keep = nothing ? 0u : 0xFFFFFFFFu;
         if (mask) {
           const uint8_t* p = mask + (head >> 3) + c0;
           keep = 0u;
@@ -194,11 +208,21 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
             }
           }
         }
+        return keep;
+      };
+      uint32_t next = kept(tid);
+      for (int c0 = tid; c0 < chunks; c0 += kLogitsThreads * kAhead) {
+        const unsigned char* from = in + static_cast<int64_t>(head + 8 * c0) * kSize;
+        unsigned char* to = out + static_cast<int64_t>(head + 8 * c0) * kSize;
+        Chunk<F32> x[kAhead];
+        const uint32_t keep = next;
+        uint32_t touched = 0u;                                               // 8 bits for each chunk
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
           const uint32_t k = (keep >> (8 * u)) & 0xFFu;
           if (c0 + u * kLogitsThreads < chunks && k != 0u && !(P.in_place && k == 0xFFu)) x[u].load(from + u * (kLogitsThreads * 8 * kSize));
         }
+        next = kept(c0 + kLogitsThreads * kAhead);
         if (n_hist) {
           const uint8_t* p = reinterpret_cast<const uint8_t*>(named) + ((head - lo) >> 3) + c0;
 #pragma unroll
@@ -239,9 +263,9 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
       __syncthreads();
       const uint32_t width = static_cast<uint32_t>(hi - lo);
       if (!stream) {
-        for (int i = tid; i < 1 << P.table_log2; i += kLogitsThreads) {
-          const uint32_t v = table.key[i], n = table.count[i];
-          if (v != kNoToken && !(n & kBiasMask)) set_logit<F32>(out, lo + static_cast<int>(v), penalised(logit_at<F32>(in, lo + static_cast<int>(v)), n));
+        for (int i = tid; i < table.words(); i += kLogitsThreads) {
+          const uint32_t v = table.log2 ? table.key[i] : static_cast<uint32_t>(i), n = table.count[i];
+          if ((n & (kSeen | kOutMask)) && !(n & kBiasMask)) set_logit<F32>(out, lo + static_cast<int>(v), penalised(logit_at<F32>(in, lo + static_cast<int>(v)), n));
         }
       }
       const float* values = P.bias_values + row * P.bias_values_stride;

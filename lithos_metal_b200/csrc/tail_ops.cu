@@ -242,13 +242,14 @@ int lm_process_logits(const lm_logits_args* a) {
   }
   if (slices < 1) slices = 1;
   if (slices > (a->vocab + kLogitsMinSlice - 1) / kLogitsMinSlice) slices = (a->vocab + kLogitsMinSlice - 1) / kLogitsMinSlice;
-  if (names > kLogitsMaxNamed && slices < (a->vocab + kLogitsMaxNamed - 32) / (kLogitsMaxNamed - 31)) slices = (a->vocab + kLogitsMaxNamed - 32) / (kLogitsMaxNamed - 31);
+  const long long widest = names > kLogitsMaxNamed ? kLogitsMaxDirect : kLogitsMaxSlice;
+  if (slices < (a->vocab + widest - 1) / widest) slices = (a->vocab + widest - 1) / widest;
   P.slice = static_cast<int>(((a->vocab + slices - 1) / slices + 31) / 32 * 32);
   P.slices = static_cast<int>((a->vocab + P.slice - 1) / P.slice);
-  const long long named = names < P.slice ? names : P.slice;
   P.table_log2 = 8;
-  while ((3LL << P.table_log2) < 4 * named) P.table_log2++;                 // three quarters full at most
-  const size_t smem = lists ? (size_t{8} << P.table_log2) + static_cast<size_t>(P.slice) / 8 + 16 : 0;
+  while ((3LL << P.table_log2) < 4 * names) P.table_log2++;                 // three quarters full at most
+  if (P.slice <= 2LL << P.table_log2) P.table_log2 = 0;                     // (no larger than the hash table, keys and counts: a word per token)
+  const size_t smem = lists ? (P.table_log2 ? size_t{8} << P.table_log2 : static_cast<size_t>(P.slice) * 4) + static_cast<size_t>(P.slice) / 8 + 32 : 0;
   const bool f32 = a->dtype == LM_DTYPE_F32;
   void (*const kernel)(LogitsDev) = f32 ? (lists ? logits_kernel<true, true> : logits_kernel<true, false>) : (lists ? logits_kernel<false, true> : logits_kernel<false, false>);
   if (lists) {
