@@ -5,7 +5,7 @@
 // The penalties touch as many logits as the history has tokens, the biases as many as their list; a mask usually touches most. A block has a row, or a slice of one where there are few. It
 // looks through the row's lists once: a bit in shared memory for every token of the history in its slice, and a table of these and the biased tokens with their counts: a word for every token of
 // the slice, or where that is smaller a hash table (its size is given by the lists' lengths: it never fills up). Then it streams the slice, 16 bytes a load, four under way per thread: copied and masked (in place: only what changes is
-// written, and read where a mask keeps some of eight), and logits whose bit is set are looked up and penalised in the registers that hold them. Tokens with a bias are set behind that, by their
+// written, and read where a mask keeps some of eight), and logits whose bit is set are looked up and penalised right behind their chunk. Tokens with a bias are set behind that, by their
 // (first) entry of the list. In place without a mask only the tokens that the lists name are touched.
 #pragma once
 #include "common.cuh"
@@ -51,23 +51,14 @@ __device__ __forceinline__ uint32_t two_kept(uint32_t w, uint32_t keep) {    // 
 template <bool F32> struct Chunk;
 template <> struct Chunk<false> {
   uint4 q;
-  __device__ __forceinline__ void load(const void* p) { q = __ldcs(static_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void load(const void* p) { q = *static_cast<const uint4*>(p); }
   __device__ __forceinline__ void store(void* p) const { *static_cast<uint4*>(p) = q; }
   __device__ __forceinline__ void apply(uint32_t keep) { q.x = two_kept(q.x, keep); q.y = two_kept(q.y, keep >> 2); q.z = two_kept(q.z, keep >> 4); q.w = two_kept(q.w, keep >> 6); }
-  __device__ __forceinline__ float get(int e) const {
-    const uint32_t w = e & 4 ? (e & 2 ? q.w : q.z) : (e & 2 ? q.y : q.x);
-    return e & 1 ? bf16_hi(w) : bf16_lo(w);
-  }
-  __device__ __forceinline__ void set(int e, float z) {
-    const uint32_t h = __bfloat16_as_ushort(__float2bfloat16_rn(z)), sel = e & 1 ? 0x5410u : 0x3254u;      // h in the upper or the lower half
-    const int i = e >> 1;
-    q.x = i == 0 ? __byte_perm(q.x, h, sel) : q.x; q.y = i == 1 ? __byte_perm(q.y, h, sel) : q.y; q.z = i == 2 ? __byte_perm(q.z, h, sel) : q.z; q.w = i == 3 ? __byte_perm(q.w, h, sel) : q.w;
-  }
 };
 template <> struct Chunk<true> {
   uint32_t v[8];
   __device__ __forceinline__ void load(const void* p) {
-    const uint4 a = __ldcs(static_cast<const uint4*>(p)), b = __ldcs(static_cast<const uint4*>(p) + 1);
+    const uint4 a = *static_cast<const uint4*>(p), b = *(static_cast<const uint4*>(p) + 1);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   }
   __device__ __forceinline__ void store(void* p) const { static_cast<uint4*>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]); static_cast<uint4*>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]); }
@@ -75,43 +66,33 @@ template <> struct Chunk<true> {
 #pragma unroll
     for (int e = 0; e < 8; e++) if (!((keep >> e) & 1u)) v[e] = 0xFF800000u;
   }
-  __device__ __forceinline__ float get(int e) const {
-    uint32_t r = v[0];
-#pragma unroll
-    for (int i = 1; i < 8; i++) r = i == e ? v[i] : r;
-    return __uint_as_float(r);
-  }
-  __device__ __forceinline__ void set(int e, float z) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = i == e ? __float_as_uint(z) : v[i];
-  }
 };
 
 // The tokens' counts in shared memory: a hash table with linear probing, or (log2 = 0) a word per token of the slice.
 constexpr uint32_t kNoToken = 0xFFFFFFFFu;
 struct TokenTable {
-  uint32_t* key; uint32_t* count; int log2; int slice;
-  __device__ __forceinline__ TokenTable(unsigned char* smem, int log2_, int slice_)
-      : key(reinterpret_cast<uint32_t*>(smem)), count(reinterpret_cast<uint32_t*>(smem) + (log2_ ? 1 << log2_ : 0)), log2(log2_), slice(slice_) {}
-  __device__ __forceinline__ int words() const { return log2 ? 1 << log2 : slice; }     // of counts (a multiple of 32)
-  __device__ __forceinline__ uint32_t* end() const { return count + words(); }
+  uint32_t* word; int log2; int slice;                                      // hash entries: token and counts, side by side
+  __device__ __forceinline__ TokenTable(unsigned char* smem, int log2_, int slice_) : word(reinterpret_cast<uint32_t*>(smem)), log2(log2_), slice(slice_) {}
+  __device__ __forceinline__ int entries() const { return log2 ? 1 << log2 : slice; }   // (a multiple of 32)
+  __device__ __forceinline__ uint32_t* end() const { return word + (log2 ? 2 << log2 : slice); }
   __device__ __forceinline__ uint32_t home(uint32_t v) const { return (v * 2654435769u) >> (32 - log2); }     // (2^32 over the golden ratio: neighbours lie apart)
-  __device__ __forceinline__ void clear() const {                            // and the bits behind the counts
-    const int keys = log2 ? 1 << log2 : 0, all = keys + words() + slice / 32;      // (slice / 32 + 1 words of bits; the last one is never used, only read)
-    for (int i = 4 * threadIdx.x; i < all; i += 4 * kLogitsThreads) { const uint32_t z = i < keys ? kNoToken : 0u; *reinterpret_cast<uint4*>(key + i) = make_uint4(z, z, z, z); }
+  __device__ __forceinline__ void clear() const {                            // and the bits behind it
+    const int hashed = log2 ? 2 << log2 : 0, all = (log2 ? 2 << log2 : slice) + slice / 32;
+    for (int i = 4 * threadIdx.x; i < all; i += 4 * kLogitsThreads) { const uint32_t k = i < hashed ? kNoToken : 0u; *reinterpret_cast<uint4*>(word + i) = make_uint4(k, 0u, k, 0u); }
   }
-  __device__ __forceinline__ uint32_t insert(uint32_t v) const {
-    if (!log2) return v;
+  __device__ __forceinline__ uint32_t* insert(uint32_t v) const {            // the token's counts
+    if (!log2) return word + v;
     for (uint32_t i = home(v);; i = (i + 1u) & ((1u << log2) - 1u)) {
-      const uint32_t k = atomicCAS(&key[i], kNoToken, v);
-      if (k == kNoToken || k == v) return i;
+      const uint32_t k = atomicCAS(&word[2 * i], kNoToken, v);
+      if (k == kNoToken || k == v) return &word[2 * i + 1];
     }
   }
-  __device__ __forceinline__ uint32_t find(uint32_t v) const {               // (of a token that is there)
-    if (!log2) return v;
+  __device__ __forceinline__ uint32_t counts(uint32_t v) const {             // of a token that is there
+    if (!log2) return word[v];
     uint32_t i = home(v);
-    while (key[i] != v) i = (i + 1u) & ((1u << log2) - 1u);
-    return i;
+    uint2 e = *reinterpret_cast<const uint2*>(word + 2 * i);
+    while (e.x != v) { i = (i + 1u) & ((1u << log2) - 1u); e = *reinterpret_cast<const uint2*>(word + 2 * i); }
+    return e.y;
   }
 };
 
@@ -139,12 +120,10 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
     const int n_bias = kLists && !nothing ? P.bias_len : 0;
     const int32_t* hist = P.history + row * P.hist_stride;
     const int32_t* ids = P.bias_ids + row * P.bias_ids_stride;
+    const float rho = kLists && P.rho ? P.rho[row] : P.rho_s, pi = kLists && P.pi ? P.pi[row] : P.pi_s, phi = kLists && P.phi ? P.phi[row] : P.phi_s;
     auto penalised = [&](float z, uint32_t n) {
-      if (n & (kSeen | kOutMask)) { const float rho = P.rho ? __ldg(P.rho + row) : P.rho_s; z = (z > 0.0f) ? __fdiv_rn(z, rho) : __fmul_rn(z, rho); }
-      if (n & kOutMask) {
-        const float pi = P.pi ? __ldg(P.pi + row) : P.pi_s, phi = P.phi ? __ldg(P.phi + row) : P.phi_s;
-        z = __fsub_rn(__fsub_rn(z, pi), __fmul_rn(phi, static_cast<float>(n & kOutMask)));
-      }
+      if (n & (kSeen | kOutMask)) z = (z > 0.0f) ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
+      if (n & kOutMask) z = __fsub_rn(__fsub_rn(z, pi), __fmul_rn(phi, static_cast<float>(n & kOutMask)));
       return z;
     };
     if (n_hist || n_bias) {
@@ -160,7 +139,7 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
         for (int e = 0; e < 4; e++) {
           const uint32_t v = t[e];
           if (v < width) {
-            uint32_t* n = &table.count[table.insert(v)];
+            uint32_t* n = table.insert(v);
             if (base + e * kLogitsThreads >= prompt) atomicAdd(n, 1u); else atomicOr(n, kSeen);
             atomicOr(&named[v >> 5], 1u << (v & 31));
           }
@@ -168,7 +147,7 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
       }
       for (int i = tid; i < n_bias; i += kLogitsThreads) {
         const uint32_t v = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(lo);
-        if (v < width) atomicAdd(&table.count[table.insert(v)], kBiasOne);
+        if (v < width) atomicAdd(table.insert(v), kBiasOne);
       }
       __syncthreads();
     }
@@ -185,7 +164,7 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
         const int v = i < head - lo ? lo + i : tail + (i - (head - lo));
         if (!keeps(v)) { set_logit<F32>(out, v, -INFINITY); continue; }
         if (n_hist && ((named[(v - lo) >> 5] >> ((v - lo) & 31)) & 1u)) {
-          const uint32_t n = table.count[table.find(static_cast<uint32_t>(v - lo))];
+          const uint32_t n = table.counts(static_cast<uint32_t>(v - lo));
           if (!(n & kBiasMask)) { set_logit<F32>(out, v, penalised(logit_at<F32>(in, v), n)); continue; }
         }
         if (!P.in_place) {
@@ -245,16 +224,9 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
         }
         for (; touched; touched &= touched - 1u) {                           // (behind the stores of their chunks, by the same thread)
           const int b = __ffs(static_cast<int>(touched)) - 1, u = b >> 3, v = (c0 + u * kLogitsThreads) * 8 + (b & 7);     // from head on
-          const uint32_t n = table.count[table.find(static_cast<uint32_t>(head - lo + v))];
+          const uint32_t n = table.counts(static_cast<uint32_t>(head - lo + v));
           if (n & kBiasMask) continue;                                       // (set below, from the logit itself)
-          float z;
-          if (P.in_place && ((keep >> (8 * u)) & 0xFFu) == 0xFFu) z = logit_at<F32>(in, head + v);     // (not loaded)
-          else {
-            z = x[0].get(b & 7);
-#pragma unroll
-            for (int q = 1; q < kAhead; q++) { const float zq = x[q].get(b & 7); z = q == u ? zq : z; }
-          }
-          set_logit<F32>(out, head + v, penalised(z, n));
+          set_logit<F32>(out, head + v, penalised(logit_at<F32>(in, head + v), n));     // (read again, from the line just loaded)
         }
       }
     }
@@ -263,8 +235,8 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
       __syncthreads();
       const uint32_t width = static_cast<uint32_t>(hi - lo);
       if (!stream) {
-        for (int i = tid; i < table.words(); i += kLogitsThreads) {
-          const uint32_t v = table.log2 ? table.key[i] : static_cast<uint32_t>(i), n = table.count[i];
+        for (int i = tid; i < table.entries(); i += kLogitsThreads) {
+          const uint32_t v = table.log2 ? table.word[2 * i] : static_cast<uint32_t>(i), n = table.word[table.log2 ? 2 * i + 1 : i];
           if ((n & (kSeen | kOutMask)) && !(n & kBiasMask)) set_logit<F32>(out, lo + static_cast<int>(v), penalised(logit_at<F32>(in, lo + static_cast<int>(v)), n));
         }
       }
@@ -273,7 +245,7 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
         const int id = ids[i];
         const uint32_t v = static_cast<uint32_t>(id) - static_cast<uint32_t>(lo);
         if (v >= width || !keeps(id)) continue;
-        const uint32_t n = table.count[table.find(v)];
+        const uint32_t n = table.counts(v);
         int others = static_cast<int>((n & kBiasMask) / kBiasOne) - 1;       // (a token listed more than once: the first entry adds all values in list order)
         bool first = true;
         for (int e = 0; others > 0 && first && e < i; e++) first = ids[e] != id;
