@@ -39,8 +39,9 @@ enum KernelSlot { kSlotFast, kSlotTopk, kSlotTopkOrdered, kSlotGeneric, kSlotVoc
                   kSlotVerify = kSlotDraftQ + 2,    // (twelve)
                   kSlotVerifyGiven = kSlotVerify + 12,   // (four)
                   kSlotHeadNvfp4 = kSlotVerifyGiven + 4,     // (four)
-                  kSlotHeadNvfp4Batch = kSlotHeadNvfp4 + 4, kSlotLogits, kSlotLogitsF32,
-                  kSlotCount };
+                  kSlotHeadNvfp4Batch = kSlotHeadNvfp4 + 4,
+                  kSlotLogits,                      // (four)
+                  kSlotCount = kSlotLogits + 4 };
 
 inline int ensure_dynamic_smem(KernelSlot slot, const void* func, size_t bytes, bool large_clusters = false) {
   constexpr int kMaxDevices = 64;

@@ -96,8 +96,7 @@ struct TokenTable {
   }
 };
 
-// kLists: there is a history or a bias list.
-template <bool F32, bool kLists>
+template <bool F32, bool kBias>
 static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_kernel(LogitsDev P) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const TokenTable table(smem_raw, P.table_log2, P.slice);
@@ -116,11 +115,11 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
     const bool stream = !P.in_place || mask || nothing;
     auto keeps = [&](int v) { return !nothing && (!mask || ((mask[v >> 3] >> (v & 7)) & 1u)); };
     // ---- the lists
-    const int n_hist = kLists && P.history && !nothing ? min(P.lengths ? max(P.lengths[row], 0) : P.hist_len, P.hist_len) : 0;
-    const int n_bias = kLists && !nothing ? P.bias_len : 0;
+    const int n_hist = P.history && !nothing ? min(P.lengths ? max(P.lengths[row], 0) : P.hist_len, P.hist_len) : 0;
+    const int n_bias = !kBias || nothing ? 0 : P.bias_len;
     const int32_t* hist = P.history + row * P.hist_stride;
     const int32_t* ids = P.bias_ids + row * P.bias_ids_stride;
-    const float rho = kLists && P.rho ? P.rho[row] : P.rho_s, pi = kLists && P.pi ? P.pi[row] : P.pi_s, phi = kLists && P.phi ? P.phi[row] : P.phi_s;
+    const float rho = P.rho ? P.rho[row] : P.rho_s, pi = P.pi ? P.pi[row] : P.pi_s, phi = P.phi ? P.phi[row] : P.phi_s;
     auto penalised = [&](float z, uint32_t n) {
       if (n & (kSeen | kOutMask)) z = (z > 0.0f) ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
       if (n & kOutMask) z = __fsub_rn(__fsub_rn(z, pi), __fmul_rn(phi, static_cast<float>(n & kOutMask)));
@@ -165,7 +164,7 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
         if (!keeps(v)) { set_logit<F32>(out, v, -INFINITY); continue; }
         if (n_hist && ((named[(v - lo) >> 5] >> ((v - lo) & 31)) & 1u)) {
           const uint32_t n = table.counts(static_cast<uint32_t>(v - lo));
-          if (!(n & kBiasMask)) { set_logit<F32>(out, v, penalised(logit_at<F32>(in, v), n)); continue; }
+          if (!kBias || !(n & kBiasMask)) { set_logit<F32>(out, v, penalised(logit_at<F32>(in, v), n)); continue; }
         }
         if (!P.in_place) {
           if (F32) reinterpret_cast<uint32_t*>(out)[v] = reinterpret_cast<const uint32_t*>(in)[v]; else reinterpret_cast<uint16_t*>(out)[v] = reinterpret_cast<const uint16_t*>(in)[v];
@@ -225,7 +224,7 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
         for (; touched; touched &= touched - 1u) {                           // (behind the stores of their chunks, by the same thread)
           const int b = __ffs(static_cast<int>(touched)) - 1, u = b >> 3, v = (c0 + u * kLogitsThreads) * 8 + (b & 7);     // from head on
           const uint32_t n = table.counts(static_cast<uint32_t>(head - lo + v));
-          if (n & kBiasMask) continue;                                       // (set below, from the logit itself)
+          if (kBias && (n & kBiasMask)) continue;                                       // (set below, from the logit itself)
           set_logit<F32>(out, head + v, penalised(logit_at<F32>(in, head + v), n));     // (read again, from the line just loaded)
         }
       }
@@ -241,21 +240,99 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
         }
       }
       const float* values = P.bias_values + row * P.bias_values_stride;
-      for (int i = tid; i < n_bias; i += kLogitsThreads) {
-        const int id = ids[i];
+      for (int base = tid & ~31; base < n_bias; base += kLogitsThreads) {      // (a warp together)
+        const int i = base + (tid & 31), id = i < n_bias ? ids[i] : -1;
         const uint32_t v = static_cast<uint32_t>(id) - static_cast<uint32_t>(lo);
-        if (v >= width || !keeps(id)) continue;
-        const uint32_t n = table.counts(v);
-        int others = static_cast<int>((n & kBiasMask) / kBiasOne) - 1;       // (a token listed more than once: the first entry adds all values in list order)
-        bool first = true;
-        for (int e = 0; others > 0 && first && e < i; e++) first = ids[e] != id;
-        if (!first) continue;
-        float z = __fadd_rn(penalised(logit_at<F32>(in, id), n), values[i]);
-        for (int e = i + 1; others > 0 && e < n_bias; e++) if (ids[e] == id) { z = __fadd_rn(z, values[e]); others--; }
-        set_logit<F32>(out, id, z);
+        const bool mine = i < n_bias && v < width && keeps(id);
+        const uint32_t n = mine ? table.counts(v) : 0u;
+        const bool alone = (n & kBiasMask) == kBiasOne;
+        float z = mine ? penalised(logit_at<F32>(in, id), n) : 0.0f;
+        if (mine && alone) set_logit<F32>(out, id, __fadd_rn(z, values[i]));
+        // tokens listed more than once: the first entry adds all values in list order, the warp looks for them
+        for (uint32_t others = __ballot_sync(kFull, mine && !alone); others; others &= others - 1u) {
+          const int lane = __ffs(static_cast<int>(others)) - 1, what = __shfl_sync(kFull, id, lane);
+          float sum = __shfl_sync(kFull, z, lane);
+          int first = -1;
+          for (int e0 = 0; e0 < n_bias; e0 += 32) {
+            const int e = e0 + (tid & 31);
+            const bool same = e < n_bias && ids[e] == what;
+            const float value = same ? values[e] : 0.0f;
+            for (uint32_t m = __ballot_sync(kFull, same); m; m &= m - 1u) {
+              const int at = __ffs(static_cast<int>(m)) - 1;
+              if (first < 0) first = e0 + at;
+              sum = __fadd_rn(sum, __shfl_sync(kFull, value, at));
+            }
+          }
+          if ((tid & 31) == lane && first == i) set_logit<F32>(out, id, sum);
+        }
       }
     }
-    if (kLists) __syncthreads();                                            // the tables are the next slice's
+    __syncthreads();                                                        // the tables are the next slice's
+  }
+}
+
+// Without lists: copied and masked (in place: masked). The blocks stay and take a slice of kMaskSlice logits after the other; the next slice's bits of the mask come while this one's logits do.
+template <bool F32> constexpr int kMaskAhead = F32 ? 2 : 4;
+template <bool F32> constexpr int kMaskSlice = kLogitsThreads * 8 * kMaskAhead<F32>;
+
+template <bool F32>
+static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_mask_kernel(LogitsDev P) {
+  constexpr int kSize = F32 ? 4 : 2, kAhead = kMaskAhead<F32>;
+  const int tid = threadIdx.x;
+  after_predecessor();
+  const long long items = static_cast<long long>(P.rows) * P.slices;
+  struct Part { int row, lo, hi, head, chunks; uint32_t keep; bool nothing; const uint8_t* mask; } now, next;
+  auto part = [&](long long item, Part& a) {
+    a.row = static_cast<int>(item / P.slices); a.lo = static_cast<int>(item % P.slices) * P.slice; a.hi = min(a.lo + P.slice, P.vocab);
+    const int which = P.mask ? (P.mask_rows ? P.mask_rows[a.row] : a.row) : -1;
+    a.nothing = which >= P.mask_count && which >= 0;                        // the row's mask does not exist: everything is masked
+    a.mask = which >= 0 && !a.nothing ? reinterpret_cast<const uint8_t*>(P.mask + which * P.mask_stride) : nullptr;
+    const uintptr_t in = reinterpret_cast<uintptr_t>(P.in) + static_cast<uintptr_t>((a.row * P.in_stride + a.lo) * kSize), out = reinterpret_cast<uintptr_t>(P.out) + static_cast<uintptr_t>((a.row * P.out_stride + a.lo) * kSize);
+    a.head = a.lo; a.chunks = 0;                                            // [lo, head) singly, then chunks of 8 from 16-byte boundaries, then the rest singly
+    if (((in ^ out) & 15u) == 0) { a.head = min(a.lo + static_cast<int>(((16u - (out & 15u)) & 15u) / kSize), a.hi); a.chunks = (a.hi - a.head) / 8; }
+    a.keep = a.nothing ? 0u : 0xFFFFFFFFu;                                  // 8 bits for each of this thread's chunks
+    if (a.mask) {
+      const int shift = a.head & 7;
+      const uint8_t* p = a.mask + (a.head >> 3) + tid;
+      a.keep = 0u;
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) {
+        if (tid + u * kLogitsThreads < a.chunks) {
+          uint32_t k = __ldg(p + u * kLogitsThreads);
+          if (shift) k = ((k | static_cast<uint32_t>(__ldg(p + u * kLogitsThreads + 1)) << 8) >> shift) & 0xFFu;     // (v + 7 is in the row, and so is its byte)
+          a.keep |= k << (8 * u);
+        }
+      }
+    }
+  };
+  if (blockIdx.x < items) part(blockIdx.x, now);
+  for (long long item = blockIdx.x; item < items; item += gridDim.x, now = next) {
+    const unsigned char* in = static_cast<const unsigned char*>(P.in) + now.row * P.in_stride * kSize;
+    unsigned char* out = static_cast<unsigned char*>(P.out) + now.row * P.out_stride * kSize;
+    const int64_t at = static_cast<int64_t>(now.head + 8 * tid) * kSize;
+    Chunk<F32> x[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) {
+      const uint32_t k = (now.keep >> (8 * u)) & 0xFFu;
+      if (tid + u * kLogitsThreads < now.chunks && k != 0u && !(P.in_place && k == 0xFFu)) x[u].load(in + at + u * (kLogitsThreads * 8 * kSize));
+    }
+    if (item + gridDim.x < items) part(item + gridDim.x, next);
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) {
+      const uint32_t k = (now.keep >> (8 * u)) & 0xFFu;
+      if (tid + u * kLogitsThreads < now.chunks && !(P.in_place && k == 0xFFu)) {
+        if (k != 0xFFu) x[u].apply(k);
+        x[u].store(out + at + u * (kLogitsThreads * 8 * kSize));
+      }
+    }
+    const int tail = now.head + 8 * now.chunks, singles = (now.head - now.lo) + (now.hi - tail);
+    for (int i = tid; i < singles; i += kLogitsThreads) {
+      const int v = i < now.head - now.lo ? now.lo + i : tail + (i - (now.head - now.lo));
+      if (now.nothing || (now.mask && !((now.mask[v >> 3] >> (v & 7)) & 1u))) set_logit<F32>(out, v, -INFINITY);
+      else if (!P.in_place) {
+        if (F32) reinterpret_cast<uint32_t*>(out)[v] = reinterpret_cast<const uint32_t*>(in)[v]; else reinterpret_cast<uint16_t*>(out)[v] = reinterpret_cast<const uint16_t*>(in)[v];
+      }
+    }
   }
 }
 

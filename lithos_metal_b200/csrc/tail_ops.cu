@@ -226,14 +226,27 @@ int lm_process_logits(const lm_logits_args* a) {
   P.rho = a->repetition; P.rho_s = a->repetition_s; P.pi = a->presence; P.pi_s = a->presence_s; P.phi = a->frequency; P.phi_s = a->frequency_s;
   P.bias_ids = a->bias_ids; P.bias_ids_stride = a->bias_ids_stride; P.bias_values = a->bias_values; P.bias_values_stride = a->bias_values_stride; P.bias_len = static_cast<int>(a->bias_len);
   P.mask = a->mask; P.mask_stride = a->mask_stride; P.mask_rows = a->mask_rows; P.mask_count = static_cast<int>(a->mask_count);
+  const bool f32 = a->dtype == LM_DTYPE_F32;
+  cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  const long long at_once = static_cast<long long>(kLogitsPerSM) * sms;
+  P.table_log2 = 0;
+  if (!lists) {
+    // slices of as many logits as a block takes at once, shorter ones where these would leave SMs idle
+    const long long per = f32 ? kMaskSlice<true> : kMaskSlice<false>, few = (static_cast<long long>(a->rows) * a->vocab + at_once - 1) / at_once;
+    P.slice = static_cast<int>(((few < per ? few : per) + 31) / 32 * 32);
+    if (P.slice < kLogitsMinSlice) P.slice = kLogitsMinSlice;
+    P.slices = static_cast<int>((a->vocab + P.slice - 1) / P.slice);
+    const long long items = static_cast<long long>(P.rows) * P.slices;
+    const dim3 grid(static_cast<unsigned>(items < at_once ? items : at_once));
+    return f32 ? launch_beside(logits_mask_kernel<true>, grid, kLogitsThreads, 0, 1, st, P) : launch_beside(logits_mask_kernel<false>, grid, kLogitsThreads, 0, 1, st, P);
+  }
   // A block to a row, or to a slice of one: one block to an SM while the slices are short (the launch is then made ready beside its predecessor), otherwise rounds of kLogitsPerSM blocks to an SM
-  // that are as full as they can be. Lists that are longer than the table takes: slices no wider than that.
+  // that are as full as they can be. Lists that are longer than the hash table takes: slices no wider than a word per token takes.
   const long long names = (P.history ? P.hist_len : 0) + P.bias_len, total = static_cast<long long>(a->rows) * a->vocab;
   long long slices = 1;
   if (total <= 16384LL * sms) slices = sms / a->rows;
   else {
     double best = 0.0;
-    const long long at_once = static_cast<long long>(kLogitsPerSM) * sms;
     for (int rounds = 1; rounds <= 4; rounds++) {
       const long long n = rounds * at_once / a->rows > 1 ? rounds * at_once / a->rows : 1, items = n * a->rows;
       const double full = static_cast<double>(items) / static_cast<double>((items + at_once - 1) / at_once * at_once);
@@ -248,16 +261,15 @@ int lm_process_logits(const lm_logits_args* a) {
   P.slices = static_cast<int>((a->vocab + P.slice - 1) / P.slice);
   P.table_log2 = 8;
   while ((3LL << P.table_log2) < 4 * names) P.table_log2++;                 // three quarters full at most
-  if (P.slice <= 2LL << P.table_log2) P.table_log2 = 0;                     // (no larger than the hash table, keys and counts: a word per token)
-  const size_t smem = lists ? (P.table_log2 ? size_t{8} << P.table_log2 : static_cast<size_t>(P.slice) * 4) + static_cast<size_t>(P.slice) / 8 + 32 : 0;
-  const bool f32 = a->dtype == LM_DTYPE_F32;
-  void (*const kernel)(LogitsDev) = f32 ? (lists ? logits_kernel<true, true> : logits_kernel<true, false>) : (lists ? logits_kernel<false, true> : logits_kernel<false, false>);
-  if (lists) {
-    rc = ensure_dynamic_smem(f32 ? kSlotLogitsF32 : kSlotLogits, reinterpret_cast<const void*>(kernel), smem);
-    if (rc != LM_OK) return rc;
-  }
+  if (P.slice <= 2LL << P.table_log2) P.table_log2 = 0;                     // (no larger than the hash table: a word per token)
+  const size_t smem = (P.table_log2 ? size_t{8} << P.table_log2 : static_cast<size_t>(P.slice) * 4) + static_cast<size_t>(P.slice) / 8 + 32;
+  const bool bias = a->bias_len > 0;
+  void (*const kernel)(LogitsDev) = f32 ? (bias ? logits_kernel<true, true> : logits_kernel<true, false>) : (bias ? logits_kernel<false, true> : logits_kernel<false, false>);
+  rc = ensure_dynamic_smem(static_cast<KernelSlot>(kSlotLogits + (f32 ? 2 : 0) + (bias ? 1 : 0)), reinterpret_cast<const void*>(kernel), smem);
+  if (rc != LM_OK) return rc;
   const long long items = static_cast<long long>(P.rows) * P.slices;
-  return launch_beside(kernel, dim3(static_cast<unsigned>(items < 0x7FFFFFFF ? items : 0x7FFFFFFF)), kLogitsThreads, smem, 1, static_cast<cudaStream_t>(a->stream), P);
+  const dim3 grid(static_cast<unsigned>(items < 0x7FFFFFFF ? items : 0x7FFFFFFF));
+  return launch_beside(kernel, grid, kLogitsThreads, smem, 1, st, P);
 }
 
 }  // extern "C"
