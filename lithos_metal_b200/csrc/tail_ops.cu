@@ -51,7 +51,7 @@ int lm_quantize_nvfp4(const lm_quantize_nvfp4_args* a) {
   P.scale = a->scale; P.amax = static_cast<uint32_t*>(a->amax); P.find = a->find_scale ? 1 : 0;
   P.codes = a->codes; P.codes_stride = a->codes_stride; P.scales = a->scales; P.scales_stride = a->scales_stride;
   const long long blocks = a->rows * (a->cols / kFp4Block);
-  const unsigned grid = stride_grid(blocks, kQuantThreads, sms, 16);
+  const unsigned grid = stride_grid(blocks, kQuantThreads, sms, 8);
   const bool f32 = a->dtype == LM_DTYPE_F32;
   if (P.find) {
     const cudaError_t e = cudaMemsetAsync(P.amax, 0, sizeof(uint32_t), st);
@@ -75,7 +75,7 @@ int lm_dequantize_nvfp4(const lm_dequantize_nvfp4_args* a) {
   rc = sm_count(&sms);
   if (rc != LM_OK) return rc;
   DequantDev P{a->codes, a->codes_stride, a->scales, a->scales_stride, a->scale, a->rows, static_cast<int>(a->cols), a->out, a->out_stride};
-  return launch_stream(false, nvfp4_dequantize_kernel, dim3(stride_grid(a->rows * (a->cols / 8), kQuantThreads, sms, 16)), kQuantThreads, 0, 1, static_cast<cudaStream_t>(a->stream), P);
+  return launch_stream(false, nvfp4_dequantize_kernel, dim3(stride_grid(a->rows * (a->cols / 4), kQuantThreads, sms, 8)), kQuantThreads, 0, 1, static_cast<cudaStream_t>(a->stream), P);
 }
 
 // Rows of x that the mma.sync kernel takes: as many eights as its shared memory holds, four at most.
