@@ -237,7 +237,7 @@ class _NoHost:
     def _leave(self, *args):
         return None
 
-    sample = stochastic = argmax = draft_q = verify = lm_head = lm_head_nvfp4 = process_logits = _leave
+    sample = stochastic = argmax = draft_q = verify = lm_head = lm_head_nvfp4 = process_logits = quantize_nvfp4 = dequantize_nvfp4 = _leave
 
 
 def host():
@@ -252,7 +252,8 @@ def host():
             m = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(m)
             sampler, verify = (importlib.import_module(f"{__package__}.{n}") for n in ("sampler", "verify"))
-            names = ("lm_sample", "lm_argmax", "lm_argmax_i64", "lm_verify", "lm_draft_q", "lm_head", "lm_head_nvfp4", "lm_head_nvfp4_workspace_bytes", "lm_process_logits", "lm_workspace_bytes", "lm_verify_workspace_bytes")
+            names = ("lm_sample", "lm_argmax", "lm_argmax_i64", "lm_verify", "lm_draft_q", "lm_head", "lm_head_nvfp4", "lm_head_nvfp4_workspace_bytes", "lm_process_logits", "lm_quantize_nvfp4", "lm_dequantize_nvfp4",
+                     "lm_workspace_bytes", "lm_verify_workspace_bytes")
             m.init({n: C.cast(getattr(L, n), C.c_void_p).value for n in names}, sampler.SamplingParams, sampler.SampleOutput, verify.DraftQ, check, sampler._workspace)
         except (ImportError, OSError, RuntimeError) as e:
             warnings.warn(f"lithos_metal_b200: no native call path ({e}); calls go through ctypes", RuntimeWarning, stacklevel=3)

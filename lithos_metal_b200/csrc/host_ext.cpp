@@ -34,6 +34,8 @@ struct Abi {
   decltype(&lm_head_nvfp4) head_nvfp4 = nullptr;
   decltype(&lm_head_nvfp4_workspace_bytes) head_nvfp4_workspace_bytes = nullptr;
   decltype(&lm_process_logits) process_logits = nullptr;
+  decltype(&lm_quantize_nvfp4) quantize_nvfp4 = nullptr;
+  decltype(&lm_dequantize_nvfp4) dequantize_nvfp4 = nullptr;
   decltype(&lm_workspace_bytes) workspace_bytes = nullptr;
   decltype(&lm_verify_workspace_bytes) verify_workspace_bytes = nullptr;
 } abi;
@@ -458,6 +460,62 @@ PyObject* py_lm_head_nvfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// quantize_nvfp4(x, scale) -> (codes, scales, scale)
+PyObject* py_quantize_nvfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 2) { PyErr_SetString(PyExc_TypeError, "quantize_nvfp4: 2 arguments"); return nullptr; }
+  const at::Tensor *x = as_tensor(args[0]), *g = args[1] == Py_None ? nullptr : as_tensor(args[1]);
+  if (!x || (args[1] != Py_None && !g) || !plain_rows(*x) || x->numel() == 0 || x->size(1) % 16 != 0 || (x->size(0) > 1 && x->stride(0) < x->size(1))) return none();
+  const at::Device dev = x->device();
+  if (g && (g->scalar_type() != at::kFloat || g->device() != dev || g->numel() != 1)) return none();
+  const int64_t rows = x->size(0), cols = x->size(1), blocks = cols / 16, padded = (blocks + 15) / 16 * 16;      // (rows of scales start at multiples of 16 bytes)
+  at::Tensor codes = make({rows, cols / 2}, at::kByte, dev), scales = make({rows, padded}, at::kByte, dev), scale, amax;
+  if (padded != blocks) scales = scales.narrow(1, 0, blocks);
+  lm_quantize_nvfp4_args a{};
+  a.struct_size = sizeof(a);
+  a.dtype = dtype_code(*x); a.x = ptr(*x); a.rows = rows; a.cols = cols; a.row_stride = row_stride(*x);
+  if (g) a.scale = static_cast<float*>(ptr(*g));
+  else {
+    scale = make({1}, at::kFloat, dev); amax = make({1}, at::kInt, dev);
+    a.scale = static_cast<float*>(ptr(scale)); a.amax = ptr(amax); a.find_scale = 1;
+  }
+  a.codes = static_cast<uint8_t*>(ptr(codes)); a.codes_stride = cols / 2; a.scales = static_cast<uint8_t*>(ptr(scales)); a.scales_stride = padded;
+  a.stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const int rc = call(dev, nullptr, [&] { return abi.quantize_nvfp4(&a); });
+  if (rc != LM_OK) return failed(rc, "lm_quantize_nvfp4");
+  Ref c(THPVariable_Wrap(codes)), s(THPVariable_Wrap(scales)), o(g ? (Py_INCREF(args[1]), args[1]) : THPVariable_Wrap(scale));
+  if (!c.p || !s.p || !o.p) return nullptr;
+  return PyTuple_Pack(3, c.p, s.p, o.p);
+  END_HANDLE_TH_ERRORS
+}
+
+// dequantize_nvfp4(codes, scales, scale, out) -> out; the weight's tensors were checked when its Nvfp4Weight was made
+PyObject* py_dequantize_nvfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) { PyErr_SetString(PyExc_TypeError, "dequantize_nvfp4: 4 arguments"); return nullptr; }
+  const at::Tensor *c = as_tensor(args[0]), *s = as_tensor(args[1]), *g = as_tensor(args[2]);
+  if (!c || !s || !g) return none();
+  const at::Device dev = c->device();
+  const int64_t rows = c->size(0), cols = c->size(1) * 2;
+  at::Tensor out;
+  if (args[3] == Py_None) out = make({rows, cols}, at::kFloat, dev);
+  else {
+    const at::Tensor* t = as_tensor(args[3]);
+    if (!t || t->device() != dev || t->dim() != 2 || t->size(0) != rows || t->size(1) != cols || t->scalar_type() != at::kFloat || t->stride(1) != 1 || (rows > 1 && t->stride(0) < cols)) return none();
+    out = *t;
+  }
+  lm_dequantize_nvfp4_args a{};
+  a.struct_size = sizeof(a);
+  a.codes = static_cast<const uint8_t*>(c->const_data_ptr()); a.codes_stride = row_stride(*c); a.scales = static_cast<const uint8_t*>(s->const_data_ptr()); a.scales_stride = row_stride(*s);
+  a.scale = static_cast<const float*>(g->const_data_ptr()); a.rows = rows; a.cols = cols; a.out = static_cast<float*>(ptr(out)); a.out_stride = row_stride(out);
+  a.stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const int rc = call(dev, nullptr, [&] { return abi.dequantize_nvfp4(&a); });
+  if (rc != LM_OK) return failed(rc, "lm_dequantize_nvfp4");
+  if (args[3] != Py_None) { Py_INCREF(args[3]); return args[3]; }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // process_logits(logits, history, history_len, prompt_len, repetition, presence, frequency, bias_ids, bias_values, mask, mask_rows, out) -> out
 PyObject* py_process_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -532,10 +590,12 @@ PyObject* py_init(PyObject*, PyObject* args) {
   abi.head_nvfp4 = reinterpret_cast<decltype(abi.head_nvfp4)>(get("lm_head_nvfp4"));
   abi.head_nvfp4_workspace_bytes = reinterpret_cast<decltype(abi.head_nvfp4_workspace_bytes)>(get("lm_head_nvfp4_workspace_bytes"));
   abi.process_logits = reinterpret_cast<decltype(abi.process_logits)>(get("lm_process_logits"));
+  abi.quantize_nvfp4 = reinterpret_cast<decltype(abi.quantize_nvfp4)>(get("lm_quantize_nvfp4"));
+  abi.dequantize_nvfp4 = reinterpret_cast<decltype(abi.dequantize_nvfp4)>(get("lm_dequantize_nvfp4"));
   abi.workspace_bytes = reinterpret_cast<decltype(abi.workspace_bytes)>(get("lm_workspace_bytes"));
   abi.verify_workspace_bytes = reinterpret_cast<decltype(abi.verify_workspace_bytes)>(get("lm_verify_workspace_bytes"));
   if (PyErr_Occurred()) return nullptr;
-  if (!abi.sample || !abi.argmax || !abi.argmax_i64 || !abi.verify || !abi.draft_q || !abi.head || !abi.head_nvfp4 || !abi.head_nvfp4_workspace_bytes || !abi.process_logits || !abi.workspace_bytes || !abi.verify_workspace_bytes) {
+  if (!abi.sample || !abi.argmax || !abi.argmax_i64 || !abi.verify || !abi.draft_q || !abi.head || !abi.head_nvfp4 || !abi.head_nvfp4_workspace_bytes || !abi.process_logits || !abi.quantize_nvfp4 || !abi.dequantize_nvfp4 || !abi.workspace_bytes || !abi.verify_workspace_bytes) {
     PyErr_SetString(PyExc_ValueError, "init: an address is missing");
     return nullptr;
   }
@@ -553,6 +613,8 @@ PyMethodDef methods[] = {
     {"verify", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_verify)), METH_FASTCALL, nullptr},
     {"lm_head", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_lm_head)), METH_FASTCALL, nullptr},
     {"lm_head_nvfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_lm_head_nvfp4)), METH_FASTCALL, nullptr},
+    {"quantize_nvfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_quantize_nvfp4)), METH_FASTCALL, nullptr},
+    {"dequantize_nvfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_dequantize_nvfp4)), METH_FASTCALL, nullptr},
     {"process_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_process_logits)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "lithos_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -89,7 +89,9 @@ __device__ __forceinline__ uint32_t picked(const uint32_t (&v)[32], int j) {
 }
 
 // A block takes its tiles in passes of per_pass, in a pass the steps of 256 columns, in a step the tiles. These (step, tile) are numbered through: number i has place i % code_slots for its
-// codes and pair i % 2 of the operands in the making.
+// codes and pair i % 2 of the operands in the making. code_slots is even: a place then belongs to one pair, whose warps have all seen one filling before they wait for the next. (With three
+// places a pair could come to one whose codes for the other pair were still on their way, and a wait by parity takes the phase before the current one for the phase after it: it read codes
+// that were arriving, and the barriers lost count.)
 static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap scale_map, Batch4Dev P) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_address(smem_raw) & 1023u)) & 1023u);
@@ -136,18 +138,13 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
 #pragma unroll
     for (int i = 0; i < 4; i++) piece[i] = ((half * 4 + i) ^ (lane & 7)) << 4;
     uint32_t phase = 1u, slot_phase = 0u;
-    int slot = pair;
-    if (slot >= P.code_slots) { slot -= P.code_slots; slot_phase = 1u; }
+    int slot = pair;                                                        // (code_slots is even: slots of this pair's parity)
     for (int left = (end - begin) * steps - pair; left > 0; left -= 2) {       // (which tile and step: the copies know)
       barrier_wait(c_full + 8 * slot, slot_phase, given_up);                 // (where a wait has run out, what follows is harmless and the block writes NaN)
       uint4 cc[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) cc[i] = *reinterpret_cast<const uint4*>(code_row + slot * kB4CodeBytes + piece[i]);
       const uint2 sc = *reinterpret_cast<const uint2*>(scale_row + slot * (kB4SlotBytes - kB4CodeBytes));
-      __syncwarp();
-      if (lane == 0) barrier_arrive(c_empty + 8 * slot);
-      slot += 2;
-      if (slot >= P.code_slots) { slot -= P.code_slots; slot_phase ^= 1u; }
       barrier_wait(empty, phase, given_up);
       phase ^= 1u;
       __syncwarp();
@@ -170,7 +167,10 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) barrier_arrive(full);
+      // (The place is handed back when its codes have been converted, not when their loads have been issued: with shared memory busy these were overtaken by the copy that followed.)
+      if (lane == 0) { barrier_arrive(c_empty + 8 * slot); barrier_arrive(full); }
+      slot += 2;
+      if (slot >= P.code_slots) { slot -= P.code_slots; slot_phase ^= 1u; }
     }
   } else if (warp == kB4MmaWarp) {
     // (the whole warp walks, and one lane issues: its operands are then uniform values. A single lane's walk took 1300 clocks a tile.)

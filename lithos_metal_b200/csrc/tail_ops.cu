@@ -142,11 +142,12 @@ static int head_nvfp4_batch(const lm_head_nvfp4_args* a, const Rows4Dev& R, int 
     P.logits = static_cast<uint16_t*>(a->logits) + r * a->logits_stride;
     P.column_stride = P.n <= 32 ? 32 : P.n <= 64 ? 64 : P.n <= 128 ? 128 : 256;
     P.per_pass = kB4SumColumns / P.column_stride;
-    // of x eight pieces in shared memory (a step's four and the next's, where tiles share them) or as many as fit beside three tiles of codes, and as many of these as fit then
-    P.x_stages = static_cast<int>((kB4SmemLimit - batch4_smem_bytes(P.n, 3, 0)) / static_cast<size_t>(batch4_x_stage_bytes(P.n)));
+    // of x eight pieces in shared memory (a step's four and the next's, where tiles share them) or as many as fit beside two tiles of codes, and as many of these as fit then: an even number
+    // (batch kernel: a place's codes are then always the same pair's)
+    P.x_stages = static_cast<int>((kB4SmemLimit - batch4_smem_bytes(P.n, 2, 0)) / static_cast<size_t>(batch4_x_stage_bytes(P.n)));
     if (P.x_stages > kB4MaxXStages) P.x_stages = kB4MaxXStages;
     P.code_slots = kB4MaxCodeSlots;
-    while (batch4_smem_bytes(P.n, P.code_slots, P.x_stages) > kB4SmemLimit) P.code_slots--;
+    while (batch4_smem_bytes(P.n, P.code_slots, P.x_stages) > kB4SmemLimit) P.code_slots -= 2;
     rc = launch_stream(true, lm_head_nvfp4_batch_kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), kB4Threads, batch4_smem_bytes(P.n, P.code_slots, P.x_stages), 1, st, code_map, scale_map, P);
     if (rc != LM_OK) return rc;
   }

@@ -60,6 +60,9 @@ class Nvfp4Weight:
 
     def dequantize(self, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The float32 values [rows, cols]."""
+        r = _lib.host().dequantize_nvfp4(self.codes, self.scales, self.scale, out)
+        if r is not None:
+            return r
         rows, cols = self.shape
         if out is None:
             out = torch.empty(rows, cols, dtype=torch.float32, device=self.device)
@@ -82,6 +85,11 @@ def quantize_nvfp4(x: torch.Tensor, scale: Optional[torch.Tensor] = None) -> Nvf
     arithmetic. A block of 16 that holds a NaN or an infinity becomes NaN. Asynchronous on the current stream."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise RuntimeError("lithos_metal_b200 runs on CUDA tensors only (there is no CPU path)")
+    r = _lib.host().quantize_nvfp4(x, scale)
+    if r is not None:
+        w = Nvfp4Weight.__new__(Nvfp4Weight)                                  # (tensors of the right kind: nothing to check)
+        w.codes, w.scales, w.scale = r
+        return w
     if x.dim() != 2 or x.shape[1] % BLOCK != 0:
         raise ValueError("quantize_nvfp4: x must be [rows, cols], cols a multiple of 16")
     dtype = _dtype_code(x)

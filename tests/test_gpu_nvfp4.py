@@ -230,6 +230,22 @@ def test_a_shard_of_the_weight_gives_the_bits_of_the_whole(rows):
         assert torch.equal(torch.cat(parts, dim=1).view(torch.int16), whole.view(torch.int16))
 
 
+@pytest.mark.parametrize("rows,hidden,vocab", [(256, 4096, 20000), (200, 2048, 40000), (130, 4096, 20000), (128, 4096, 40000), (40, 4096, 40000), (17, 6400, 20000)])
+def test_rows_together_are_the_rows_one_by_eight(rows, hidden, vocab):
+    """Long runs of tiles and steps through every place of the batch kernel's shared memory, several times: within one BF16 unit of the few-rows kernel everywhere (two summation orders)."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    w = lm.Nvfp4Weight(torch.randint(0, 256, (vocab, hidden // 2), dtype=torch.uint8, device="cuda", generator=gen),
+                       torch.randint(100, 120, (vocab, hidden // 16), dtype=torch.uint8, device="cuda", generator=gen), torch.tensor([0.001], device="cuda"))
+    x = torch.randn(rows, hidden, device="cuda", generator=gen).bfloat16()
+    want = torch.cat([lm.lm_head(x[r:r + 8], w) for r in range(0, rows, 8)])
+    # sums of `hidden` products off by 2^-23 of the magnitudes' sum per addition on either side (means: |x| 0.8, the weight 0.273; the largest row's sum a quarter above that), two BF16 roundings
+    close = 2 * (hidden * 2.0 ** -23) * (hidden * 0.8 * 0.273 * 1.25) + 2 * 2.0 ** -8 * want.float().abs()
+    first = lm.lm_head(x, w)
+    assert ((first.float() - want.float()).abs() <= close).all()
+    for _ in range(6):
+        assert torch.equal(lm.lm_head(x, w).view(torch.int16), first.view(torch.int16))
+
+
 @pytest.mark.parametrize("rows", [3, 8, 50, 256])
 def test_strides_and_a_given_place(rows):
     rng = np.random.default_rng(4)

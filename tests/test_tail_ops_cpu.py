@@ -128,3 +128,38 @@ def test_the_logits_restated_token_by_token():
     got, _, touched = o_logits.process(z, history=[[1, 2, 2, 9, -1, 4, 0]], history_len=[6], prompt_len=[2], repetition=2.0, presence=0.5, frequency=0.25,
                                        bias_ids=[[4, 4, -1]], bias_values=np.array([[1.0, 2.0, 7.0]]), mask=np.array([[0b11110]], dtype=np.int32))
     assert got.tolist() == [[-np.inf, -4.0, 1.5 - 0.5 - 0.25, -4.0, 2.5 - 0.5 - 0.25 + 3.0]] and touched.tolist() == [[False, True, True, False, True]]
+
+
+def wrong_looks(places, total):
+    """The batch projection's codes: orders 0, 1, 2 .. are copied into place (order mod places), the copies complete in any order, pair (order mod 2) takes them, and looks at order i when the
+    products of order i - 4 are done (all before i - 3 taken). A place is filled again when it has been taken. Every state that can be reached; those where a wait by parity ends although the
+    order's copy is not the place's last completed one."""
+    seen, wrong, queue = set(), set(), [(0, frozenset(), 0, 1)]
+    while queue:
+        state = queue.pop()
+        if state in seen:
+            continue
+        seen.add(state)
+        issued, there, even, odd = state
+        taken = lambda i: i < (odd if i % 2 else even)
+        if issued < total and (issued < places or taken(issued - places)):
+            queue.append((issued + 1, there, even, odd))
+        queue += [(issued, there | {f}, even, odd) for f in range(issued) if f not in there]
+        for i in (even, odd):
+            if i < total and all(taken(j) for j in range(i - 3)):
+                done = sum(f % places == i % places for f in there)
+                if done % 2 != (i // places) % 2:                           # the wait for the phase of parity (i // places) % 2 ends
+                    if done != i // places + 1:
+                        wrong.add((i, done))
+                    else:
+                        queue.append((issued, there, even, i + 2) if i % 2 else (issued, there, i + 2, odd))
+    return wrong
+
+
+def test_an_even_number_of_places_for_codes_cannot_be_misread():
+    assert wrong_looks(3, 8)                                                # (the check can fail)
+    assert not any(wrong_looks(places, 9) for places in (2, 4, 6))
+    source = open(os.path.join(ROOT, "lithos_metal_b200", "csrc", "tail_ops.cu")).read()
+    assert "P.code_slots = kB4MaxCodeSlots;" in source and "P.code_slots -= 2;" in source
+    header = open(os.path.join(ROOT, "lithos_metal_b200", "csrc", "lm_head_nvfp4_batch.cuh")).read()
+    assert "kB4MaxCodeSlots = 8" in header
