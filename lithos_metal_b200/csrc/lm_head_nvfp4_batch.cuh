@@ -181,6 +181,36 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     const uint32_t other_a = a ^ (a + 2 * kB4OperandColumns), other_bar = w_full ^ (w_full + 8);    // (the two pairs in turn)
     for (int first = begin; first < end; first += P.per_pass, ap ^= 1u) {
       const int count = min(P.per_pass, end - first);
+      if (count == 1) {                                                      // one tile: x piece by piece
+        barrier_wait(acc_empty, ap, given_up);                               // (the first pass finds it empty)
+        for (int k0 = 0; k0 < H; k0 += kB4StepCols) {
+          const int quarters = min(4, (H - k0) / kB4XCols);
+          barrier_wait(w_bar, wp, given_up);
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            if (q < quarters) {
+              const uint32_t x_bar = x_full + 8 * x0;
+              barrier_wait(x_bar, xp, given_up);
+              __syncwarp();
+              if (one) {
+                const uint64_t b = operand(smem_address(xs) + x0 * x_bytes);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int k = 0; k < 4; k++) product_f16(tmem, a + 32 * q + 8 * k, b + 2 * k, form, q + k > 0 ? 1u : static_cast<uint32_t>(k0));
+                products_commit(x_bar + 8 * kB4MaxXStages);                  // (x_empty)
+              }
+              if (++x0 == P.x_stages) { x0 = 0; xp ^= 1u; }
+            }
+          }
+          if (one) products_commit(w_bar + 8 * kB4Pairs);                    // (w_empty)
+          __syncwarp();
+          a ^= other_a; w_bar ^= other_bar;
+          wp ^= w_bar == w_full ? 1u : 0u;
+        }
+        if (one) products_commit(acc_full);
+        __syncwarp();
+        continue;
+      }
       for (int k0 = 0; k0 < H; k0 += kB4StepCols) {
         const int quarters = min(4, (H - k0) / kB4XCols);
         const bool last = k0 + kB4StepCols >= H;
@@ -286,6 +316,7 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     // ---- finished accumulators: a warp has 32 vocabulary rows of every tile; a column is a row of logits
     after_predecessor();
     const int part = warp & 3;
+    const uint32_t row_bytes = static_cast<uint32_t>(P.logits_stride * 2);
     const float g = __ldg(P.scale);
     bool go = true, plain = true;                                           // plain: every g * 2^-shift is a normal binary32, with room for the sum
     for (int r = lane; r < P.n; r += 32) {                                  // (each of these warps the same values)
@@ -302,7 +333,7 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
         if (!go) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const int v = tile * kB4Tile + part * 32 + lane;
-        for (int r0 = 0; r0 < P.n; r0 += 32) {
+        for (int r0 = 32 * ((warp - kB4FirstDoneWarp) >> 2); r0 < P.n; r0 += 8 * kB4DoneWarps) {
           uint32_t a[32];
           accumulators32(tmem + (static_cast<uint32_t>(part * 32) << 16) + static_cast<uint32_t>((tile - first) * P.column_stride + r0), a);
           uint16_t* out = P.logits + r0 * P.logits_stride + v;
@@ -316,7 +347,8 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
               const float4 f = *reinterpret_cast<const float4*>(factor + r0 + j);
               const float fj[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-              for (int e = 0; e < 4; e++, out += P.logits_stride) if (j + e < there) *out = f32_to_bf16(__fmul_rn(__uint_as_float(a[j + e]), fj[e]));
+              for (int e = 0; e < 4; e++)
+                if (j + e < there) *reinterpret_cast<uint16_t*>(reinterpret_cast<unsigned char*>(out) + static_cast<uint64_t>(row_bytes) * static_cast<uint32_t>(j + e)) = f32_to_bf16(__fmul_rn(__uint_as_float(a[j + e]), fj[e]));
             }
           }
         }

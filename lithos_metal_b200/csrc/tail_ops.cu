@@ -162,7 +162,7 @@ int lm_head_nvfp4(const lm_head_nvfp4_args* a) {
   int rc = fp4_matrix_ok(a->vocab, a->hidden_dim, a->codes, a->codes_stride, a->scales, a->scales_stride, a->scale);
   if (rc != LM_OK) return rc;
   if (a->rows > LM_HEAD_NVFP4_MAX_ROWS || a->vocab > LM_MAX_VOCAB || (a->hidden_dim % 64) != 0 || a->hidden_dim > kH4MaxHidden) return LM_E_UNSUPPORTED;
-  if (a->codes_stride > 0x7FFFFFFF || a->scales_stride > 0x7FFFFFFF) return LM_E_UNSUPPORTED;
+  if (a->codes_stride > 0x7FFFFFFF || a->scales_stride > 0x7FFFFFFF || a->logits_stride > 0x3FFFFFFF) return LM_E_UNSUPPORTED;
   if (misaligned(a->codes, 16) || (a->codes_stride % 16) != 0 || misaligned(a->scales, 16) || (a->scales_stride % 16) != 0) return LM_E_UNSUPPORTED;   // 16-byte copies
   if (!a->workspace || misaligned(a->workspace, 256) || a->workspace_bytes < x4_workspace_bytes(a->rows, a->hidden_dim)) return LM_E_WORKSPACE;
   int sms = 0;
