@@ -41,6 +41,7 @@ struct Batch4Dev {
   const uint8_t* xt; const uint16_t* xb; const int* shift; const int* bad;
   uint16_t* logits; int64_t logits_stride;
   int per_pass; int column_stride; int code_slots; int x_stages;
+  int each; int left; int left_blocks; int left_n;    // tiles that every block has; tiles left over; blocks to each of these; rows of x to such a block
 };
 
 __host__ __device__ inline int batch4_x_stage_bytes(int n) { return n * kB4XCols * 2; }
@@ -88,6 +89,25 @@ __device__ __forceinline__ uint32_t picked(const uint32_t (&v)[32], int j) {
   return r;
 }
 
+// Every block has as many tiles as every other; the few left over are shared by the rows of x (a block that did one with all rows made the others wait: 256 rows of 151,936 256 us).
+struct Pass4 { int first, count, n, r0; };    // tiles first .. first + count, rows r0 .. r0 + n of x
+struct Passes4 {
+  int begin, end, per_pass, main, n, tiles; Pass4 left;
+  __device__ __forceinline__ explicit Passes4(const Batch4Dev& P) {
+    begin = blockIdx.x * P.each; end = begin + P.each; per_pass = P.per_pass; main = (P.each + per_pass - 1) / per_pass; n = P.n; tiles = P.each;
+    left = Pass4{0, 0, 0, 0};
+    if (static_cast<int>(blockIdx.x) < P.left * P.left_blocks) {
+      const int r0 = blockIdx.x % P.left_blocks * P.left_n;
+      if (r0 < P.n) { left = Pass4{static_cast<int>(gridDim.x) * P.each + static_cast<int>(blockIdx.x) / P.left_blocks, 1, min(P.left_n, P.n - r0), r0}; tiles++; }
+    }
+  }
+  __device__ __forceinline__ bool get(int i, Pass4& p) const {
+    if (i < main) { p.first = begin + i * per_pass; p.count = min(per_pass, end - p.first); p.n = n; p.r0 = 0; return true; }
+    p = left;
+    return i == main && left.count > 0;
+  }
+};
+
 // A block takes its tiles in passes of per_pass, in a pass the steps of 256 columns, in a step the tiles. These (step, tile) are numbered through: number i has place i % code_slots for its
 // codes and pair i % 2 of the operands in the making. code_slots is even: a place then belongs to one pair, whose warps have all seen one filling before they wait for the next. (With three
 // places a pair could come to one whose codes for the other pair were still on their way, and a wait by parity takes the phase before the current one for the phase after it: it read codes
@@ -101,14 +121,14 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
   unsigned char* ss = xs + P.x_stages * x_bytes;                             // scales: code_slots times [128 rows][16 bytes]
   float* factor = reinterpret_cast<float*>(ss + P.code_slots * (kB4SlotBytes - kB4CodeBytes));    // [n] g * 2^-shift
   uint64_t* bars = reinterpret_cast<uint64_t*>(factor + kB4MaxN);
-  uint32_t* words = reinterpret_cast<uint32_t*>(bars + 2 * (kB4Pairs + kB4MaxXStages + kB4MaxSums + kB4MaxCodeSlots) + 1);     // [0] tensor memory, [1] given up
+  uint32_t* words = reinterpret_cast<uint32_t*>(bars + 2 * (kB4Pairs + kB4MaxXStages + kB4MaxSums + kB4MaxCodeSlots) + 1);     // [0] tensor memory, [1] given up, [2] rows to do over
   volatile uint32_t* given_up = words + 1;
   const uint32_t w_full = smem_address(bars), w_empty = w_full + 8 * kB4Pairs, x_full = w_empty + 8 * kB4Pairs, x_empty = x_full + 8 * kB4MaxXStages, acc_full = x_empty + 8 * kB4MaxXStages,
                  acc_empty = acc_full + 8 * kB4MaxSums, c_full = acc_empty + 8 * kB4MaxSums, c_empty = c_full + 8 * kB4MaxCodeSlots, drained = c_empty + 8 * kB4MaxCodeSlots;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int H = P.hidden, steps = (H + kB4StepCols - 1) / kB4StepCols;
-  const int n_tiles = (P.vocab + kB4Tile - 1) / kB4Tile;
-  const int begin = static_cast<int>(static_cast<long long>(blockIdx.x) * n_tiles / gridDim.x), end = static_cast<int>(static_cast<long long>(blockIdx.x + 1) * n_tiles / gridDim.x);
+  const Passes4 passes(P);
+  Pass4 pass;
   if (warp == kB4MmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_address(words)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -119,7 +139,7 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     for (int s = 0; s < kB4MaxSums; s++) { barrier_init(acc_full + 8 * s, 1); barrier_init(acc_empty + 8 * s, kB4DoneWarps); }
     for (int s = 0; s < kB4MaxCodeSlots; s++) { barrier_init(c_full + 8 * s, 1); barrier_init(c_empty + 8 * s, 8); }
     barrier_init(drained, 1);
-    words[1] = 0u;
+    words[1] = words[2] = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -139,7 +159,7 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     for (int i = 0; i < 4; i++) piece[i] = ((half * 4 + i) ^ (lane & 7)) << 4;
     uint32_t phase = 1u, slot_phase = 0u;
     int slot = pair;                                                        // (code_slots is even: slots of this pair's parity)
-    for (int left = (end - begin) * steps - pair; left > 0; left -= 2) {       // (which tile and step: the copies know)
+    for (int left = passes.tiles * steps - pair; left > 0; left -= 2) {        // (which tile and step: the copies know)
       barrier_wait(c_full + 8 * slot, slot_phase, given_up);                 // (where a wait has run out, what follows is harmless and the block writes NaN)
       uint4 cc[4];
 #pragma unroll
@@ -174,43 +194,44 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     }
   } else if (warp == kB4MmaWarp) {
     // (the whole warp walks, and one lane issues: its operands are then uniform values. A single lane's walk took 1300 clocks a tile.)
-    const uint32_t form = (1u << 4) | (static_cast<uint32_t>(P.n >> 3) << 17) | (static_cast<uint32_t>(kB4Tile >> 4) << 24);   // binary16 operands, FP32 accumulators
     const bool one = elected();
     int x0 = 0;
     uint32_t a = tmem + kB4SumColumns, w_bar = w_full, wp = 0u, xp = 0u, ap = 1u;
     const uint32_t other_a = a ^ (a + 2 * kB4OperandColumns), other_bar = w_full ^ (w_full + 8);    // (the two pairs in turn)
-    for (int first = begin; first < end; first += P.per_pass, ap ^= 1u) {
-      const int count = min(P.per_pass, end - first);
-      if (count == 1) {                                                      // one tile: x piece by piece
-        barrier_wait(acc_empty, ap, given_up);                               // (the first pass finds it empty)
-        for (int k0 = 0; k0 < H; k0 += kB4StepCols) {
-          const int quarters = min(4, (H - k0) / kB4XCols);
-          barrier_wait(w_bar, wp, given_up);
+    const auto one_tile = [&](uint32_t form) {                              // x piece by piece
+      barrier_wait(acc_empty, ap, given_up);                               // (the first pass finds it empty)
+      for (int k0 = 0; k0 < H; k0 += kB4StepCols) {
+        const int quarters = min(4, (H - k0) / kB4XCols);
+        barrier_wait(w_bar, wp, given_up);
 #pragma unroll
-          for (int q = 0; q < 4; q++) {
-            if (q < quarters) {
-              const uint32_t x_bar = x_full + 8 * x0;
-              barrier_wait(x_bar, xp, given_up);
-              __syncwarp();
-              if (one) {
-                const uint64_t b = operand(smem_address(xs) + x0 * x_bytes);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (int q = 0; q < 4; q++) {
+          if (q < quarters) {
+            const uint32_t x_bar = x_full + 8 * x0;
+            barrier_wait(x_bar, xp, given_up);
+            __syncwarp();
+            if (one) {
+              const uint64_t b = operand(smem_address(xs) + x0 * x_bytes);
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-                for (int k = 0; k < 4; k++) product_f16(tmem, a + 32 * q + 8 * k, b + 2 * k, form, q + k > 0 ? 1u : static_cast<uint32_t>(k0));
-                products_commit(x_bar + 8 * kB4MaxXStages);                  // (x_empty)
-              }
-              if (++x0 == P.x_stages) { x0 = 0; xp ^= 1u; }
+              for (int k = 0; k < 4; k++) product_f16(tmem, a + 32 * q + 8 * k, b + 2 * k, form, q + k > 0 ? 1u : static_cast<uint32_t>(k0));
+              products_commit(x_bar + 8 * kB4MaxXStages);                  // (x_empty)
             }
+            if (++x0 == P.x_stages) { x0 = 0; xp ^= 1u; }
           }
-          if (one) products_commit(w_bar + 8 * kB4Pairs);                    // (w_empty)
-          __syncwarp();
-          a ^= other_a; w_bar ^= other_bar;
-          wp ^= w_bar == w_full ? 1u : 0u;
         }
-        if (one) products_commit(acc_full);
+        if (one) products_commit(w_bar + 8 * kB4Pairs);                    // (w_empty)
         __syncwarp();
-        continue;
+        a ^= other_a; w_bar ^= other_bar;
+        wp ^= w_bar == w_full ? 1u : 0u;
       }
+      if (one) products_commit(acc_full);
+      __syncwarp();
+    };
+    const auto form_of = [](int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kB4Tile >> 4) << 24); };    // binary16 operands, FP32 accumulators
+    const uint32_t form = form_of(P.n);
+    for (int first = passes.begin; first < passes.end; first += P.per_pass, ap ^= 1u) {
+      const int count = min(P.per_pass, passes.end - first);
+      if (count == 1) { one_tile(form); continue; }
       for (int k0 = 0; k0 < H; k0 += kB4StepCols) {
         const int quarters = min(4, (H - k0) / kB4XCols);
         const bool last = k0 + kB4StepCols >= H;
@@ -259,6 +280,7 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
         if (x0 >= P.x_stages) { x0 -= P.x_stages; xp ^= 1u; }
       }
     }
+    if (passes.left.count > 0) one_tile(form_of(passes.left.n));
     if (*given_up && one) {                                                 // what is under way ends before the block does
       products_commit(drained);
       for (uint32_t i = 0; i < kWait4Limit && !barrier_try(drained, 0u); i++) {}
@@ -268,12 +290,13 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     if (lane == 0) {
       int stage = 0, issued = 0; uint32_t phase = 0u;
       bool go = true;
-      for (int first = begin; go && first < end; first += P.per_pass) {
+      for (int i = 0; go && passes.get(i, pass); i++) {
+        const uint32_t bytes = static_cast<uint32_t>(pass.n * kB4XCols * 2);
         for (int k = 0; k < H / kB4XCols; k++) {
           go = barrier_wait(x_empty + 8 * stage, phase ^ 1u, given_up);
           if (!go) break;
-          barrier_expect(x_full + 8 * stage, static_cast<uint32_t>(x_bytes));
-          bulk_copy(smem_address(xs) + stage * x_bytes, P.xt + static_cast<size_t>(k) * x_bytes, static_cast<uint32_t>(x_bytes), x_full + 8 * stage);
+          barrier_expect(x_full + 8 * stage, bytes);
+          bulk_copy(smem_address(xs) + stage * x_bytes, P.xt + static_cast<size_t>(k) * x_bytes + pass.r0 * (kB4XCols * 2), bytes, x_full + 8 * stage);
           issued++;
           if (++stage == P.x_stages) { stage = 0; phase ^= 1u; }
         }
@@ -290,10 +313,9 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
       bool go = true;
       int issued = 0, slot = 0;
       uint32_t phase = 0u;
-      for (int first = begin; go && first < end; first += P.per_pass) {
-        const int last = min(first + P.per_pass, end);
+      for (int i = 0; go && passes.get(i, pass); i++) {
         for (int step = 0; go && step < steps; step++) {
-          for (int tile = first; tile < last; tile++) {
+          for (int tile = pass.first; tile < pass.first + pass.count; tile++) {
             const uint32_t bar = c_full + 8 * slot;
             go = barrier_wait(c_empty + 8 * slot, phase ^ 1u, given_up);
             if (!go) break;
@@ -318,30 +340,32 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     const int part = warp & 3;
     const uint32_t row_bytes = static_cast<uint32_t>(P.logits_stride * 2);
     const float g = __ldg(P.scale);
-    bool go = true, plain = true;                                           // plain: every g * 2^-shift is a normal binary32, with room for the sum
+    bool go = true, plain = true, bad = false;                              // plain: every g * 2^-shift is a normal binary32, with room for the sum
     for (int r = lane; r < P.n; r += 32) {                                  // (each of these warps the same values)
       const double f = static_cast<double>(g) * __hiloint2double((1023 - P.shift[r]) << 20, 0);
       plain &= fabs(f) >= 0x1p-100 && fabs(f) <= 0x1p80;
       factor[r] = static_cast<float>(f);
+      bad |= P.bad[r] != 0;
     }
+    if (bad) words[2] = 1u;
     plain = __all_sync(kFull, plain);
     uint32_t phase = 0u;
-    for (int first = begin; go && first < end; first += P.per_pass, phase ^= 1u) {
-      const int last = min(first + P.per_pass, end);
-      for (int tile = first; tile < last; tile++) {
-        go = __all_sync(kFull, barrier_wait(acc_full + 8 * (tile - first), phase, given_up));
+    for (int i = 0; go && passes.get(i, pass); i++, phase ^= 1u) {
+      for (int sum = 0; sum < pass.count; sum++) {
+        const int tile = pass.first + sum;
+        go = __all_sync(kFull, barrier_wait(acc_full + 8 * sum, phase, given_up));
         if (!go) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const int v = tile * kB4Tile + part * 32 + lane;
-        for (int r0 = 32 * ((warp - kB4FirstDoneWarp) >> 2); r0 < P.n; r0 += 8 * kB4DoneWarps) {
+        const int v = tile * kB4Tile + part * 32 + lane, rows = min(P.rows, pass.r0 + pass.n);
+        for (int r0 = pass.r0 + 32 * ((warp - kB4FirstDoneWarp) >> 2); r0 < pass.r0 + pass.n; r0 += 8 * kB4DoneWarps) {
           uint32_t a[32];
-          accumulators32(tmem + (static_cast<uint32_t>(part * 32) << 16) + static_cast<uint32_t>((tile - first) * P.column_stride + r0), a);
+          accumulators32(tmem + (static_cast<uint32_t>(part * 32) << 16) + static_cast<uint32_t>(sum * P.column_stride + r0 - pass.r0), a);
           uint16_t* out = P.logits + r0 * P.logits_stride + v;
           if (!plain) {
             for (int j = 0; j < 32; j++)
-              if (v < P.vocab && r0 + j < P.rows) out[j * P.logits_stride] = f32_to_bf16(head4_finish(__uint_as_float(picked(a, j)), g, P.shift[r0 + j]));
+              if (v < P.vocab && r0 + j < rows) out[j * P.logits_stride] = f32_to_bf16(head4_finish(__uint_as_float(picked(a, j)), g, P.shift[r0 + j]));
           } else {
-            const int there = v < P.vocab ? P.rows - r0 : 0;                  // rows of logits among the 32
+            const int there = v < P.vocab ? rows - r0 : 0;                  // rows of logits among the 32
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
               const float4 f = *reinterpret_cast<const float4*>(factor + r0 + j);
@@ -354,7 +378,7 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) barrier_arrive(acc_empty + 8 * (tile - first));
+        if (lane == 0) barrier_arrive(acc_empty + 8 * sum);
       }
     }
   }
@@ -364,19 +388,17 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   if (warp == kB4MmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
-  const int v0 = begin * kB4Tile, v1 = min(end * kB4Tile, P.vocab);
-  if (*given_up) {
-    for (int r = 0; r < P.rows; r++)
-      for (int v = v0 + tid; v < v1; v += kB4Threads) P.logits[r * P.logits_stride + v] = 0x7FFFu;
-    return;
-  }
-  // ---- rows whose x is no binary16 after the scaling: FP64
-  for (int r = 0; r < P.rows; r++) {
-    if (!P.bad[r]) continue;
+  // ---- rows whose x is no binary16 after the scaling, or (a wait ran out) everything of this block's
+  const bool all = *given_up != 0u;
+  for (int r = 0; r < P.rows && (all || words[2]); r++) {                   // (256 looks one after the other took 10 us and more)
+    if (!all && !P.bad[r]) continue;
     const uint16_t* x = P.xb + static_cast<size_t>(r) * H;
-    for (int v = v0 + warp; v < v1; v += kB4Threads / 32) {
-      const double sum = exact_sum(x, P.codes + v * P.codes_stride, P.scales + v * P.scales_stride, H, lane);
-      if (lane == 0) P.logits[r * P.logits_stride + v] = f32_to_bf16(head4_finish(sum, __ldg(P.scale), 0));
+    for (int i = 0; passes.get(i, pass); i++) {
+      if (r < pass.r0 || r >= pass.r0 + pass.n) continue;
+      for (int v = pass.first * kB4Tile + warp; v < min((pass.first + pass.count) * kB4Tile, P.vocab); v += kB4Threads / 32) {
+        const float z = all ? __int_as_float(0x7FC00000) : head4_finish(exact_sum(x, P.codes + v * P.codes_stride, P.scales + v * P.scales_stride, H, lane), __ldg(P.scale), 0);
+        if (lane == 0) P.logits[r * P.logits_stride + v] = f32_to_bf16(z);
+      }
     }
   }
 }

@@ -148,7 +148,13 @@ static int head_nvfp4_batch(const lm_head_nvfp4_args* a, const Rows4Dev& R, int 
     if (P.x_stages > kB4MaxXStages) P.x_stages = kB4MaxXStages;
     P.code_slots = kB4MaxCodeSlots;
     while (batch4_smem_bytes(P.n, P.code_slots, P.x_stages) > kB4SmemLimit) P.code_slots -= 2;
-    rc = launch_stream(true, lm_head_nvfp4_batch_kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), kB4Threads, batch4_smem_bytes(P.n, P.code_slots, P.x_stages), 1, st, code_map, scale_map, P);
+    // Left over, or all there are: as many blocks to each as there are blocks, or sixteens of rows.
+    P.each = tiles / sms; P.left = tiles % sms;
+    P.left_blocks = P.left == 0 ? 1 : sms / P.left < P.n / 16 ? sms / P.left : P.n / 16;
+    P.left_n = ((P.n + P.left_blocks - 1) / P.left_blocks + 15) / 16 * 16;
+    P.left_blocks = (P.n + P.left_n - 1) / P.left_n;
+    const int grid = P.each > 0 ? sms : P.left * P.left_blocks;
+    rc = launch_stream(true, lm_head_nvfp4_batch_kernel, dim3(static_cast<unsigned>(grid)), kB4Threads, batch4_smem_bytes(P.n, P.code_slots, P.x_stages), 1, st, code_map, scale_map, P);
     if (rc != LM_OK) return rc;
   }
   return LM_OK;
