@@ -38,8 +38,8 @@ enum KernelSlot { kSlotFast, kSlotTopk, kSlotTopkOrdered, kSlotGeneric, kSlotVoc
                   kSlotDraftQ = kSlotArgmax + 2,    // (two instances)
                   kSlotVerify = kSlotDraftQ + 2,    // (twelve)
                   kSlotVerifyGiven = kSlotVerify + 12,   // (four)
-                  kSlotHeadNvfp4 = kSlotVerifyGiven + 4,     // (four)
-                  kSlotHeadNvfp4Batch = kSlotHeadNvfp4 + 4,
+                  kSlotHeadNvfp4 = kSlotVerifyGiven + 4,     // (two)
+                  kSlotHeadNvfp4Batch = kSlotHeadNvfp4 + 2,
                   kSlotLogits,                      // (four)
                   kSlotCount = kSlotLogits + 4 };
 

@@ -1,5 +1,5 @@
 // The vocabulary projection of a decode step with a 4-bit weight (nvfp4.cuh): logits[t, v] = bf16(g * sum_k x[t, k] * e2m1(c[v, k]) * e4m3(s[v, k / 16])),
-// FP32 accumulation, for up to 8 NT rows (NT of 1 to 4), the final RMSNorm fused on the input as in lm_head.cuh (the norm's output is rounded to BF16 by definition).
+// FP32 accumulation, for up to 8 NT rows (NT of 1 or 2), the final RMSNorm fused on the input as in lm_head.cuh (the norm's output is rounded to BF16 by definition).
 //
 // The weight is read once: 0.5625 bytes an element instead of 2 (350 MB for 151,936 x 4096: 53 us at the measured copy rate), so an SM has to take in
 // some 43 weights a clock. A code becomes binary16 by the conversion instruction (two codes each), times its block's scale by one packed multiplication:
@@ -25,7 +25,7 @@ namespace lm {
 constexpr int kH4Threads = 512;
 constexpr int kH4Warps = kH4Threads / 32;
 constexpr int kH4Rows = 8;                   // rows of x to an mma (its n dimension)
-constexpr int kH4MaxNT = 4;
+constexpr int kH4MaxNT = 2;
 constexpr int kH4Tile = 16;                  // vocabulary rows per warp tile (the m dimension)
 constexpr int kH4Step = 256;                 // columns per step: 32 bytes of codes per thread and row, a whole 128-byte line per row and quad
 constexpr int kH4MaxHidden = 12736;

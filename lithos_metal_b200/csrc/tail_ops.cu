@@ -78,7 +78,9 @@ int lm_dequantize_nvfp4(const lm_dequantize_nvfp4_args* a) {
   return launch_stream(false, nvfp4_dequantize_kernel, dim3(stride_grid(a->rows * (a->cols / 4), kQuantThreads, sms, 8)), kQuantThreads, 0, 1, static_cast<cudaStream_t>(a->stream), P);
 }
 
-// Rows of x that the mma.sync kernel takes: as many eights as its shared memory holds, four at most.
+// Whether the mma.sync kernel takes the call: 16 rows at most (its products grow by eights of rows, the other kernel's conversion of the weight is the same for all), and two eights only where
+// shared memory holds them. Measured, mma.sync against tcgen05: 16 rows of 50,257 x 4096 38.9 and 47.2 us, of 20,011 x 1024 10.9 and 13.2, of 4,099 x 4096 11.6 and 18.2, of 151,936 x 4096
+// 89.8 and 94.6, of 128,000 x 2048 44.8 and 43.7; 24 rows (with three eights) 50.7 and 47.2, 12.8 and 13.3, 13.0 and 18.1, 125.6 and 96.5, 55.5 and 44.6.
 static bool head4_few_rows(int64_t rows, int64_t hidden) {
   const int64_t nt = (rows + kH4Rows - 1) / kH4Rows;
   return nt <= 1 || (nt <= kH4MaxNT && head4_smem_bytes(static_cast<int>(hidden), static_cast<int>(nt)) <= 200 * 1024);
@@ -185,12 +187,7 @@ int lm_head_nvfp4(const lm_head_nvfp4_args* a) {
   rc = launch_beside(nvfp4_rows_kernel, dim3(static_cast<unsigned>(R.few ? R.rows : padded)), kX4Threads, 0, 1, static_cast<cudaStream_t>(a->stream), R);
   if (rc != LM_OK) return rc;
   if (!R.few) return head_nvfp4_batch(a, R, sms);
-  switch ((a->rows + kH4Rows - 1) / kH4Rows) {
-    case 1: return head_nvfp4_few(lm_head_nvfp4_kernel<1, 4>, a, R, 1, sms);
-    case 2: return head_nvfp4_few(lm_head_nvfp4_kernel<2, 3>, a, R, 2, sms);
-    case 3: return head_nvfp4_few(lm_head_nvfp4_kernel<3, 2>, a, R, 3, sms);
-    default: return head_nvfp4_few(lm_head_nvfp4_kernel<4, 2>, a, R, 4, sms);
-  }
+  return a->rows <= kH4Rows ? head_nvfp4_few(lm_head_nvfp4_kernel<1, 4>, a, R, 1, sms) : head_nvfp4_few(lm_head_nvfp4_kernel<2, 3>, a, R, 2, sms);
 }
 
 // Whether writing `out` can change what is read of `in` (both [rows, vocab] in elements of `size` bytes): same place and strides is in place, sharing nothing is fine.
