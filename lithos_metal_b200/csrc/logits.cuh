@@ -96,44 +96,55 @@ struct TokenTable {
   }
 };
 
+// A block's slice of a row: what the parts of the kernel below each work out for themselves (kept over the streaming loop, the lists' values were spilled there: 1024 rows of 151,936 with a history
+// of 2048 tokens 150 us, with a bias that is never reached in the code behind the loop 180).
+template <bool F32> struct Slice {
+  int row, lo, hi; const unsigned char* in; unsigned char* out; const uint8_t* mask; bool nothing, stream;
+  __device__ __forceinline__ explicit Slice(const LogitsDev& P) {
+    uint32_t item = blockIdx.x;
+    asm volatile("" : "+r"(item));
+    constexpr int kSize = F32 ? 4 : 2;
+    row = static_cast<int>(item / static_cast<uint32_t>(P.slices)); lo = (static_cast<int>(item) - row * P.slices) * P.slice; hi = min(lo + P.slice, P.vocab);
+    in = static_cast<const unsigned char*>(P.in) + row * P.in_stride * kSize; out = static_cast<unsigned char*>(P.out) + row * P.out_stride * kSize;
+    const int which = P.mask ? (P.mask_rows ? P.mask_rows[row] : row) : -1;
+    nothing = which >= P.mask_count && which >= 0;                          // the row's mask does not exist: everything is masked
+    mask = which >= 0 && !nothing ? reinterpret_cast<const uint8_t*>(P.mask + which * P.mask_stride) : nullptr;     // the row's bits, or none
+    stream = !P.in_place || mask || nothing;
+  }
+  __device__ __forceinline__ bool keeps(int v) const { return !nothing && (!mask || ((mask[v >> 3] >> (v & 7)) & 1u)); }
+};
+
 template <bool F32, bool kBias>
 static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_kernel(LogitsDev P) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ float s_knob[3];                                               // rho, pi, phi
   const TokenTable table(smem_raw, P.table_log2, P.slice);
   uint32_t* named = table.end();                                            // [slice / 32 + 1] a bit for every token of the history
   constexpr int kSize = F32 ? 4 : 2, kAhead = F32 ? 2 : 4;
   const int tid = threadIdx.x;
   after_predecessor();
-  const long long items = static_cast<long long>(P.rows) * P.slices;
-  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-    const int row = static_cast<int>(item / P.slices), lo = static_cast<int>(item % P.slices) * P.slice, hi = min(lo + P.slice, P.vocab);
-    const unsigned char* in = static_cast<const unsigned char*>(P.in) + row * P.in_stride * kSize;
-    unsigned char* out = static_cast<unsigned char*>(P.out) + row * P.out_stride * kSize;
-    const int which = P.mask ? (P.mask_rows ? P.mask_rows[row] : row) : -1;
-    const bool nothing = which >= P.mask_count && which >= 0;               // the row's mask does not exist: everything is masked
-    const uint8_t* mask = which >= 0 && !nothing ? reinterpret_cast<const uint8_t*>(P.mask + which * P.mask_stride) : nullptr;     // the row's bits, or none
-    const bool stream = !P.in_place || mask || nothing;
-    auto keeps = [&](int v) { return !nothing && (!mask || ((mask[v >> 3] >> (v & 7)) & 1u)); };
-    // ---- the lists
-    const int n_hist = P.history && !nothing ? min(P.lengths ? max(P.lengths[row], 0) : P.hist_len, P.hist_len) : 0;
-    const int n_bias = !kBias || nothing ? 0 : P.bias_len;
-    const int32_t* hist = P.history + row * P.hist_stride;
-    const int32_t* ids = P.bias_ids + row * P.bias_ids_stride;
-    const float rho = P.rho ? P.rho[row] : P.rho_s, pi = P.pi ? P.pi[row] : P.pi_s, phi = P.phi ? P.phi[row] : P.phi_s;
-    auto penalised = [&](float z, uint32_t n) {
-      if (n & (kSeen | kOutMask)) z = (z > 0.0f) ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
-      if (n & kOutMask) z = __fsub_rn(__fsub_rn(z, pi), __fmul_rn(phi, static_cast<float>(n & kOutMask)));
-      return z;
-    };
+  auto penalised = [&](float z, uint32_t n) {
+    if (n & (kSeen | kOutMask)) z = (z > 0.0f) ? __fdiv_rn(z, s_knob[0]) : __fmul_rn(z, s_knob[0]);
+    if (n & kOutMask) z = __fsub_rn(__fsub_rn(z, s_knob[1]), __fmul_rn(s_knob[2], static_cast<float>(n & kOutMask)));
+    return z;
+  };
+  // ---- the lists
+  bool history;
+  {
+    const Slice<F32> S(P);
+    const int n_hist = P.history && !S.nothing ? min(P.lengths ? max(P.lengths[S.row], 0) : P.hist_len, P.hist_len) : 0, n_bias = !kBias || S.nothing ? 0 : P.bias_len;
+    history = n_hist > 0;
+    if (tid == 0) { s_knob[0] = P.rho ? P.rho[S.row] : P.rho_s; s_knob[1] = P.pi ? P.pi[S.row] : P.pi_s; s_knob[2] = P.phi ? P.phi[S.row] : P.phi_s; }
     if (n_hist || n_bias) {
-      const uint32_t width = static_cast<uint32_t>(hi - lo);
+      const uint32_t width = static_cast<uint32_t>(S.hi - S.lo);
+      const int32_t *hist = P.history + S.row * P.hist_stride, *ids = P.bias_ids + S.row * P.bias_ids_stride;
       table.clear();
       __syncthreads();
-      const int prompt = P.prompts ? P.prompts[row] : 0;
+      const int prompt = P.prompts ? P.prompts[S.row] : 0;
       for (int base = tid; base < n_hist; base += 4 * kLogitsThreads) {
         uint32_t t[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) t[e] = base + e * kLogitsThreads < n_hist ? static_cast<uint32_t>(hist[base + e * kLogitsThreads]) - static_cast<uint32_t>(lo) : kNoToken;
+        for (int e = 0; e < 4; e++) t[e] = base + e * kLogitsThreads < n_hist ? static_cast<uint32_t>(hist[base + e * kLogitsThreads]) - static_cast<uint32_t>(S.lo) : kNoToken;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const uint32_t v = t[e];
@@ -145,129 +156,136 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
         }
       }
       for (int i = tid; i < n_bias; i += kLogitsThreads) {
-        const uint32_t v = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(lo);
+        const uint32_t v = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(S.lo);
         if (v < width) atomicAdd(table.insert(v), kBiasOne);
       }
       __syncthreads();
     }
-    // ---- the slice: [lo, head) singly, then chunks of 8 from 16-byte boundaries, then the rest singly
-    if (stream) {
-      int head = lo, chunks = 0;
-      if (((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0) {
-        const uintptr_t at = reinterpret_cast<uintptr_t>(out) + static_cast<uintptr_t>(lo) * kSize;
-        head = min(lo + static_cast<int>(((16u - (at & 15u)) & 15u) / kSize), hi);
-        chunks = (hi - head) / 8;
+  }
+  // ---- the slice: [lo, head) singly, then chunks of 8 from 16-byte boundaries, then the rest singly
+  {
+    const Slice<F32> S(P);
+    const unsigned char* const in = S.in;
+    unsigned char* const out = S.out;
+    const uint8_t* const mask = S.mask;
+    const int lo = S.lo, hi = S.stream ? S.hi : S.lo;
+    int head = lo, chunks = 0;
+    if (((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(out) + static_cast<uintptr_t>(lo) * kSize;
+      head = min(lo + static_cast<int>(((16u - (at & 15u)) & 15u) / kSize), hi);
+      chunks = (hi - head) / 8;
+    }
+    const int tail = head + 8 * chunks, singles = (head - lo) + (hi - tail);
+    for (int i = tid; i < singles; i += kLogitsThreads) {
+      const int v = i < head - lo ? lo + i : tail + (i - (head - lo));
+      if (!S.keeps(v)) { set_logit<F32>(out, v, -INFINITY); continue; }
+      if (history && ((named[(v - lo) >> 5] >> ((v - lo) & 31)) & 1u)) {
+        const uint32_t n = table.counts(static_cast<uint32_t>(v - lo));
+        if (!kBias || !(n & kBiasMask)) { set_logit<F32>(out, v, penalised(logit_at<F32>(in, v), n)); continue; }
       }
-      const int tail = head + 8 * chunks, singles = (head - lo) + (hi - tail);
-      for (int i = tid; i < singles; i += kLogitsThreads) {
-        const int v = i < head - lo ? lo + i : tail + (i - (head - lo));
-        if (!keeps(v)) { set_logit<F32>(out, v, -INFINITY); continue; }
-        if (n_hist && ((named[(v - lo) >> 5] >> ((v - lo) & 31)) & 1u)) {
-          const uint32_t n = table.counts(static_cast<uint32_t>(v - lo));
-          if (!kBias || !(n & kBiasMask)) { set_logit<F32>(out, v, penalised(logit_at<F32>(in, v), n)); continue; }
-        }
-        if (!P.in_place) {
-          if (F32) reinterpret_cast<uint32_t*>(out)[v] = reinterpret_cast<const uint32_t*>(in)[v]; else reinterpret_cast<uint16_t*>(out)[v] = reinterpret_cast<const uint16_t*>(in)[v];
-        }
-      }
-      const int shift = head & 7;                                            // of a chunk's bits in their byte (lo is a multiple of 32)
-      // the mask's bits of kAhead chunks, 8 for each
-      auto kept = [&](int c0) {
-        uint32_t keep = nothing ? 0u : 0xFFFFFFFFu;
-        if (mask) {
-          const uint8_t* p = mask + (head >> 3) + c0;
-          keep = 0u;
-#pragma unroll
-          for (int u = 0; u < kAhead; u++) {
-            if (c0 + u * kLogitsThreads < chunks) {
-              uint32_t k = __ldg(p + u * kLogitsThreads);
-              if (shift) k = ((k | static_cast<uint32_t>(__ldg(p + u * kLogitsThreads + 1)) << 8) >> shift) & 0xFFu;     // (v + 7 is in the row, and so is its byte)
-              keep |= k << (8 * u);
-            }
-          }
-        }
-        return keep;
-      };
-      uint32_t next = kept(tid);
-      for (int c0 = tid; c0 < chunks; c0 += kLogitsThreads * kAhead) {
-        const unsigned char* from = in + static_cast<int64_t>(head + 8 * c0) * kSize;
-        unsigned char* to = out + static_cast<int64_t>(head + 8 * c0) * kSize;
-        Chunk<F32> x[kAhead];
-        const uint32_t keep = next;
-        uint32_t touched = 0u;                                               // 8 bits for each chunk
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-          const uint32_t k = (keep >> (8 * u)) & 0xFFu;
-          if (c0 + u * kLogitsThreads < chunks && k != 0u && !(P.in_place && k == 0xFFu)) x[u].load(from + u * (kLogitsThreads * 8 * kSize));
-        }
-        next = kept(c0 + kLogitsThreads * kAhead);
-        if (n_hist) {
-          const uint8_t* p = reinterpret_cast<const uint8_t*>(named) + ((head - lo) >> 3) + c0;
-#pragma unroll
-          for (int u = 0; u < kAhead; u++) {
-            if (c0 + u * kLogitsThreads < chunks) {
-              uint32_t k = p[u * kLogitsThreads];
-              if (shift) k = ((k | static_cast<uint32_t>(p[u * kLogitsThreads + 1]) << 8) >> shift) & 0xFFu;
-              touched |= k << (8 * u);
-            }
-          }
-          touched &= keep;
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-          const uint32_t k = (keep >> (8 * u)) & 0xFFu;
-          if (c0 + u * kLogitsThreads < chunks && !(P.in_place && k == 0xFFu)) {
-            if (k != 0xFFu) x[u].apply(k);
-            x[u].store(to + u * (kLogitsThreads * 8 * kSize));
-          }
-        }
-        for (; touched; touched &= touched - 1u) {                           // (behind the stores of their chunks, by the same thread)
-          const int b = __ffs(static_cast<int>(touched)) - 1, u = b >> 3, v = (c0 + u * kLogitsThreads) * 8 + (b & 7);     // from head on
-          const uint32_t n = table.counts(static_cast<uint32_t>(head - lo + v));
-          if (kBias && (n & kBiasMask)) continue;                                       // (set below, from the logit itself)
-          set_logit<F32>(out, head + v, penalised(logit_at<F32>(in, head + v), n));     // (read again, from the line just loaded)
-        }
+      if (!P.in_place) {
+        if (F32) reinterpret_cast<uint32_t*>(out)[v] = reinterpret_cast<const uint32_t*>(in)[v]; else reinterpret_cast<uint16_t*>(out)[v] = reinterpret_cast<const uint16_t*>(in)[v];
       }
     }
-    // ---- tokens of the history where nothing was streamed, and those with a bias
-    if ((n_hist || n_bias) && (!stream || n_bias)) {
-      __syncthreads();
-      const uint32_t width = static_cast<uint32_t>(hi - lo);
-      if (!stream) {
-        for (int i = tid; i < table.entries(); i += kLogitsThreads) {
-          const uint32_t v = table.log2 ? table.word[2 * i] : static_cast<uint32_t>(i), n = table.word[table.log2 ? 2 * i + 1 : i];
-          if ((n & (kSeen | kOutMask)) && !(n & kBiasMask)) set_logit<F32>(out, lo + static_cast<int>(v), penalised(logit_at<F32>(in, lo + static_cast<int>(v)), n));
+    const int shift = head & 7;                                            // of a chunk's bits in their byte (lo is a multiple of 32)
+    // the mask's bits of kAhead chunks, 8 for each
+    auto kept = [&](int c0) {
+      uint32_t keep = S.nothing ? 0u : 0xFFFFFFFFu;
+      if (mask) {
+        const uint8_t* p = mask + (head >> 3) + c0;
+        keep = 0u;
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+          if (c0 + u * kLogitsThreads < chunks) {
+            uint32_t k = __ldg(p + u * kLogitsThreads);
+            if (shift) k = ((k | static_cast<uint32_t>(__ldg(p + u * kLogitsThreads + 1)) << 8) >> shift) & 0xFFu;     // (v + 7 is in the row, and so is its byte)
+            keep |= k << (8 * u);
+          }
         }
       }
-      const float* values = P.bias_values + row * P.bias_values_stride;
-      for (int base = tid & ~31; base < n_bias; base += kLogitsThreads) {      // (a warp together)
-        const int i = base + (tid & 31), id = i < n_bias ? ids[i] : -1;
-        const uint32_t v = static_cast<uint32_t>(id) - static_cast<uint32_t>(lo);
-        const bool mine = i < n_bias && v < width && keeps(id);
-        const uint32_t n = mine ? table.counts(v) : 0u;
-        const bool alone = (n & kBiasMask) == kBiasOne;
-        float z = mine ? penalised(logit_at<F32>(in, id), n) : 0.0f;
-        if (mine && alone) set_logit<F32>(out, id, __fadd_rn(z, values[i]));
-        // tokens listed more than once: the first entry adds all values in list order, the warp looks for them
-        for (uint32_t others = __ballot_sync(kFull, mine && !alone); others; others &= others - 1u) {
-          const int lane = __ffs(static_cast<int>(others)) - 1, what = __shfl_sync(kFull, id, lane);
-          float sum = __shfl_sync(kFull, z, lane);
-          int first = -1;
-          for (int e0 = 0; e0 < n_bias; e0 += 32) {
-            const int e = e0 + (tid & 31);
-            const bool same = e < n_bias && ids[e] == what;
-            const float value = same ? values[e] : 0.0f;
-            for (uint32_t m = __ballot_sync(kFull, same); m; m &= m - 1u) {
-              const int at = __ffs(static_cast<int>(m)) - 1;
-              if (first < 0) first = e0 + at;
-              sum = __fadd_rn(sum, __shfl_sync(kFull, value, at));
-            }
+      return keep;
+    };
+    uint32_t next = kept(tid);
+    for (int c0 = tid; c0 < chunks; c0 += kLogitsThreads * kAhead) {
+      const unsigned char* from = in + static_cast<int64_t>(head + 8 * c0) * kSize;
+      unsigned char* to = out + static_cast<int64_t>(head + 8 * c0) * kSize;
+      Chunk<F32> x[kAhead];
+      const uint32_t keep = next;
+      uint32_t touched = 0u;                                               // 8 bits for each chunk
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) {
+        const uint32_t k = (keep >> (8 * u)) & 0xFFu;
+        if (c0 + u * kLogitsThreads < chunks && k != 0u && !(P.in_place && k == 0xFFu)) x[u].load(from + u * (kLogitsThreads * 8 * kSize));
+      }
+      next = kept(c0 + kLogitsThreads * kAhead);
+      if (history) {
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(named) + ((head - lo) >> 3) + c0;
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+          if (c0 + u * kLogitsThreads < chunks) {
+            uint32_t k = p[u * kLogitsThreads];
+            if (shift) k = ((k | static_cast<uint32_t>(p[u * kLogitsThreads + 1]) << 8) >> shift) & 0xFFu;
+            touched |= k << (8 * u);
           }
-          if ((tid & 31) == lane && first == i) set_logit<F32>(out, id, sum);
         }
+        touched &= keep;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) {
+        const uint32_t k = (keep >> (8 * u)) & 0xFFu;
+        if (c0 + u * kLogitsThreads < chunks && !(P.in_place && k == 0xFFu)) {
+          if (k != 0xFFu) x[u].apply(k);
+          x[u].store(to + u * (kLogitsThreads * 8 * kSize));
+        }
+      }
+      for (; touched; touched &= touched - 1u) {                           // (behind the stores of their chunks, by the same thread)
+        const int b = __ffs(static_cast<int>(touched)) - 1, u = b >> 3, v = (c0 + u * kLogitsThreads) * 8 + (b & 7);     // from head on
+        const uint32_t n = table.counts(static_cast<uint32_t>(head - lo + v));
+        if (kBias && (n & kBiasMask)) continue;                                       // (set below, from the logit itself)
+        set_logit<F32>(out, head + v, penalised(logit_at<F32>(in, head + v), n));     // (read again, from the line just loaded)
       }
     }
-    __syncthreads();                                                        // the tables are the next slice's
+  }
+  // ---- tokens of the history where nothing was streamed, and those with a bias
+  const Slice<F32> S(P);
+  if ((history && !S.stream) || (kBias && !S.nothing)) {
+    __syncthreads();
+    const uint32_t width = static_cast<uint32_t>(S.hi - S.lo);
+    if (!S.stream) {
+      for (int i = tid; i < table.entries(); i += kLogitsThreads) {
+        const uint32_t v = table.log2 ? table.word[2 * i] : static_cast<uint32_t>(i), n = table.word[table.log2 ? 2 * i + 1 : i];
+        if ((n & (kSeen | kOutMask)) && !(n & kBiasMask)) set_logit<F32>(S.out, S.lo + static_cast<int>(v), penalised(logit_at<F32>(S.in, S.lo + static_cast<int>(v)), n));
+      }
+    }
+    const int n_bias = !kBias || S.nothing ? 0 : P.bias_len;
+    const int32_t* ids = P.bias_ids + S.row * P.bias_ids_stride;
+    const float* values = P.bias_values + S.row * P.bias_values_stride;
+    for (int base = tid & ~31; base < n_bias; base += kLogitsThreads) {      // (a warp together)
+      const int i = base + (tid & 31), id = i < n_bias ? ids[i] : -1;
+      const uint32_t v = static_cast<uint32_t>(id) - static_cast<uint32_t>(S.lo);
+      const bool mine = i < n_bias && v < width && S.keeps(id);
+      const uint32_t n = mine ? table.counts(v) : 0u;
+      const bool alone = (n & kBiasMask) == kBiasOne;
+      float z = mine ? penalised(logit_at<F32>(S.in, id), n) : 0.0f;
+      if (mine && alone) set_logit<F32>(S.out, id, __fadd_rn(z, values[i]));
+      // tokens listed more than once: the first entry adds all values in list order, the warp looks for them
+      for (uint32_t others = __ballot_sync(kFull, mine && !alone); others; others &= others - 1u) {
+        const int lane = __ffs(static_cast<int>(others)) - 1, what = __shfl_sync(kFull, id, lane);
+        float sum = __shfl_sync(kFull, z, lane);
+        int first = -1;
+        for (int e0 = 0; e0 < n_bias; e0 += 32) {
+          const int e = e0 + (tid & 31);
+          const bool same = e < n_bias && ids[e] == what;
+          const float value = same ? values[e] : 0.0f;
+          for (uint32_t m = __ballot_sync(kFull, same); m; m &= m - 1u) {
+            const int at = __ffs(static_cast<int>(m)) - 1;
+            if (first < 0) first = e0 + at;
+            sum = __fadd_rn(sum, __shfl_sync(kFull, value, at));
+          }
+        }
+        if ((tid & 31) == lane && first == i) set_logit<F32>(S.out, id, sum);
+      }
+    }
   }
 }
 

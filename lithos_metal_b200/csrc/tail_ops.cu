@@ -272,8 +272,8 @@ int lm_process_logits(const lm_logits_args* a) {
   rc = ensure_dynamic_smem(static_cast<KernelSlot>(kSlotLogits + (f32 ? 2 : 0) + (bias ? 1 : 0)), reinterpret_cast<const void*>(kernel), smem);
   if (rc != LM_OK) return rc;
   const long long items = static_cast<long long>(P.rows) * P.slices;
-  const dim3 grid(static_cast<unsigned>(items < 0x7FFFFFFF ? items : 0x7FFFFFFF));
-  return launch_beside(kernel, grid, kLogitsThreads, smem, 1, st, P);
+  if (items > 0x7FFFFFFF) return LM_E_UNSUPPORTED;
+  return launch_beside(kernel, dim3(static_cast<unsigned>(items)), kLogitsThreads, smem, 1, st, P);
 }
 
 }  // extern "C"
