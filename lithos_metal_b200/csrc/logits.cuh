@@ -15,6 +15,7 @@ namespace lm {
 constexpr int kLogitsThreads = 512;
 constexpr int kLogitsPerSM = 3;              // blocks
 constexpr int kLogitsMinSlice = 1024;
+constexpr int kLogitsSliceBytes = 160 * 1024;
 constexpr int kLogitsMaxNamed = 12288;       // tokens in a hash table at most (16384 entries, 128 KB); longer lists: slices of
 constexpr int kLogitsMaxDirect = 24576;      // at most so many tokens (96 KB)
 constexpr int kLogitsMaxSlice = 524288;      // and never wider than this (64 KB of bits)
@@ -298,10 +299,10 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ma
   constexpr int kSize = F32 ? 4 : 2, kAhead = kMaskAhead<F32>;
   const int tid = threadIdx.x;
   after_predecessor();
-  const long long items = static_cast<long long>(P.rows) * P.slices;
+  const uint32_t items = static_cast<uint32_t>(P.rows) * static_cast<uint32_t>(P.slices);
   struct Part { int row, lo, hi, head, chunks; uint32_t keep; bool nothing; const uint8_t* mask; } now, next;
-  auto part = [&](long long item, Part& a) {
-    a.row = static_cast<int>(item / P.slices); a.lo = static_cast<int>(item % P.slices) * P.slice; a.hi = min(a.lo + P.slice, P.vocab);
+  auto part = [&](uint32_t item, Part& a) {
+    a.row = static_cast<int>(item / static_cast<uint32_t>(P.slices)); a.lo = (static_cast<int>(item) - a.row * P.slices) * P.slice; a.hi = min(a.lo + P.slice, P.vocab);
     const int which = P.mask ? (P.mask_rows ? P.mask_rows[a.row] : a.row) : -1;
     a.nothing = which >= P.mask_count && which >= 0;                        // the row's mask does not exist: everything is masked
     a.mask = which >= 0 && !a.nothing ? reinterpret_cast<const uint8_t*>(P.mask + which * P.mask_stride) : nullptr;
@@ -324,7 +325,7 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ma
     }
   };
   if (blockIdx.x < items) part(blockIdx.x, now);
-  for (long long item = blockIdx.x; item < items; item += gridDim.x, now = next) {
+  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x, now = next) {
     const unsigned char* in = static_cast<const unsigned char*>(P.in) + now.row * P.in_stride * kSize;
     unsigned char* out = static_cast<unsigned char*>(P.out) + now.row * P.out_stride * kSize;
     const int64_t at = static_cast<int64_t>(now.head + 8 * tid) * kSize;
