@@ -426,6 +426,7 @@ PyObject* py_lm_head(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* py_lm_head_nvfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 8) { PyErr_SetString(PyExc_TypeError, "lm_head_nvfp4: 8 arguments"); return nullptr; }
+  if (!abi.head_nvfp4 || !abi.head_nvfp4_workspace_bytes) return none();
   const at::Tensor *x = as_tensor(args[0]), *c = as_tensor(args[1]), *s = as_tensor(args[2]), *g = as_tensor(args[3]), *nw = args[4] == Py_None ? nullptr : as_tensor(args[4]);
   if (!x || !c || !s || !g || (args[4] != Py_None && !nw)) return none();
   const at::Device dev = c->device();
@@ -464,6 +465,7 @@ PyObject* py_lm_head_nvfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* py_quantize_nvfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 2) { PyErr_SetString(PyExc_TypeError, "quantize_nvfp4: 2 arguments"); return nullptr; }
+  if (!abi.quantize_nvfp4) return none();
   const at::Tensor *x = as_tensor(args[0]), *g = args[1] == Py_None ? nullptr : as_tensor(args[1]);
   if (!x || (args[1] != Py_None && !g) || !plain_rows(*x) || x->numel() == 0 || x->size(1) % 16 != 0 || (x->size(0) > 1 && x->stride(0) < x->size(1))) return none();
   const at::Device dev = x->device();
@@ -493,6 +495,7 @@ PyObject* py_quantize_nvfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* py_dequantize_nvfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 4) { PyErr_SetString(PyExc_TypeError, "dequantize_nvfp4: 4 arguments"); return nullptr; }
+  if (!abi.dequantize_nvfp4) return none();
   const at::Tensor *c = as_tensor(args[0]), *s = as_tensor(args[1]), *g = as_tensor(args[2]);
   if (!c || !s || !g) return none();
   const at::Device dev = c->device();
@@ -520,6 +523,7 @@ PyObject* py_dequantize_nvfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* py_process_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 12) { PyErr_SetString(PyExc_TypeError, "process_logits: 12 arguments"); return nullptr; }
+  if (!abi.process_logits) return none();
   const at::Tensor* x = as_tensor(args[0]);
   if (!x || !plain_rows(*x) || (x->size(0) > 1 && x->stride(0) < x->size(1))) return none();
   const at::Device dev = x->device();
@@ -587,15 +591,17 @@ PyObject* py_init(PyObject*, PyObject* args) {
   abi.verify = reinterpret_cast<decltype(abi.verify)>(get("lm_verify"));
   abi.draft_q = reinterpret_cast<decltype(abi.draft_q)>(get("lm_draft_q"));
   abi.head = reinterpret_cast<decltype(abi.head)>(get("lm_head"));
-  abi.head_nvfp4 = reinterpret_cast<decltype(abi.head_nvfp4)>(get("lm_head_nvfp4"));
-  abi.head_nvfp4_workspace_bytes = reinterpret_cast<decltype(abi.head_nvfp4_workspace_bytes)>(get("lm_head_nvfp4_workspace_bytes"));
-  abi.process_logits = reinterpret_cast<decltype(abi.process_logits)>(get("lm_process_logits"));
-  abi.quantize_nvfp4 = reinterpret_cast<decltype(abi.quantize_nvfp4)>(get("lm_quantize_nvfp4"));
-  abi.dequantize_nvfp4 = reinterpret_cast<decltype(abi.dequantize_nvfp4)>(get("lm_dequantize_nvfp4"));
   abi.workspace_bytes = reinterpret_cast<decltype(abi.workspace_bytes)>(get("lm_workspace_bytes"));
   abi.verify_workspace_bytes = reinterpret_cast<decltype(abi.verify_workspace_bytes)>(get("lm_verify_workspace_bytes"));
+  // (these may be left out: their calls then go by the addresses of an earlier init, or through ctypes)
+  auto also = [&](auto& entry, const char* name) { if (void* p = get(name)) entry = reinterpret_cast<std::remove_reference_t<decltype(entry)>>(p); };
+  also(abi.head_nvfp4, "lm_head_nvfp4");
+  also(abi.head_nvfp4_workspace_bytes, "lm_head_nvfp4_workspace_bytes");
+  also(abi.process_logits, "lm_process_logits");
+  also(abi.quantize_nvfp4, "lm_quantize_nvfp4");
+  also(abi.dequantize_nvfp4, "lm_dequantize_nvfp4");
   if (PyErr_Occurred()) return nullptr;
-  if (!abi.sample || !abi.argmax || !abi.argmax_i64 || !abi.verify || !abi.draft_q || !abi.head || !abi.head_nvfp4 || !abi.head_nvfp4_workspace_bytes || !abi.process_logits || !abi.quantize_nvfp4 || !abi.dequantize_nvfp4 || !abi.workspace_bytes || !abi.verify_workspace_bytes) {
+  if (!abi.sample || !abi.argmax || !abi.argmax_i64 || !abi.verify || !abi.draft_q || !abi.head || !abi.workspace_bytes || !abi.verify_workspace_bytes) {
     PyErr_SetString(PyExc_ValueError, "init: an address is missing");
     return nullptr;
   }
