@@ -162,10 +162,17 @@ static int head_nvfp4_batch(const lm_head_nvfp4_args* a, const Rows4Dev& R, int 
   return LM_OK;
 }
 
-int lm_head_nvfp4(const lm_head_nvfp4_args* a) {
-  if (!a || a->struct_size != sizeof(lm_head_nvfp4_args)) return LM_E_INVALID;
+int lm_head_nvfp4(const lm_head_nvfp4_args* given) {
+  if (!given || given->struct_size != sizeof(lm_head_nvfp4_args)) return LM_E_INVALID;
+  lm_head_nvfp4_args one = *given;
+  const lm_head_nvfp4_args* const a = &one;
   if (a->rows < 0 || a->vocab < 0 || a->hidden_dim < 1) return LM_E_INVALID;
   if (a->rows == 0 || a->vocab == 0) return LM_OK;
+  // what lies between rows is of no account where there is one
+  if (a->rows == 1 && a->hidden_stride >= a->hidden_dim && a->logits_stride >= a->vocab) { one.hidden_stride = a->hidden_dim; one.logits_stride = a->vocab; }
+  if (a->vocab == 1 && a->codes_stride >= a->hidden_dim / 2 && a->scales_stride >= a->hidden_dim / kFp4Block) {
+    one.codes_stride = (a->hidden_dim / 2 + 15) / 16 * 16; one.scales_stride = (a->hidden_dim / kFp4Block + 15) / 16 * 16;
+  }
   if (!a->hidden || !a->logits || a->hidden_stride < a->hidden_dim || a->logits_stride < a->vocab) return LM_E_INVALID;
   int rc = fp4_matrix_ok(a->vocab, a->hidden_dim, a->codes, a->codes_stride, a->scales, a->scales_stride, a->scale);
   if (rc != LM_OK) return rc;

@@ -43,7 +43,18 @@ class Nvfp4Weight:
         scales = scales.view(torch.uint8)
         if scales.numel() and (scales.data_ptr() % 16 or (scales.shape[0] > 1 and scales.stride(0) % 16)):
             scales = _padded_scales(*scales.shape, scales.device).copy_(scales)
-        self.codes, self.scales, self.scale = codes, scales, scale
+        self._hold(codes, scales, scale)
+
+    def _hold(self, *tensors: torch.Tensor) -> "Nvfp4Weight":
+        for name, t in zip(self.__slots__, tensors):
+            object.__setattr__(self, name, t)
+        return self
+
+    def __setattr__(self, name: str, value: object) -> None:                 # (they were checked together; what they hold may change)
+        raise AttributeError("Nvfp4Weight: its tensors stay the same; make another weight")
+
+    def __reduce__(self):
+        return Nvfp4Weight, (self.codes, self.scales, self.scale)
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -87,9 +98,7 @@ def quantize_nvfp4(x: torch.Tensor, scale: Optional[torch.Tensor] = None) -> Nvf
         raise RuntimeError("lithos_metal_b200 runs on CUDA tensors only (there is no CPU path)")
     r = _lib.host().quantize_nvfp4(x, scale)
     if r is not None:
-        w = Nvfp4Weight.__new__(Nvfp4Weight)                                  # (tensors of the right kind: nothing to check)
-        w.codes, w.scales, w.scale = r
-        return w
+        return Nvfp4Weight.__new__(Nvfp4Weight)._hold(*r)                     # (tensors of the right kind: nothing to check)
     if x.dim() != 2 or x.shape[1] % BLOCK != 0:
         raise ValueError("quantize_nvfp4: x must be [rows, cols], cols a multiple of 16")
     dtype = _dtype_code(x)

@@ -77,7 +77,7 @@ def check(got, before, kw, dtype):
     assert np.array_equal(a[same], b[same])
     finite = touched & np.isfinite(want)
     limit = bound + HALF[dtype] * (np.abs(want) + bound) + 1e-44
-    assert (np.abs(have - want)[finite] <= limit[finite]).all()
+    assert (np.abs(have[finite] - want[finite]) <= limit[finite]).all()
     odd = touched & ~np.isfinite(want)
     assert np.array_equal(have[odd], want[odd], equal_nan=True)
 
@@ -207,6 +207,20 @@ def test_conversions_of_the_arguments():
     assert torch.equal(got.view(torch.int32), want.view(torch.int32))
     t = lm.process_logits(x.T.contiguous().T, **on_gpu(kw))
     assert torch.equal(t.view(torch.int32), want.view(torch.int32))
+
+
+def test_offsets_past_32_bits():
+    """4400 rows of 1,048,576 logits: the last rows are those of a call of their own, into another place and in place."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    rows, vocab = 4400, 1 << 20
+    x = torch.randn(64, vocab, device="cuda", generator=gen).bfloat16().repeat(70, 1)[:rows]
+    history = torch.randint(0, vocab, (rows, 100), device="cuda", generator=gen, dtype=torch.int32)
+    mask = torch.randint(-2 ** 31, 2 ** 31 - 1, (rows, vocab // 32), device="cuda", generator=gen, dtype=torch.int32)
+    for kw in (dict(history=history), dict(mask=mask), dict(history=history, mask=mask)):
+        want = lm.process_logits(x[-3:], repetition_penalty=1.3, **{k: v[-3:] for k, v in kw.items()}).view(torch.int16)
+        assert torch.equal(lm.process_logits(x, repetition_penalty=1.3, **kw)[-3:].view(torch.int16), want)
+        place = x.clone()
+        assert torch.equal(lm.process_logits(place, repetition_penalty=1.3, out=place, **kw)[-3:].view(torch.int16), want)
 
 
 def test_refusals():

@@ -1,6 +1,9 @@
 """The microscaled 4-bit weight and the projection with it on the GPU, against the binary64 restatement (oracle/nvfp4.py). Codes and block scales are equal, bit for
 bit: they are defined as roundings of real quotients. A logit is the BF16 rounding (half a step: 2^-8 of the value) of a sum whose FP32 accumulation may be off by
 2^-23 of the magnitudes' sum per addition."""
+import copy
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -85,6 +88,17 @@ def test_every_border_and_its_neighbours(g):
     _, codes, scales, _ = quantized(torch.from_numpy(x).cuda(), torch.tensor([g], device="cuda"))
     want_codes, want_scales = o.quantize(x, g)
     assert np.array_equal(scales, want_scales) and np.array_equal(codes, want_codes)
+
+
+@pytest.mark.parametrize("g", [0.0, -0.0, -1.0, float("inf"), float("nan"), 1e-40, 1e-45, 3e38])
+def test_a_scale_of_any_kind(g):
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((8, 64)).astype(np.float32)
+    x[0, 0], x[1, :16], x[2, 3], x[3, 20] = 0.0, 0.0, np.inf, np.nan
+    _, codes, scales, _ = quantized(torch.from_numpy(x).cuda(), torch.tensor([g], device="cuda"))
+    with np.errstate(all="ignore"):
+        want_codes, want_scales = o.quantize(x, np.float32(g))
+    assert np.array_equal(codes, want_codes) and np.array_equal(scales, want_scales)
 
 
 def test_zeros_infinities_and_nan():
@@ -260,6 +274,65 @@ def test_strides_and_a_given_place(rows):
     assert got.data_ptr() == out[1:, 5:].data_ptr() and torch.equal(got.view(torch.int16), whole.view(torch.int16))
     assert (out[0] == 7).all() and (out[-1] == 7).all() and (out[:, :5] == 7).all() and (out[:, 338:] == 7).all()
     assert lm.lm_head(x[:0], w).shape == (0, 333) and lm.lm_head(x, w[:0]).shape == (rows, 0)
+
+
+@pytest.mark.parametrize("rows", [1, 16, 17, 70])
+@pytest.mark.parametrize("hidden", [64, 320])
+def test_one_row_of_the_weight(rows, hidden):
+    """Its strides are of no account, aligned or not."""
+    rng = np.random.default_rng(hidden + rows)
+    codes, scales, g = random_weight(rng, 3, hidden)
+    x = bf16(oracle.f32_to_bf16(rng.standard_normal((rows, hidden)).astype(np.float32)))
+    for w in (as_weight(codes[1:2].copy(), scales[1:2].copy(), g), as_weight(codes, scales, g)[1:2]):
+        got = lm.lm_head(x, w)
+        assert got.shape == (rows, 1)
+        check_head(got, x.float().cpu().numpy(), codes[1:2], scales[1:2], g)
+
+
+def test_a_weight_keeps_its_tensors():
+    w = lm.quantize_nvfp4(torch.ones(20, 64, device="cuda"))
+    with pytest.raises(AttributeError):
+        w.codes = w.codes[:3]
+    again = copy.deepcopy(w)
+    assert again.codes.data_ptr() != w.codes.data_ptr() and torch.equal(again.dequantize(), w.dequantize())
+    again.codes.zero_()
+    assert (again.dequantize() == 0).all() and (w.dequantize() != 0).all()
+
+
+def test_two_threads_at_once():
+    rng = np.random.default_rng(8)
+    codes, scales, g = random_weight(rng, 30000, 512)
+    w = as_weight(codes, scales, g)
+    xs = [bf16(oracle.f32_to_bf16(rng.standard_normal((n, 512)).astype(np.float32))) for n in (5, 40, 200)]
+    want = [lm.lm_head(x, w).view(torch.int16) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                if not torch.equal(lm.lm_head(xs[i], w).view(torch.int16), want[i]):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1, 2, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_offsets_past_32_bits():
+    """A weight of 1,048,000 x 8192 (2^32 codes are 2 GB, logits of 300 rows 2^28 and more): its last rows as a weight of their own give the same bits."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(1024, 8192, device="cuda", generator=gen).bfloat16().repeat(1024, 1)[:1_048_000]
+    w = lm.quantize_nvfp4(x)
+    last = lm.quantize_nvfp4(x[-3000:], scale=w.scale)
+    assert torch.equal(w.codes[-3000:], last.codes) and torch.equal(w.scales[-3000:], last.scales)
+    del x
+    for rows in (2, 40, 300):
+        h = torch.randn(rows, 8192, device="cuda", generator=gen).bfloat16()
+        assert torch.equal(lm.lm_head(h, w)[:, -3000:].contiguous().view(torch.int16), lm.lm_head(h, last).view(torch.int16))
 
 
 def test_refusals():
