@@ -12,7 +12,8 @@
 
 namespace lm {
 
-constexpr int kLogitsThreads = 512;
+// (Without biases more warps pay, 1024 rows with a history 121 us, with 384 threads 127; with them the compiler needs the registers: with 512 threads 147 us, spilling, with 384 127.)
+template <bool kBias> constexpr int kLogitsThreads = kBias ? 384 : 512;
 constexpr int kLogitsPerSM = 3;              // blocks
 constexpr int kLogitsMinSlice = 1024;
 constexpr int kLogitsSliceBytes = 160 * 1024;
@@ -46,15 +47,22 @@ template <bool F32> __device__ __forceinline__ void set_logit(void* row, int64_t
 }
 
 // Eight logits; those whose bit of `keep` is clear become -inf.
-__device__ __forceinline__ uint32_t two_kept(uint32_t w, uint32_t keep) {    // of two BF16: bytes of w or of two -inf
-  return __byte_perm(w, 0xFF80FF80u, 0x7654u - (keep & 1u) * 0x44u - (keep & 2u) * 0x2200u);
+__device__ __forceinline__ uint32_t two_signs(uint32_t bytes, uint32_t which) {   // two of four bytes' top bits, 16 times each (0x9988: of bytes 0 and 1)
+  uint32_t r;
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(bytes), "r"(which));
+  return r;
 }
+__device__ __forceinline__ uint32_t two_kept(uint32_t w, uint32_t keep) { return (w & keep) | (0xFF80FF80u & ~keep); }
 template <bool F32> struct Chunk;
 template <> struct Chunk<false> {
   uint4 q;
   __device__ __forceinline__ void load(const void* p) { q = *static_cast<const uint4*>(p); }
   __device__ __forceinline__ void store(void* p) const { *static_cast<uint4*>(p) = q; }
-  __device__ __forceinline__ void apply(uint32_t keep) { q.x = two_kept(q.x, keep); q.y = two_kept(q.y, keep >> 2); q.z = two_kept(q.z, keep >> 4); q.w = two_kept(q.w, keep >> 6); }
+  __device__ __forceinline__ void apply(uint32_t keep) {
+    const uint32_t lo = (keep & 15u) * 0x10204080u, hi = (keep >> 4) * 0x10204080u;    // a bit to the top of each byte
+    q.x = two_kept(q.x, two_signs(lo, 0x9988u)); q.y = two_kept(q.y, two_signs(lo, 0xBBAAu)); q.z = two_kept(q.z, two_signs(hi, 0x9988u)); q.w = two_kept(q.w, two_signs(hi, 0xBBAAu));
+  }
+  __device__ __forceinline__ void store_once(void* p) const { __stcs(static_cast<uint4*>(p), q); }
 };
 template <> struct Chunk<true> {
   uint32_t v[8];
@@ -63,11 +71,46 @@ template <> struct Chunk<true> {
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   }
   __device__ __forceinline__ void store(void* p) const { static_cast<uint4*>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]); static_cast<uint4*>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]); }
+  __device__ __forceinline__ void store_once(void* p) const { __stcs(static_cast<uint4*>(p), make_uint4(v[0], v[1], v[2], v[3])); __stcs(static_cast<uint4*>(p) + 1, make_uint4(v[4], v[5], v[6], v[7])); }
   __device__ __forceinline__ void apply(uint32_t keep) {
 #pragma unroll
     for (int e = 0; e < 8; e++) if (!((keep >> e) & 1u)) v[e] = 0xFF800000u;
   }
 };
+
+// A lane's kAhead chunks of eight logits, kStride chunks apart (a block's threads): their bits of a mask, 8 for each. Where these begin at words, a lane loads the word of four lanes' chunks and the
+// lanes exchange them (mask_ahead, and mask_bits when they are wanted), elsewhere every lane loads its own bytes. (With bytes everywhere 256 masked rows of 151,936 took 35 us, and 18.6 in place
+// where nothing had to be written.)
+template <int kAhead, int kStride> __device__ __forceinline__ uint32_t mask_ahead(const uint8_t* mask, int first, int chunk, int chunks, int lane) {   // first: chunk 0's token; chunk: the lane's first
+  const int shift = first & 7;
+  uint32_t bits = 0u;
+  if ((first & 31) == 0) {
+    const int c = chunk - lane + (lane >> 3) * kStride + 4 * (lane & 7);
+    if (lane < 8 * kAhead && c < chunks) bits = __ldg(reinterpret_cast<const uint32_t*>(mask + (first >> 3) + c));
+  } else {
+    const uint8_t* p = mask + (first >> 3) + chunk;
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) {
+      if (chunk + kStride * u < chunks) {
+        uint32_t k = __ldg(p + kStride * u);
+        if (shift) k = ((k | static_cast<uint32_t>(__ldg(p + kStride * u + 1)) << 8) >> shift) & 0xFFu;     // (v + 7 is in the row, and so is its byte)
+        bits |= k << (8 * u);
+      }
+    }
+  }
+  return bits;
+}
+template <int kAhead> __device__ __forceinline__ uint32_t mask_bits(uint32_t ahead, int first, int lane) {    // (by the whole warp)
+  if ((first & 31) != 0) return ahead;
+  uint32_t bits = 0u;
+  const uint32_t byte = static_cast<uint32_t>(lane & 3) * 0x11u + 0x40u;      // that byte of both words
+#pragma unroll
+  for (int u = 0; u < kAhead; u += 2) {
+    const uint32_t a = __shfl_sync(kFull, ahead, 8 * u + (lane >> 2)), b = __shfl_sync(kFull, ahead, 8 * u + 8 + (lane >> 2));
+    bits |= (__byte_perm(a, b, byte) & 0xFFFFu) << (8 * u);
+  }
+  return bits;
+}
 
 // The tokens' counts in shared memory: a hash table with linear probing, or (log2 = 0) a word per token of the slice.
 constexpr uint32_t kNoToken = 0xFFFFFFFFu;
@@ -77,9 +120,9 @@ struct TokenTable {
   __device__ __forceinline__ int entries() const { return log2 ? 1 << log2 : slice; }   // (a multiple of 32)
   __device__ __forceinline__ uint32_t* end() const { return word + (log2 ? 2 << log2 : slice); }
   __device__ __forceinline__ uint32_t home(uint32_t v) const { return (v * 2654435769u) >> (32 - log2); }     // (2^32 over the golden ratio: neighbours lie apart)
-  __device__ __forceinline__ void clear() const {                            // and the bits behind it
+  template <int kThreads> __device__ __forceinline__ void clear() const {     // and the bits behind it
     const int hashed = log2 ? 2 << log2 : 0, all = (log2 ? 2 << log2 : slice) + slice / 32;
-    for (int i = 4 * threadIdx.x; i < all; i += 4 * kLogitsThreads) { const uint32_t k = i < hashed ? kNoToken : 0u; *reinterpret_cast<uint4*>(word + i) = make_uint4(k, 0u, k, 0u); }
+    for (int i = 4 * threadIdx.x; i < all; i += 4 * kThreads) { const uint32_t k = i < hashed ? kNoToken : 0u; *reinterpret_cast<uint4*>(word + i) = make_uint4(k, 0u, k, 0u); }
   }
   __device__ __forceinline__ uint32_t* insert(uint32_t v) const {            // the token's counts
     if (!log2) return word + v;
@@ -116,12 +159,12 @@ template <bool F32> struct Slice {
 };
 
 template <bool F32, bool kBias>
-static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_kernel(LogitsDev P) {
+static __global__ void __launch_bounds__(kLogitsThreads<kBias>, kLogitsPerSM) logits_kernel(LogitsDev P) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ float s_knob[3];                                               // rho, pi, phi
   const TokenTable table(smem_raw, P.table_log2, P.slice);
   uint32_t* named = table.end();                                            // [slice / 32 + 1] a bit for every token of the history
-  constexpr int kSize = F32 ? 4 : 2, kAhead = F32 ? 2 : 4;
+  constexpr int kSize = F32 ? 4 : 2, kAhead = F32 ? 2 : 4, kThreads = kLogitsThreads<kBias>;
   const int tid = threadIdx.x;
   after_predecessor();
   auto penalised = [&](float z, uint32_t n) {
@@ -139,24 +182,24 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
     if (n_hist || n_bias) {
       const uint32_t width = static_cast<uint32_t>(S.hi - S.lo);
       const int32_t *hist = P.history + S.row * P.hist_stride, *ids = P.bias_ids + S.row * P.bias_ids_stride;
-      table.clear();
+      table.clear<kThreads>();
       __syncthreads();
       const int prompt = P.prompts ? P.prompts[S.row] : 0;
-      for (int base = tid; base < n_hist; base += 4 * kLogitsThreads) {
+      for (int base = tid; base < n_hist; base += 4 * kThreads) {
         uint32_t t[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) t[e] = base + e * kLogitsThreads < n_hist ? static_cast<uint32_t>(hist[base + e * kLogitsThreads]) - static_cast<uint32_t>(S.lo) : kNoToken;
+        for (int e = 0; e < 4; e++) t[e] = base + e * kThreads < n_hist ? static_cast<uint32_t>(hist[base + e * kThreads]) - static_cast<uint32_t>(S.lo) : kNoToken;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const uint32_t v = t[e];
           if (v < width) {
             uint32_t* n = table.insert(v);
-            if (base + e * kLogitsThreads >= prompt) atomicAdd(n, 1u); else atomicOr(n, kSeen);
+            if (base + e * kThreads >= prompt) atomicAdd(n, 1u); else atomicOr(n, kSeen);
             atomicOr(&named[v >> 5], 1u << (v & 31));
           }
         }
       }
-      for (int i = tid; i < n_bias; i += kLogitsThreads) {
+      for (int i = tid; i < n_bias; i += kThreads) {
         const uint32_t v = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(S.lo);
         if (v < width) atomicAdd(table.insert(v), kBiasOne);
       }
@@ -177,7 +220,7 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
       chunks = (hi - head) / 8;
     }
     const int tail = head + 8 * chunks, singles = (head - lo) + (hi - tail);
-    for (int i = tid; i < singles; i += kLogitsThreads) {
+    for (int i = tid; i < singles; i += kThreads) {
       const int v = i < head - lo ? lo + i : tail + (i - (head - lo));
       if (!S.keeps(v)) { set_logit<F32>(out, v, -INFINITY); continue; }
       if (history && ((named[(v - lo) >> 5] >> ((v - lo) & 31)) & 1u)) {
@@ -188,44 +231,27 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
         if (F32) reinterpret_cast<uint32_t*>(out)[v] = reinterpret_cast<const uint32_t*>(in)[v]; else reinterpret_cast<uint16_t*>(out)[v] = reinterpret_cast<const uint16_t*>(in)[v];
       }
     }
-    const int shift = head & 7;                                            // of a chunk's bits in their byte (lo is a multiple of 32)
-    // the mask's bits of kAhead chunks, 8 for each
-    auto kept = [&](int c0) {
-      uint32_t keep = S.nothing ? 0u : 0xFFFFFFFFu;
-      if (mask) {
-        const uint8_t* p = mask + (head >> 3) + c0;
-        keep = 0u;
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-          if (c0 + u * kLogitsThreads < chunks) {
-            uint32_t k = __ldg(p + u * kLogitsThreads);
-            if (shift) k = ((k | static_cast<uint32_t>(__ldg(p + u * kLogitsThreads + 1)) << 8) >> shift) & 0xFFu;     // (v + 7 is in the row, and so is its byte)
-            keep |= k << (8 * u);
-          }
-        }
-      }
-      return keep;
-    };
-    uint32_t next = kept(tid);
-    for (int c0 = tid; c0 < chunks; c0 += kLogitsThreads * kAhead) {
+    const int shift = head & 7, lane = tid & 31;                            // (of a chunk's bits in their byte: lo is a multiple of 32)
+    uint32_t next = mask ? mask_ahead<kAhead, kThreads>(mask, head, tid, chunks, lane) : 0u;
+    for (int c0 = tid; c0 - lane < chunks; c0 += kThreads * kAhead) {   // (a warp together)
       const unsigned char* from = in + static_cast<int64_t>(head + 8 * c0) * kSize;
       unsigned char* to = out + static_cast<int64_t>(head + 8 * c0) * kSize;
       Chunk<F32> x[kAhead];
-      const uint32_t keep = next;
+      const uint32_t keep = mask ? mask_bits<kAhead>(next, head, lane) : S.nothing ? 0u : 0xFFFFFFFFu;
       uint32_t touched = 0u;                                               // 8 bits for each chunk
 #pragma unroll
       for (int u = 0; u < kAhead; u++) {
         const uint32_t k = (keep >> (8 * u)) & 0xFFu;
-        if (c0 + u * kLogitsThreads < chunks && k != 0u && !(P.in_place && k == 0xFFu)) x[u].load(from + u * (kLogitsThreads * 8 * kSize));
+        if (c0 + u * kThreads < chunks && k != 0u && !(P.in_place && k == 0xFFu)) x[u].load(from + u * (kThreads * 8 * kSize));
       }
-      next = kept(c0 + kLogitsThreads * kAhead);
+      if (mask) next = mask_ahead<kAhead, kThreads>(mask, head, c0 + kThreads * kAhead, chunks, lane);
       if (history) {
         const uint8_t* p = reinterpret_cast<const uint8_t*>(named) + ((head - lo) >> 3) + c0;
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
-          if (c0 + u * kLogitsThreads < chunks) {
-            uint32_t k = p[u * kLogitsThreads];
-            if (shift) k = ((k | static_cast<uint32_t>(p[u * kLogitsThreads + 1]) << 8) >> shift) & 0xFFu;
+          if (c0 + u * kThreads < chunks) {
+            uint32_t k = p[u * kThreads];
+            if (shift) k = ((k | static_cast<uint32_t>(p[u * kThreads + 1]) << 8) >> shift) & 0xFFu;
             touched |= k << (8 * u);
           }
         }
@@ -234,13 +260,13 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
 #pragma unroll
       for (int u = 0; u < kAhead; u++) {
         const uint32_t k = (keep >> (8 * u)) & 0xFFu;
-        if (c0 + u * kLogitsThreads < chunks && !(P.in_place && k == 0xFFu)) {
+        if (c0 + u * kThreads < chunks && !(P.in_place && k == 0xFFu)) {
           if (k != 0xFFu) x[u].apply(k);
-          x[u].store(to + u * (kLogitsThreads * 8 * kSize));
+          x[u].store(to + u * (kThreads * 8 * kSize));
         }
       }
       for (; touched; touched &= touched - 1u) {                           // (behind the stores of their chunks, by the same thread)
-        const int b = __ffs(static_cast<int>(touched)) - 1, u = b >> 3, v = (c0 + u * kLogitsThreads) * 8 + (b & 7);     // from head on
+        const int b = __ffs(static_cast<int>(touched)) - 1, u = b >> 3, v = (c0 + u * kThreads) * 8 + (b & 7);     // from head on
         const uint32_t n = table.counts(static_cast<uint32_t>(head - lo + v));
         if (kBias && (n & kBiasMask)) continue;                                       // (set below, from the logit itself)
         set_logit<F32>(out, head + v, penalised(logit_at<F32>(in, head + v), n));     // (read again, from the line just loaded)
@@ -253,7 +279,7 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
     __syncthreads();
     const uint32_t width = static_cast<uint32_t>(S.hi - S.lo);
     if (!S.stream) {
-      for (int i = tid; i < table.entries(); i += kLogitsThreads) {
+      for (int i = tid; i < table.entries(); i += kThreads) {
         const uint32_t v = table.log2 ? table.word[2 * i] : static_cast<uint32_t>(i), n = table.word[table.log2 ? 2 * i + 1 : i];
         if ((n & (kSeen | kOutMask)) && !(n & kBiasMask)) set_logit<F32>(S.out, S.lo + static_cast<int>(v), penalised(logit_at<F32>(S.in, S.lo + static_cast<int>(v)), n));
       }
@@ -261,7 +287,7 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
     const int n_bias = !kBias || S.nothing ? 0 : P.bias_len;
     const int32_t* ids = P.bias_ids + S.row * P.bias_ids_stride;
     const float* values = P.bias_values + S.row * P.bias_values_stride;
-    for (int base = tid & ~31; base < n_bias; base += kLogitsThreads) {      // (a warp together)
+    for (int base = tid & ~31; base < n_bias; base += kThreads) {      // (a warp together)
       const int i = base + (tid & 31), id = i < n_bias ? ids[i] : -1;
       const uint32_t v = static_cast<uint32_t>(id) - static_cast<uint32_t>(S.lo);
       const bool mine = i < n_bias && v < width && S.keeps(id);
@@ -290,67 +316,45 @@ static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_ke
   }
 }
 
-// Without lists: copied and masked (in place: masked). The blocks stay and take a slice of kMaskSlice logits after the other; the next slice's bits of the mask come while this one's logits do.
+// Without lists: copied and masked (in place: masked), a block to a slice of kMaskSlice logits, four chunks of eight to a thread.
+constexpr int kMaskThreads = 256, kMaskPerSM = 6;
 template <bool F32> constexpr int kMaskAhead = F32 ? 2 : 4;
-template <bool F32> constexpr int kMaskSlice = kLogitsThreads * 8 * kMaskAhead<F32>;
+template <bool F32> constexpr int kMaskSlice = kMaskThreads * 8 * kMaskAhead<F32>;
 
 template <bool F32>
-static __global__ void __launch_bounds__(kLogitsThreads, kLogitsPerSM) logits_mask_kernel(LogitsDev P) {
+static __global__ void __launch_bounds__(kMaskThreads, kMaskPerSM) logits_mask_kernel(LogitsDev P) {
   constexpr int kSize = F32 ? 4 : 2, kAhead = kMaskAhead<F32>;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
   after_predecessor();
-  const uint32_t items = static_cast<uint32_t>(P.rows) * static_cast<uint32_t>(P.slices);
-  struct Part { int row, lo, hi, head, chunks; uint32_t keep; bool nothing; const uint8_t* mask; } now, next;
-  auto part = [&](uint32_t item, Part& a) {
-    a.row = static_cast<int>(item / static_cast<uint32_t>(P.slices)); a.lo = (static_cast<int>(item) - a.row * P.slices) * P.slice; a.hi = min(a.lo + P.slice, P.vocab);
-    const int which = P.mask ? (P.mask_rows ? P.mask_rows[a.row] : a.row) : -1;
-    a.nothing = which >= P.mask_count && which >= 0;                        // the row's mask does not exist: everything is masked
-    a.mask = which >= 0 && !a.nothing ? reinterpret_cast<const uint8_t*>(P.mask + which * P.mask_stride) : nullptr;
-    const uintptr_t in = reinterpret_cast<uintptr_t>(P.in) + static_cast<uintptr_t>((a.row * P.in_stride + a.lo) * kSize), out = reinterpret_cast<uintptr_t>(P.out) + static_cast<uintptr_t>((a.row * P.out_stride + a.lo) * kSize);
-    a.head = a.lo; a.chunks = 0;                                            // [lo, head) singly, then chunks of 8 from 16-byte boundaries, then the rest singly
-    if (((in ^ out) & 15u) == 0) { a.head = min(a.lo + static_cast<int>(((16u - (out & 15u)) & 15u) / kSize), a.hi); a.chunks = (a.hi - a.head) / 8; }
-    a.keep = a.nothing ? 0u : 0xFFFFFFFFu;                                  // 8 bits for each of this thread's chunks
-    if (a.mask) {
-      const int shift = a.head & 7;
-      const uint8_t* p = a.mask + (a.head >> 3) + tid;
-      a.keep = 0u;
+  const Slice<F32> S(P);
+  int head = S.lo, chunks = 0;                                              // [lo, head) singly, then chunks of 8 from 16-byte boundaries, then the rest singly
+  if (((reinterpret_cast<uintptr_t>(S.in) ^ reinterpret_cast<uintptr_t>(S.out)) & 15u) == 0) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(S.out) + static_cast<uintptr_t>(S.lo) * kSize;
+    head = min(S.lo + static_cast<int>(((16u - (at & 15u)) & 15u) / kSize), S.hi);
+    chunks = (S.hi - head) / 8;
+  }
+  const uint32_t keep = S.mask ? mask_bits<kAhead>(mask_ahead<kAhead, kMaskThreads>(S.mask, head, tid, chunks, lane), head, lane) : S.nothing ? 0u : 0xFFFFFFFFu;    // 8 bits for each chunk
+  const int64_t at = static_cast<int64_t>(head + 8 * tid) * kSize;
+  Chunk<F32> x[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; u++) {
-        if (tid + u * kLogitsThreads < a.chunks) {
-          uint32_t k = __ldg(p + u * kLogitsThreads);
-          if (shift) k = ((k | static_cast<uint32_t>(__ldg(p + u * kLogitsThreads + 1)) << 8) >> shift) & 0xFFu;     // (v + 7 is in the row, and so is its byte)
-          a.keep |= k << (8 * u);
-        }
-      }
-    }
-  };
-  if (blockIdx.x < items) part(blockIdx.x, now);
-  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x, now = next) {
-    const unsigned char* in = static_cast<const unsigned char*>(P.in) + now.row * P.in_stride * kSize;
-    unsigned char* out = static_cast<unsigned char*>(P.out) + now.row * P.out_stride * kSize;
-    const int64_t at = static_cast<int64_t>(now.head + 8 * tid) * kSize;
-    Chunk<F32> x[kAhead];
+  for (int u = 0; u < kAhead; u++) {
+    const uint32_t k = (keep >> (8 * u)) & 0xFFu;
+    if (tid + u * kMaskThreads < chunks && k != 0u && !(P.in_place && k == 0xFFu)) x[u].load(S.in + at + u * (kMaskThreads * 8 * kSize));
+  }
 #pragma unroll
-    for (int u = 0; u < kAhead; u++) {
-      const uint32_t k = (now.keep >> (8 * u)) & 0xFFu;
-      if (tid + u * kLogitsThreads < now.chunks && k != 0u && !(P.in_place && k == 0xFFu)) x[u].load(in + at + u * (kLogitsThreads * 8 * kSize));
+  for (int u = 0; u < kAhead; u++) {
+    const uint32_t k = (keep >> (8 * u)) & 0xFFu;
+    if (tid + u * kMaskThreads < chunks && !(P.in_place && k == 0xFFu)) {
+      if (k != 0xFFu) x[u].apply(k);
+      x[u].store_once(S.out + at + u * (kMaskThreads * 8 * kSize));
     }
-    if (item + gridDim.x < items) part(item + gridDim.x, next);
-#pragma unroll
-    for (int u = 0; u < kAhead; u++) {
-      const uint32_t k = (now.keep >> (8 * u)) & 0xFFu;
-      if (tid + u * kLogitsThreads < now.chunks && !(P.in_place && k == 0xFFu)) {
-        if (k != 0xFFu) x[u].apply(k);
-        x[u].store(out + at + u * (kLogitsThreads * 8 * kSize));
-      }
-    }
-    const int tail = now.head + 8 * now.chunks, singles = (now.head - now.lo) + (now.hi - tail);
-    for (int i = tid; i < singles; i += kLogitsThreads) {
-      const int v = i < now.head - now.lo ? now.lo + i : tail + (i - (now.head - now.lo));
-      if (now.nothing || (now.mask && !((now.mask[v >> 3] >> (v & 7)) & 1u))) set_logit<F32>(out, v, -INFINITY);
-      else if (!P.in_place) {
-        if (F32) reinterpret_cast<uint32_t*>(out)[v] = reinterpret_cast<const uint32_t*>(in)[v]; else reinterpret_cast<uint16_t*>(out)[v] = reinterpret_cast<const uint16_t*>(in)[v];
-      }
+  }
+  const int tail = head + 8 * chunks, singles = (head - S.lo) + (S.hi - tail);
+  for (int i = tid; i < singles; i += kMaskThreads) {
+    const int v = i < head - S.lo ? S.lo + i : tail + (i - (head - S.lo));
+    if (!S.keeps(v)) set_logit<F32>(S.out, v, -INFINITY);
+    else if (!P.in_place) {
+      if (F32) reinterpret_cast<uint32_t*>(S.out)[v] = reinterpret_cast<const uint32_t*>(S.in)[v]; else reinterpret_cast<uint16_t*>(S.out)[v] = reinterpret_cast<const uint16_t*>(S.in)[v];
     }
   }
 }

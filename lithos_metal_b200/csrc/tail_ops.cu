@@ -243,14 +243,14 @@ int lm_process_logits(const lm_logits_args* a) {
   P.table_log2 = 0;
   if (!lists) {
     // slices of as many logits as a block takes at once, shorter ones where these would leave SMs idle
-    const long long per = f32 ? kMaskSlice<true> : kMaskSlice<false>, few = (static_cast<long long>(a->rows) * a->vocab + at_once - 1) / at_once;
+    const long long per = f32 ? kMaskSlice<true> : kMaskSlice<false>, few = (static_cast<long long>(a->rows) * a->vocab + kMaskPerSM * sms - 1) / (kMaskPerSM * sms);
     P.slice = static_cast<int>(((few < per ? few : per) + 31) / 32 * 32);
     if (P.slice < kLogitsMinSlice) P.slice = kLogitsMinSlice;
     P.slices = static_cast<int>((a->vocab + P.slice - 1) / P.slice);
     const long long items = static_cast<long long>(P.rows) * P.slices;
     if (items > 0x7FFFFFFF) return LM_E_UNSUPPORTED;
-    const dim3 grid(static_cast<unsigned>(items < at_once ? items : at_once));
-    return f32 ? launch_beside(logits_mask_kernel<true>, grid, kLogitsThreads, 0, 1, st, P) : launch_beside(logits_mask_kernel<false>, grid, kLogitsThreads, 0, 1, st, P);
+    const dim3 grid(static_cast<unsigned>(items));
+    return f32 ? launch_beside(logits_mask_kernel<true>, grid, kMaskThreads, 0, 1, st, P) : launch_beside(logits_mask_kernel<false>, grid, kMaskThreads, 0, 1, st, P);
   }
   // A block to a row, or to a slice of one. One block to an SM while the slices are short (the launch is then made ready beside its predecessor). Otherwise the number of slices for which the rounds
   // of kLogitsPerSM blocks to an SM are cheapest, a block's lists counted as the bytes that it could pass on meanwhile, and no slice so wide that what a round reads leaves L2 before the listed
@@ -282,7 +282,7 @@ int lm_process_logits(const lm_logits_args* a) {
   if (rc != LM_OK) return rc;
   const long long items = static_cast<long long>(P.rows) * P.slices;
   if (items > 0x7FFFFFFF) return LM_E_UNSUPPORTED;
-  return launch_beside(kernel, dim3(static_cast<unsigned>(items)), kLogitsThreads, smem, 1, st, P);
+  return launch_beside(kernel, dim3(static_cast<unsigned>(items)), bias ? kLogitsThreads<true> : kLogitsThreads<false>, smem, 1, st, P);
 }
 
 }  // extern "C"

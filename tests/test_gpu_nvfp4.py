@@ -323,7 +323,7 @@ def test_two_threads_at_once():
 
 
 def test_offsets_past_32_bits():
-    """A weight of 1,048,000 x 8192 (2^32 codes are 2 GB, logits of 300 rows 2^28 and more): its last rows as a weight of their own give the same bits."""
+    """A weight of 1,048,000 x 8192 (8.6e9 elements, 4.3 GB of codes): its last rows as a weight of their own give the same bits."""
     gen = torch.Generator(device="cuda").manual_seed(3)
     x = torch.randn(1024, 8192, device="cuda", generator=gen).bfloat16().repeat(1024, 1)[:1_048_000]
     w = lm.quantize_nvfp4(x)
