@@ -40,8 +40,8 @@ enum KernelSlot { kSlotFast, kSlotTopk, kSlotTopkOrdered, kSlotGeneric, kSlotVoc
                   kSlotVerifyGiven = kSlotVerify + 12,   // (four)
                   kSlotHeadNvfp4 = kSlotVerifyGiven + 4,     // (two)
                   kSlotHeadNvfp4Batch = kSlotHeadNvfp4 + 2,
-                  kSlotLogits,                      // (four)
-                  kSlotCount = kSlotLogits + 4 };
+                  kSlotLogits,                      // (eight)
+                  kSlotCount = kSlotLogits + 8 };
 
 inline int ensure_dynamic_smem(KernelSlot slot, const void* func, size_t bytes, bool large_clusters = false) {
   constexpr int kMaxDevices = 64;

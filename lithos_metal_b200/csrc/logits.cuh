@@ -142,7 +142,7 @@ struct TokenTable {
 
 // A block's slice of a row: what the parts of the kernel below each work out for themselves (kept over the streaming loop, the lists' values were spilled there: 1024 rows of 151,936 with a history
 // of 2048 tokens 150 us, with a bias that is never reached in the code behind the loop 180).
-template <bool F32> struct Slice {
+template <bool F32, bool kMask> struct Slice {
   int row, lo, hi; const unsigned char* in; unsigned char* out; const uint8_t* mask; bool nothing, stream;
   __device__ __forceinline__ explicit Slice(const LogitsDev& P) {
     uint32_t item = blockIdx.x;
@@ -150,7 +150,7 @@ template <bool F32> struct Slice {
     constexpr int kSize = F32 ? 4 : 2;
     row = static_cast<int>(item / static_cast<uint32_t>(P.slices)); lo = (static_cast<int>(item) - row * P.slices) * P.slice; hi = min(lo + P.slice, P.vocab);
     in = static_cast<const unsigned char*>(P.in) + row * P.in_stride * kSize; out = static_cast<unsigned char*>(P.out) + row * P.out_stride * kSize;
-    const int which = P.mask ? (P.mask_rows ? P.mask_rows[row] : row) : -1;
+    const int which = kMask && P.mask ? (P.mask_rows ? P.mask_rows[row] : row) : -1;
     nothing = which >= P.mask_count && which >= 0;                          // the row's mask does not exist: everything is masked
     mask = which >= 0 && !nothing ? reinterpret_cast<const uint8_t*>(P.mask + which * P.mask_stride) : nullptr;     // the row's bits, or none
     stream = !P.in_place || mask || nothing;
@@ -158,7 +158,7 @@ template <bool F32> struct Slice {
   __device__ __forceinline__ bool keeps(int v) const { return !nothing && (!mask || ((mask[v >> 3] >> (v & 7)) & 1u)); }
 };
 
-template <bool F32, bool kBias>
+template <bool F32, bool kBias, bool kMask>
 static __global__ void __launch_bounds__(kLogitsThreads<kBias>, kLogitsPerSM) logits_kernel(LogitsDev P) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ float s_knob[3];                                               // rho, pi, phi
@@ -175,7 +175,7 @@ static __global__ void __launch_bounds__(kLogitsThreads<kBias>, kLogitsPerSM) lo
   // ---- the lists
   bool history;
   {
-    const Slice<F32> S(P);
+    const Slice<F32, kMask> S(P);
     const int n_hist = P.history && !S.nothing ? min(P.lengths ? max(P.lengths[S.row], 0) : P.hist_len, P.hist_len) : 0, n_bias = !kBias || S.nothing ? 0 : P.bias_len;
     history = n_hist > 0;
     if (tid == 0) { s_knob[0] = P.rho ? P.rho[S.row] : P.rho_s; s_knob[1] = P.pi ? P.pi[S.row] : P.pi_s; s_knob[2] = P.phi ? P.phi[S.row] : P.phi_s; }
@@ -208,7 +208,7 @@ static __global__ void __launch_bounds__(kLogitsThreads<kBias>, kLogitsPerSM) lo
   }
   // ---- the slice: [lo, head) singly, then chunks of 8 from 16-byte boundaries, then the rest singly
   {
-    const Slice<F32> S(P);
+    const Slice<F32, kMask> S(P);
     const unsigned char* const in = S.in;
     unsigned char* const out = S.out;
     const uint8_t* const mask = S.mask;
@@ -274,7 +274,7 @@ static __global__ void __launch_bounds__(kLogitsThreads<kBias>, kLogitsPerSM) lo
     }
   }
   // ---- tokens of the history where nothing was streamed, and those with a bias
-  const Slice<F32> S(P);
+  const Slice<F32, kMask> S(P);
   if ((history && !S.stream) || (kBias && !S.nothing)) {
     __syncthreads();
     const uint32_t width = static_cast<uint32_t>(S.hi - S.lo);
@@ -326,7 +326,7 @@ static __global__ void __launch_bounds__(kMaskThreads, kMaskPerSM) logits_mask_k
   constexpr int kSize = F32 ? 4 : 2, kAhead = kMaskAhead<F32>;
   const int tid = threadIdx.x, lane = tid & 31;
   after_predecessor();
-  const Slice<F32> S(P);
+  const Slice<F32, true> S(P);
   int head = S.lo, chunks = 0;                                              // [lo, head) singly, then chunks of 8 from 16-byte boundaries, then the rest singly
   if (((reinterpret_cast<uintptr_t>(S.in) ^ reinterpret_cast<uintptr_t>(S.out)) & 15u) == 0) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(S.out) + static_cast<uintptr_t>(S.lo) * kSize;

@@ -277,8 +277,11 @@ int lm_process_logits(const lm_logits_args* a) {
   if (P.slice <= 2LL << P.table_log2) P.table_log2 = 0;                     // (no larger than the hash table: a word per token)
   const size_t smem = (P.table_log2 ? size_t{8} << P.table_log2 : static_cast<size_t>(P.slice) * 4) + static_cast<size_t>(P.slice) / 8 + 32;
   const bool bias = a->bias_len > 0;
-  void (*const kernel)(LogitsDev) = f32 ? (bias ? logits_kernel<true, true> : logits_kernel<true, false>) : (bias ? logits_kernel<false, true> : logits_kernel<false, false>);
-  rc = ensure_dynamic_smem(static_cast<KernelSlot>(kSlotLogits + (f32 ? 2 : 0) + (bias ? 1 : 0)), reinterpret_cast<const void*>(kernel), smem);
+  static void (*const kernels[8])(LogitsDev) = {logits_kernel<false, false, false>, logits_kernel<false, false, true>, logits_kernel<false, true, false>, logits_kernel<false, true, true>,
+                                                logits_kernel<true, false, false>, logits_kernel<true, false, true>, logits_kernel<true, true, false>, logits_kernel<true, true, true>};
+  const int which = (f32 ? 4 : 0) + (bias ? 2 : 0) + (P.mask ? 1 : 0);
+  void (*const kernel)(LogitsDev) = kernels[which];
+  rc = ensure_dynamic_smem(static_cast<KernelSlot>(kSlotLogits + which), reinterpret_cast<const void*>(kernel), smem);
   if (rc != LM_OK) return rc;
   const long long items = static_cast<long long>(P.rows) * P.slices;
   if (items > 0x7FFFFFFF) return LM_E_UNSUPPORTED;
