@@ -10,6 +10,8 @@
 // conversion instructions; where both give the same code it is the real quotient's, otherwise one fused multiply-add tells on which side of x the exact product border * s * g (31 bits)
 // lies. (That is not rare: with BF16 inputs and a scale formed from one of them, quotients fall on borders but for the scale's own rounding; comparing in binary64 then took 1.6 of 1.8 ms for
 // 151,936 x 4096.) Scales beyond 2^-100 .. 2^100: all by comparisons in binary64.
+// Bound by HBM, each a pass over the matrix, a thread a block of 16. 151,936 x 4096 in BF16: quantised under a given scale 289 us (1.6 GB, 5.5 TB/s), the scale found first 480 (L2 does not keep
+// the matrix between the passes: 2.8 GB, 5.9 TB/s), the values written as binary32 498 (2.8 GB, 5.7 TB/s).
 #pragma once
 #include "common.cuh"
 
