@@ -1,4 +1,4 @@
-// The vocabulary projection with a 4-bit weight for more rows than a decode step has (9 and up): logits = x * W^T on tcgen05, 128 vocabulary rows (M) by up to
+// The vocabulary projection with a 4-bit weight for more rows than a decode step has (17 and up; 9 where shared memory does not hold two eights of long rows): logits = x * W^T on tcgen05, 128 vocabulary rows (M) by up to
 // 256 rows of x (N) to an accumulator, FP32 in tensor memory.
 //
 // W arrives in shared memory as codes and goes to tensor memory as binary16: 16 warps turn codes into binary16, multiply by the block scales (exact, nvfp4.cuh) and store the A
@@ -10,7 +10,8 @@
 // A block owns a contiguous range of tiles and walks the hidden dimension once for as many of them as tensor memory holds accumulators beside four operands (256 columns: a tile of
 // 256 rows, 8 of 32): x then crosses from L2 once for all of these. The order of a logit's additions is that of the hidden dimension, whatever the tile or the block.
 // Measured, 151,936 x 4096: 17 rows 95 us, 64 109, 128 148, 256 240 (1330 TFLOP/s, 0.79 of the measured library rate; tensor pipe 0.74 busy at 1.6 GHz). Up to 64 rows the conversion of the weight
-// bounds it (a tile's step 256 conversions, multiplications and stores a lane quartet), with 256 the products and, between two tiles, the accumulators' way out, for which tensor memory has no second set.
+// bounds it (0.75 us a tile's step, whatever the rows; a third set of operands in tensor memory, in the place of half the accumulators: 32 rows 98 -> 105, 64 110 -> 130), with 256 what
+// comes in per SM: 128 KB of x from L2 a step, 42 bytes a clock, and, between two tiles, the accumulators' way out, for which tensor memory has no second set.
 // Every wait has a limit; a block whose wait ran out writes NaN.
 #pragma once
 #include "common.cuh"
