@@ -560,7 +560,8 @@ PyObject* py_process_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor* t = as_tensor(args[9]);
     if (!t || t->device() != dev || t->dim() != 2 || t->scalar_type() != at::kInt || t->stride(1) != 1 || (t->size(0) > 1 && t->stride(0) < t->size(1)) || t->size(1) < (vocab + 31) / 32) return none();
     if (!vec(args[10], &a.mask_rows) || (!a.mask_rows && t->size(0) != rows)) return none();
-    a.mask = static_cast<const uint32_t*>(t->const_data_ptr()); a.mask_stride = row_stride(*t); a.mask_count = t->size(0);
+    a.mask = t->size(0) ? static_cast<const uint32_t*>(t->const_data_ptr()) : reinterpret_cast<const uint32_t*>(a.mask_rows);      // (no masks: an address that is never read)
+    a.mask_stride = row_stride(*t); a.mask_count = t->size(0);
   } else if (args[10] != Py_None) return none();
   at::Tensor out;
   if (args[11] == Py_None) out = make({rows, vocab}, x->scalar_type(), dev);

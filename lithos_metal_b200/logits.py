@@ -91,8 +91,8 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
         mask_rows = _lengths(mask_rows, rows, dev, "mask_rows")
         if mask_rows is None and mask.shape[0] != rows:
             raise ValueError("process_logits: one mask per row, or mask_rows")
-        a.mask, a.mask_stride, a.mask_count = mask.data_ptr(), _row_stride(mask), mask.shape[0]
         a.mask_rows = mask_rows.data_ptr() if mask_rows is not None else None
+        a.mask, a.mask_stride, a.mask_count = mask.data_ptr() if mask.shape[0] else a.mask_rows, _row_stride(mask), mask.shape[0]     # (no masks: an address that is never read)
     elif mask_rows is not None:
         raise ValueError("process_logits: mask_rows without a mask")
     a.stream = torch.cuda.current_stream(dev).cuda_stream

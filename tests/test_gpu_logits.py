@@ -166,6 +166,20 @@ def test_infinities_and_nan_behind_a_mask():
     assert np.isnan(got[1, 0]) and got[1, 1] == np.inf and np.isneginf(got[1, 2]) and got[1, 3] == 0.5 and got[1, 5] == 2.0 and np.isneginf(got[1, 8])
 
 
+@pytest.mark.parametrize("history", [False, True])
+def test_rows_with_masks_that_do_not_exist(history):
+    """mask_rows beyond the masks hides the whole row, none at all included; a negative one leaves it alone."""
+    x = torch.randn(3, 500, device="cuda")
+    rows = torch.tensor([-1, 0, 7], dtype=torch.int32, device="cuda")
+    kw = dict(history=torch.zeros(3, 1, dtype=torch.int32, device="cuda")) if history else {}
+    for masks in (0, 1):
+        mask = torch.full((masks, 16), -1, dtype=torch.int32, device="cuda")
+        for m, r in ((mask, rows), (mask, rows.long())):                     # (as it is, and converted)
+            got = lm.process_logits(x, mask=m, mask_rows=r, **kw)
+            assert torch.equal(got[0], x[0]) and torch.isneginf(got[2]).all()
+            assert torch.equal(got[1], x[1]) if masks else torch.isneginf(got[1]).all()
+
+
 def test_plain_penalties_are_the_samplers():
     """With numbers, no prompt and no frequency, processing and then sampling FP32 logits is sampling with that history."""
     rng = np.random.default_rng(12)

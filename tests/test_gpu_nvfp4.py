@@ -322,6 +322,19 @@ def test_two_threads_at_once():
     assert not bad
 
 
+@pytest.mark.parametrize("rows,hidden,vocab", [(1, 12736, 300), (8, 12736, 300), (9, 12736, 300), (16, 6400, 300), (70, 12736, 300), (65536, 64, 40)])
+def test_the_largest_sizes(rows, hidden, vocab):
+    gen = torch.Generator(device="cuda").manual_seed(rows + hidden)
+    w = lm.quantize_nvfp4(torch.randn(vocab, hidden, device="cuda", generator=gen))
+    x = torch.randn(rows, hidden, device="cuda", generator=gen).bfloat16()
+    values = w.dequantize().double()
+    want = x.double() @ values.T
+    # sums of `hidden` products off by 2^-23 of the magnitudes' sum per addition, then one BF16 rounding
+    bound = hidden * 2.0 ** -23 * (x.double().abs() @ values.abs().T)
+    got = lm.lm_head(x, w).double()
+    assert ((got - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all()
+
+
 def test_offsets_past_32_bits():
     """A weight of 1,048,000 x 8192 (8.6e9 elements, 4.3 GB of codes): its last rows as a weight of their own give the same bits."""
     gen = torch.Generator(device="cuda").manual_seed(3)
@@ -360,6 +373,9 @@ def test_refusals():
         lm.Nvfp4Weight(w.codes.to(torch.int8), w.scales, w.scale)
     with pytest.raises(TypeError):
         w[3]
+    for rows, hidden in ((65537, 64), (2, 12800)):                           # beyond the largest sizes
+        with pytest.raises(lm._lib.LithosError):
+            lm.lm_head(torch.zeros(rows, hidden, dtype=torch.bfloat16, device="cuda"), lm.quantize_nvfp4(torch.ones(2, hidden, device="cuda")))
     with pytest.raises(lm._lib.LithosError):                                 # a hidden size that is no multiple of 64
         lm.lm_head(torch.zeros(2, 48, dtype=torch.bfloat16, device="cuda"), lm.quantize_nvfp4(torch.ones(20, 48, device="cuda")))
     with pytest.raises(lm._lib.LithosError):                                 # codes off their alignment
