@@ -565,7 +565,7 @@ LM_API int lm_dequantize_nvfp4(const lm_dequantize_nvfp4_args* args);
  * lm_head with a weight in that format: logits[r, v] = bf16(scale * sum_k x[r, k] * e2m1(codes[v, k]) * e4m3(scales[v, k / 16])), FP32 accumulation of the exact products, x as for
  * lm_head (BF16 rows, or the fused RMSNorm's BF16 output). 1 .. LM_HEAD_NVFP4_MAX_ROWS rows. hidden_dim a multiple of 64, at most 12,736; codes
  * and scales and their strides 16-byte aligned (scales of a hidden_dim that is no multiple of 256: rows padded to that). A logit does not depend on where its row of the weight lies (a shard of the weight gives the bits
- * of the whole). Stands in for the reference's NVFP4 matrix-vector kernel on the `lm_head` op (kernels/common/gemv_nvfp4_rows.metal, monolith/nn/lm_head.py:50-60).
+ * of the whole). Stands in for the reference's `lm_head` op on a weight packed in 4 bits (monolith/nn/lm_head.py:50-60).
  * workspace: lm_head_nvfp4_workspace_bytes(rows, hidden_dim) bytes, 256-byte aligned, any contents (0 bytes: NULL); calls that can overlap need one each.
  */
 #define LM_HEAD_NVFP4_MAX_ROWS 65536

@@ -1,7 +1,7 @@
 """Weights in the microscaled 4-bit format (NVFP4): 4-bit codes, an e4m3 scale for every 16 of a row's columns, one float32 scale for all.
 
 ``quantize_nvfp4`` makes one from a BF16 or FP32 matrix, ``Nvfp4Weight(codes, scales, scale)`` wraps the tensors of a checkpoint; ``lm_head`` takes
-it in the place of a BF16 weight (the reference's 4-bit packs: monolith/formats, kernels/common/gemv_nvfp4_rows.metal)."""
+it in the place of a BF16 weight (the reference's weight formats: monolith/formats)."""
 from __future__ import annotations
 
 import ctypes as C
