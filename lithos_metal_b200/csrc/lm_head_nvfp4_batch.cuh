@@ -345,13 +345,14 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
     const uint32_t row_bytes = static_cast<uint32_t>(P.logits_stride * 2);
     const float g = __ldg(P.scale);
     bool go = true, plain = true, bad = false;                              // plain: every g * 2^-shift is a normal binary32, with room for the sum
-    for (int r = lane; r < P.n; r += 32) {                                  // (each of these warps the same values)
+    for (int r = lane; r < P.n; r += 32) {                                  // (each of these warps looks at all rows and writes down a quarter of them)
       const double f = static_cast<double>(g) * __hiloint2double((1023 - P.shift[r]) << 20, 0);
       plain &= fabs(f) >= 0x1p-100 && fabs(f) <= 0x1p80;
-      factor[r] = static_cast<float>(f);
+      if ((r >> 5) % kB4DoneWarps == warp - kB4FirstDoneWarp) factor[r] = static_cast<float>(f);
       bad |= P.bad[r] != 0;
     }
     if (bad) words[2] = 1u;
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kB4DoneWarps) : "memory");    // factors are read by other lanes and warps than wrote them: a vote does not order them
     plain = __all_sync(kFull, plain);
     uint32_t phase = 0u;
     for (int i = 0; go && passes.get(i, pass); i++, phase ^= 1u) {

@@ -1,0 +1,47 @@
+"""The projection with a 4-bit weight on sums that are exact in FP32 whatever their order: small integers in x (times a power of two of each row's own), block scales of 1/2, 1 and 2. A product is a
+multiple of 1/4 (in the row's unit) and at most 48; a row of 12,736 sums to at most 2.4 million quarters, less than 2^24. So a logit has one rounding, to BF16, and is compared bit for bit, at vocabularies
+where a block has full passes of several tiles, tiles left over, or both."""
+import pytest
+import torch
+
+import lithos_metal_b200 as lm
+
+pytestmark = pytest.mark.gpu
+
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+G = 0.125
+
+
+def make_weight(gen, vocab, hidden, g=G):
+    """An Nvfp4Weight and its values over g in binary64 (by a table, without the framework)."""
+    codes = torch.randint(0, 256, (vocab, hidden // 2), dtype=torch.uint8, device="cuda", generator=gen)
+    powers = torch.randint(0, 3, (vocab, hidden // 16), device="cuda", generator=gen)
+    scales = (0x30 + 8 * powers).to(torch.uint8)                              # e4m3 of 1/2, 1, 2
+    table = torch.tensor(E2M1 + tuple(-v for v in E2M1), dtype=torch.float64, device="cuda")
+    values = torch.stack((table[(codes & 15).long()], table[(codes >> 4).long()]), dim=-1).view(vocab, hidden // 16, 16)
+    values = (values * torch.ldexp(torch.ones_like(powers, dtype=torch.float64), powers - 1).unsqueeze(-1)).view(vocab, hidden)
+    return lm.Nvfp4Weight(codes, scales, torch.full((1,), g, device="cuda")), values
+
+
+def make_x(gen, rows, hidden, low, high):
+    """Integers of -4 .. 4 times 2^low .. 2^high, another power for every row."""
+    e = torch.randint(low, high + 1, (rows, 1), device="cuda", generator=gen)
+    whole = torch.randint(-4, 5, (rows, hidden), device="cuda", generator=gen)
+    return torch.ldexp(whole.double(), e).bfloat16()
+
+
+def rounded(values):
+    """binary64 values of at most 24 bits, rounded once to BF16."""
+    assert torch.equal(values.float().double(), values)
+    return values.float().bfloat16()
+
+
+@pytest.mark.parametrize("rows", [17, 33, 70, 130, 256, 300])
+@pytest.mark.parametrize("hidden,vocab", [(192, 200_003), (512, 45_001), (1024, 300)])
+def test_every_row_by_its_own_factor(rows, hidden, vocab):
+    gen = torch.Generator(device="cuda").manual_seed(rows + hidden)
+    w, values = make_weight(gen, vocab, hidden)
+    x = make_x(gen, rows, hidden, -50, 50)
+    want = rounded((x.double() @ values.T) * G)
+    for _ in range(3):
+        assert torch.equal(lm.lm_head(x, w), want)
