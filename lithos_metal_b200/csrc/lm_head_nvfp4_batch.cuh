@@ -364,6 +364,7 @@ static __global__ void __launch_bounds__(kB4Threads, 1) lm_head_nvfp4_batch_kern
         const int v = tile * kB4Tile + part * 32 + lane, rows = min(P.rows, pass.r0 + pass.n);
         for (int r0 = pass.r0 + 32 * ((warp - kB4FirstDoneWarp) >> 2); r0 < pass.r0 + pass.n; r0 += 8 * kB4DoneWarps) {
           uint32_t a[32];
+          __syncwarp();                                                      // (a load by the whole warp, behind stores by some of its lanes)
           accumulators32(tmem + (static_cast<uint32_t>(part * 32) << 16) + static_cast<uint32_t>(sum * P.column_stride + r0 - pass.r0), a);
           uint16_t* out = P.logits + r0 * P.logits_stride + v;
           if (!plain) {

@@ -45,3 +45,14 @@ def test_every_row_by_its_own_factor(rows, hidden, vocab):
     want = rounded((x.double() @ values.T) * G)
     for _ in range(3):
         assert torch.equal(lm.lm_head(x, w), want)
+
+
+@pytest.mark.parametrize("rows", [1, 8, 16, 17, 40, 130, 256])
+@pytest.mark.parametrize("hidden,vocab", [(192, 200_003), (512, 45_001), (1024, 300)])
+def test_factors_beyond_the_ordinary_range(rows, hidden, vocab):
+    """Logits that are scaled in binary64 because g times a row's power of two leaves the range where binary32 is safe: in every pass and for every accumulator of one."""
+    gen = torch.Generator(device="cuda").manual_seed(rows + hidden + 1)
+    g = 2.0 ** -100
+    w, values = make_weight(gen, vocab, hidden, g)
+    x = make_x(gen, rows, hidden, 0, 40)
+    assert torch.equal(lm.lm_head(x, w), rounded((x.double() @ values.T) * g))
