@@ -260,7 +260,7 @@ template <int NT, int kAhead>
 static __global__ void __launch_bounds__(kH4Threads, 1) lm_head_nvfp4_kernel(Head4Dev P) {
   constexpr int kRows = kH4Rows * NT;
   extern __shared__ __align__(16) unsigned char smem_raw[];                 // [kRows][row_bytes]
-  __shared__ float s_part[4][3][32][4 * NT];                                // quarters of the tiles left over
+  __shared__ float4 s_part[4][3][32][NT];                                   // quarters of the tiles left over
   __shared__ float s_factor[kRows];                                         // g * 2^-shift
   __shared__ int s_shift[kRows];
   __shared__ uint64_t s_bar;
@@ -410,15 +410,15 @@ static __global__ void __launch_bounds__(kH4Threads, 1) lm_head_nvfp4_kernel(Hea
     }
     if (part > 0) {
 #pragma unroll
-      for (int n = 0; n < NT; n++) *reinterpret_cast<float4*>(&s_part[group][part - 1][lane][4 * n]) = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
+      for (int n = 0; n < NT; n++) s_part[group][part - 1][lane][n] = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
     }
     asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory");
     if (part == 0) {
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          c[n][e] = __fadd_rn(__fadd_rn(c[n][e], s_part[group][0][lane][4 * n + e]), __fadd_rn(s_part[group][1][lane][4 * n + e], s_part[group][2][lane][4 * n + e]));
+        const float4 p = s_part[group][0][lane][n], q = s_part[group][1][lane][n], r = s_part[group][2][lane][n];
+        c[n][0] = __fadd_rn(__fadd_rn(c[n][0], p.x), __fadd_rn(q.x, r.x)); c[n][1] = __fadd_rn(__fadd_rn(c[n][1], p.y), __fadd_rn(q.y, r.y));
+        c[n][2] = __fadd_rn(__fadd_rn(c[n][2], p.z), __fadd_rn(q.z, r.z)); c[n][3] = __fadd_rn(__fadd_rn(c[n][3], p.w), __fadd_rn(q.w, r.w));
       }
       store(tile, c);
     }

@@ -56,3 +56,14 @@ def test_factors_beyond_the_ordinary_range(rows, hidden, vocab):
     w, values = make_weight(gen, vocab, hidden, g)
     x = make_x(gen, rows, hidden, 0, 40)
     assert torch.equal(lm.lm_head(x, w), rounded((x.double() @ values.T) * g))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8, 9, 16, 17, 70, 256])
+@pytest.mark.parametrize("hidden", [64, 320, 4096, 6400, 12736])
+@pytest.mark.parametrize("vocab", [300, 40_003])
+def test_every_column_counts(rows, hidden, vocab):
+    """Quarters of a row in four warps (few rows, the tiles left over), last steps that are not whole, x in as many pieces as the longest row has."""
+    gen = torch.Generator(device="cuda").manual_seed(rows + hidden)
+    w, values = make_weight(gen, vocab, hidden)
+    x = make_x(gen, rows, hidden, -6, 6)
+    assert torch.equal(lm.lm_head(x, w), rounded((x.double() @ values.T) * G))
