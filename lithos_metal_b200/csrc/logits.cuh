@@ -298,22 +298,23 @@ static __global__ void __launch_bounds__(kLogitsThreads<kBias>, kLogitsPerSM) lo
       const bool alone = (n & kBiasMask) == kBiasOne;
       float z = mine ? penalised(logit_at<F32>(S.in, id), n) : 0.0f;
       if (mine && alone) set_logit<F32>(S.out, id, __fadd_rn(z, values[i]));
-      // tokens listed more than once: the first entry adds all values in list order, the warp looks for them
-      for (uint32_t others = __ballot_sync(kFull, mine && !alone); others; others &= others - 1u) {
+      // tokens listed more than once: the first entry adds all values in list order, the warp looks for them; any other entry's walk ends where it meets the first, and a warp's entries of one token
+      // take one walk. (Equal entries then cost their additions, one behind the other; many tokens listed twice a walk over the list each.)
+      for (uint32_t others = __ballot_sync(kFull, mine && !alone); others;) {
         const int lane = __ffs(static_cast<int>(others)) - 1, what = __shfl_sync(kFull, id, lane);
         float sum = __shfl_sync(kFull, z, lane);
         int first = -1;
         for (int e0 = 0; e0 < n_bias; e0 += 32) {
           const int e = e0 + (tid & 31);
           const bool same = e < n_bias && ids[e] == what;
+          uint32_t m = __ballot_sync(kFull, same);
+          if (first < 0 && m) first = e0 + __ffs(static_cast<int>(m)) - 1;
+          if (first >= 0 && first != base + lane) break;
           const float value = same ? values[e] : 0.0f;
-          for (uint32_t m = __ballot_sync(kFull, same); m; m &= m - 1u) {
-            const int at = __ffs(static_cast<int>(m)) - 1;
-            if (first < 0) first = e0 + at;
-            sum = __fadd_rn(sum, __shfl_sync(kFull, value, at));
-          }
+          for (; m; m &= m - 1u) sum = __fadd_rn(sum, __shfl_sync(kFull, value, __ffs(static_cast<int>(m)) - 1));
         }
         if ((tid & 31) == lane && first == i) set_logit<F32>(S.out, id, sum);
+        others &= ~__ballot_sync(kFull, id == what);
       }
     }
   }
