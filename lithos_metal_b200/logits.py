@@ -12,13 +12,24 @@ from . import _lib
 from .sampler import Knob, _check_logits, _dtype_code, _knob, _row_stride
 
 
+def _converted(t: torch.Tensor, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """`t` as `dtype` on the device. What int32 does not hold becomes its nearest end, which is as much outside every vocabulary, length and number of masks; a plain conversion would keep the low bits, and
+    2^32 + 5 would name token 5."""
+    if dtype == torch.int32 and t.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8, torch.bool):
+        wide = t.to(device=device, dtype=torch.int64)
+        if t.dtype == torch.uint64:                                           # (2^63 and more: negative by now)
+            wide = wide.masked_fill(wide < 0, 2 ** 31 - 1)
+        t = wide.clamp(-2 ** 31, 2 ** 31 - 1)
+    return t.to(device=device, dtype=dtype)
+
+
 def _rows_of(t: torch.Tensor, rows: int, dtype: torch.dtype, device: torch.device, name: str) -> torch.Tensor:
     """[n] (one list for every row) or [rows, n], as a tensor of `dtype` with unit stride along a row (a row stride of 0 is fine)."""
     if t.dim() == 1:
         t = t.unsqueeze(0).expand(rows, t.shape[0])
     if t.dim() != 2 or t.shape[0] != rows:
         raise ValueError(f"{name} must be [rows, n] or [n]")
-    t = t.to(device=device, dtype=dtype)
+    t = _converted(t, dtype, device)
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
@@ -27,7 +38,7 @@ def _lengths(t: Optional[torch.Tensor], rows: int, device: torch.device, name: s
         return None
     if t.numel() != rows:
         raise ValueError(f"{name}: expected {rows} per-row values, got {t.numel()}")
-    return t.to(device=device, dtype=torch.int32).contiguous()
+    return _converted(t, torch.int32, device).contiguous()
 
 
 def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None, history_len: Optional[torch.Tensor] = None, prompt_len: Optional[torch.Tensor] = None,
@@ -43,7 +54,8 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     word v >> 5 set = token v allowed, the others become -inf; row r has mask ``mask_rows[r]`` (negative: none; m or more: everything masked), or mask r.
 
     ``out``: the result's place, ``logits`` itself (in place: only what changes is written) or a tensor that shares nothing with it; a new tensor by default. A row
-    whose mask allows nothing is all -inf. Asynchronous on the current stream; nothing is copied to the host.
+    whose mask allows nothing is all -inf. Ids, lengths and ``mask_rows`` of another type or on another device are converted, those beyond int32 staying outside. Asynchronous on the current
+    stream; nothing is copied to the host.
     """
     r = _lib.host().process_logits(logits, history, history_len, prompt_len, repetition_penalty, presence_penalty, frequency_penalty, bias_ids, bias_values, mask, mask_rows, out)
     if r is not None:
