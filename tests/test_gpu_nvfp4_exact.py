@@ -67,3 +67,27 @@ def test_every_column_counts(rows, hidden, vocab):
     w, values = make_weight(gen, vocab, hidden)
     x = make_x(gen, rows, hidden, -6, 6)
     assert torch.equal(lm.lm_head(x, w), rounded((x.double() @ values.T) * G))
+
+
+@pytest.mark.parametrize("rows", [3, 8, 16, 17, 40, 130, 256, 300])
+@pytest.mark.parametrize("hidden,vocab", [(192, 200_003), (512, 45_001), (1024, 300)])
+def test_rows_that_are_done_over(rows, hidden, vocab):
+    """Rows of x whose elements lie too far apart for binary16, or are infinite or NaN, in the middle of rows that are not: in every pass, for every tile of one, behind full rounds. Their sums are
+    binary64's (here exact: 2^16 down to 2^-32 are 48 bits), rounded to binary32 and then to BF16."""
+    gen = torch.Generator(device="cuda").manual_seed(rows + hidden + 2)
+    w, values = make_weight(gen, vocab, hidden)
+    x = make_x(gen, rows, hidden, -6, 6)
+    far = [0, rows // 2] if rows > 3 else [0]
+    x[far] = 0.0
+    x[far, 5] = 2.0 ** 10
+    x[far, 140] = -(2.0 ** -30)
+    x[1, 17] = float("inf")
+    x[rows - 1, 33] = float("nan")
+    got = lm.lm_head(x, w)
+    exact = (x.double() @ values.T) * G
+    want = exact.float().bfloat16()
+    assert (values[:, 5] == 0).any() and (want[0][values[:, 5] == 0].abs() < 1e-6).all()          # (the small element is all that is left)
+    assert torch.isnan(got[rows - 1]).all()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(nan=1.0), want.nan_to_num(nan=1.0))
+    alone = [r for r in range(rows) if r not in (*far, 1, rows - 1)]
+    assert torch.equal(want[alone], rounded(exact[alone]))
