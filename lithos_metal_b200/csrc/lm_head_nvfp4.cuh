@@ -7,12 +7,13 @@
 // warp; measured alone, conversion, scale and mma together take in 57 weights a clock and SM, bit operations in the place of the conversion 34. (The operands go from registers to the
 // mma: on tcgen05 they pass through shared or tensor memory, which costs more than the products of so few rows: lm_head_nvfp4_batch.cuh.) A warp's loads run ahead in registers.
 //
-// x is BF16 and the mma wants binary16 on both sides. A row of x is multiplied by the power of two that brings its largest magnitude to 2^14 .. 2^15 (taken out
+// The conversion instructions know binary16 only (for BF16, which would hold e2m1 * e4m3 as well, every pair of weights would take another conversion), x is BF16, and the mma wants one type on both sides. A row of x is multiplied by the power of two that brings its largest magnitude to 2^14 .. 2^15 (taken out
 // again behind the sum); BF16 values down to 2^-31 of the largest are then exact in binary16, subnormals included. A row where some x is not (or is infinite or NaN) is
-// done over at the end, in FP64 on the CUDA cores, whose range holds every product. All this is nvfp4_rows_kernel's work, once per call; this kernel's blocks copy its result. (Every block
+// done over at the end, in FP64 on the CUDA cores, whose range holds every product: a row reads the whole weight again for itself, 0.65 ms for 151,936 x 4096, one row after the other (8 rows, 83 us: 731 with one
+// row done over, 5.2 ms with all; 256 rows, all of them NaN or with an element below 2^-31 of their largest: 126 ms). All this is nvfp4_rows_kernel's work, once per call; this kernel's blocks copy its result. (Every block
 // preparing x for itself took 13 us of a call of 8 rows of 4096.)
 //
-// Measured: 8 rows of 151,936 x 4096 72 us, 4.9 TB/s = 0.75 of the copy rate: issue slots (0.54 of the cycles; conversions, scales and mma wait for each other) and loads share the blame; 1 row 71;
+// Measured, calls back to back (with L2 full of lines that have to be written first, some 10 us more at 151,936 x 4096): 8 rows of 151,936 x 4096 72 us, 4.9 TB/s = 0.75 of the copy rate: issue slots (0.54 of the cycles; conversions, scales and mma wait for each other) and loads share the blame; 1 row 71;
 // 8 rows of 50,257 x 4096 32 us, 1 row of 32,768 x 2048 14, of 4,099 x 4096 9 (two launches, and memory's latency in each). Blocks that prepared one or two rows themselves, without the first launch:
 // 71.8, 13.7 and 8.4, for 100 bytes of spilled registers: not kept.
 //

@@ -9,9 +9,11 @@
 //
 // A block owns a contiguous range of tiles and walks the hidden dimension once for as many of them as tensor memory holds accumulators beside four operands (256 columns: a tile of
 // 256 rows, 8 of 32): x then crosses from L2 once for all of these. The order of a logit's additions is that of the hidden dimension, whatever the tile or the block.
-// Measured, 151,936 x 4096: 17 rows 95 us, 64 109, 128 148, 256 240 (1330 TFLOP/s, 0.79 of the measured library rate; tensor pipe 0.74 busy at 1.6 GHz). Up to 64 rows
-// a tile's step of 256 columns takes 0.75 us whatever the rows, which neither a third set of operands in tensor memory (32 rows 98 -> 105 us, 64 110 -> 130: half the accumulators) nor 24 converting
-// warps instead of 16 (98 -> 114) change: the products themselves, some 85 clocks for 128 x 16 of W however narrow x is. With 256 rows what comes in per SM bounds it, 128 KB of x from L2 a step, 42 bytes a
+// Measured, 151,936 x 4096, calls back to back: 17 rows 95 us, 64 109, 128 148, 256 240 (1330 TFLOP/s, 0.79 of the measured library rate; tensor pipe 0.74 busy at 1.6 GHz); beyond that a launch for every 256
+// rows, each of which converts the weight again: 512 rows 518, 1024 1036, 4096 4430. Up to 64 rows a tile's step of 256 columns takes 0.75 us whatever the rows, and no unit is full: with 32 rows (100,000 x 4096)
+// the tensor pipe is busy for 19 % of the clocks (some 15 of them to a product of 128 x 16 of W), issue slots 41 %, DRAM 3.2 TB/s. What is left is the turn of a pair: codes, conversion, store to tensor memory, products,
+// commit, and only then the next conversion. More of these under way in another split of the same room were slower: a third set of operands in tensor memory 32 rows 98 -> 105 us, 64 110 -> 130 (half the accumulators),
+// 24 converting warps instead of 16 98 -> 114. With 256 rows what comes in per SM bounds it, 128 KB of x from L2 a step, 42 bytes a
 // clock, and, between two tiles, the accumulators' way out, for which tensor memory has no second set.
 // Every wait has a limit; a block whose wait ran out writes NaN.
 #pragma once

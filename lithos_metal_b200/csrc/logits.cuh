@@ -9,7 +9,8 @@
 // (first) entry of the list. In place without a mask only the tokens that the lists name are touched.
 // Bound by HBM where there are many rows: 4096 rows of 151,936 with histories of 2048 395 us, 6.4 TB/s = 0.98 of the copy rate; 1024 rows with biases and masks as well 129 us (98 for the bytes); 256 41 (24.5);
 // 64 rows of 262,144 in place under masks 12.6 (a fill of as many bytes: 12.5). A few rows: launch, the lists and one trip to memory, 8 rows 6.6 us, 1 row 4.5. Blocks look through their lists before
-// they stream, and few rows are few rounds of blocks: that is what the middle sizes lose.
+// they stream, and few rows are few rounds of blocks: that is what the middle sizes lose. In place with a history of 2048 and without a mask 4096 rows take 330 us: lists and tables, and 2048 scattered lines a row.
+// Where logits and result lie differently against 16 bytes they pass singly: 4096 rows of 50,257 from rows of 50,304 with a history 849 us into a tensor of 50,257 columns, 242 into one of 50,304; with a mask alone 621 and 129.
 #pragma once
 #include "common.cuh"
 

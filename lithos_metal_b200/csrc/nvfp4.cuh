@@ -6,12 +6,12 @@
 //
 // Quantisation: s = e4m3(a / (6 g)) with a the block's largest magnitude, code = e2m1(x / (s g)); both quotients are the real ones, rounded once to
 // nearest, ties to even, and saturate (448, 6). So the codes are a property of the input and not of the arithmetic: any correct program finds the same.
-// The kernel forms quotients in binary32 with a reciprocal that is a little too small and one that is a little too large (by 2^-21; their error is below 2^-22) and rounds both with the
-// conversion instructions; where both give the same code it is the real quotient's, otherwise one fused multiply-add tells on which side of x the exact product border * s * g (31 bits)
+// The kernel forms quotients in binary32 with a reciprocal that is a little too small and one that is a little too large, by 2^-21 = 8 * 2^-24: the product s * g, the reciprocal (__fdividef: two units in the
+// last place), its shift and the product with x are off by (1 + 4 + 1 + 1) * 2^-24 at most, so the real quotient lies between. Both are rounded with the conversion instructions; where both give the same code it is the real quotient's, otherwise one fused multiply-add tells on which side of x the exact product border * s * g (31 bits)
 // lies. (That is not rare: with BF16 inputs and a scale formed from one of them, quotients fall on borders but for the scale's own rounding; comparing in binary64 then took 1.6 of 1.8 ms for
 // 151,936 x 4096.) Scales beyond 2^-100 .. 2^100: all by comparisons in binary64.
-// Bound by HBM, each a pass over the matrix, a thread a block of 16. 151,936 x 4096 in BF16: quantised under a given scale 289 us (1.6 GB, 5.5 TB/s), the scale found first 480 (L2 does not keep
-// the matrix between the passes: 2.8 GB, 5.9 TB/s), the values written as binary32 498 (2.8 GB, 5.7 TB/s).
+// Bound by HBM, each a pass over the matrix, a thread a block of 16. 151,936 x 4096 in BF16 (L2 cold): quantised under a given scale 277 to 289 us (1.6 GB, 5.5 to 5.8 TB/s), the scale found first 480 to 490 (L2
+// does not keep the matrix between the passes: 2.8 GB), the values written as binary32 500 (2.8 GB, 5.7 TB/s). In FP32 442 (2.8 GB, 6.4 TB/s) and 802 (5.3 GB, 6.6 TB/s).
 #pragma once
 #include "common.cuh"
 

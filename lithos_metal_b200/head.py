@@ -17,8 +17,8 @@ def lm_head(hidden: torch.Tensor, weight: Union[torch.Tensor, Nvfp4Weight], norm
             out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``bf16(x @ weightᵀ)`` with FP32 accumulation; ``x = hidden`` or, with ``norm_weight``, ``bf16(rms_norm(hidden) * (1 + norm_weight))``
     (``one_plus=False``: ``* norm_weight``), as monolith/nn/oracle.py:20-32 defines both. ``hidden`` [rows <= 8, H] and ``weight`` [V, H]
-    bfloat16 CUDA tensors with unit stride along H; returns [rows, V] bfloat16. With an ``Nvfp4Weight`` [V, H] any number of rows (to 65,536), the products
-    with the weight's values exact."""
+    bfloat16 CUDA tensors with unit stride along H; returns [rows, V] bfloat16. With an ``Nvfp4Weight`` [V, H] any number of rows (to 65,536), H a multiple of 64
+    up to 12,736, the products with the weight's values exact."""
     if isinstance(weight, Nvfp4Weight):
         return _lm_head_nvfp4(hidden, weight, norm_weight, eps, one_plus, out)
     r = _lib.host().lm_head(hidden, weight, norm_weight, eps, one_plus, out)

@@ -50,7 +50,7 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     ``history`` [rows, n] (or [n]: the same for every row) int32 token ids, of which the first ``history_len[r]`` count (default: all) and the first ``prompt_len[r]``
     are the prompt's (default: none). A token of the history: ``z / repetition_penalty`` if z > 0, else ``z * repetition_penalty``; one that occurs c > 0 times behind the
     prompt: ``- presence_penalty - frequency_penalty * c``. The penalties are numbers or per-row tensors. ``bias_ids`` int32 / ``bias_values`` float32 [rows, n] (or [n]):
-    added to the tokens' logits, one that is listed twice in list order; ids outside the vocabulary (-1) are padding. ``mask`` int32 [m, >= ceil(vocab / 32)]: bit v & 31 of
+    added to the tokens' logits, one that is listed twice in list order; ids outside the vocabulary (-1) are padding (so a vocabulary shard takes the ids less its first index). ``mask`` int32 [m, >= ceil(vocab / 32)]: bit v & 31 of
     word v >> 5 set = token v allowed, the others become -inf; row r has mask ``mask_rows[r]`` (negative: none; m or more: everything masked), or mask r.
 
     ``out``: the result's place, ``logits`` itself (in place: only what changes is written) or a tensor that shares nothing with it; a new tensor by default. A row

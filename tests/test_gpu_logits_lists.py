@@ -76,3 +76,22 @@ def test_repeated_entries_cost_no_square():
     once = fastest(rng.permutation(vocab)[:n].astype(np.int32), np.zeros(n, dtype=np.float32))
     for kind in ("equal", "padded", "twice"):
         assert fastest(*repeated(rng, kind, vocab, n)) < 100 * once
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_shards_of_a_vocabulary(dtype):
+    """Ids less a shard's first index, masks as views of whole words where it is a multiple of 32: the shards' results are the whole's columns."""
+    rng = np.random.default_rng(5)
+    rows, vocab = 5, 20_011
+    x = torch.from_numpy((rng.standard_normal((rows, vocab)) * 3).astype(np.float32)).cuda().to(dtype)
+    history = torch.from_numpy(rng.integers(-1, vocab + 3, (rows, 500)).astype(np.int32)).cuda()
+    history[:, 0] = -2 ** 31
+    ids = torch.from_numpy(rng.integers(-1, vocab, (rows, 60)).astype(np.int32)).cuda()
+    kw = dict(repetition_penalty=1.25, presence_penalty=0.5, frequency_penalty=0.25, bias_values=torch.from_numpy(rng.normal(0, 4, (rows, 60)).astype(np.float32)).cuda())
+    mask = torch.from_numpy(rng.integers(-2 ** 31, 2 ** 31, (rows, (vocab + 31) // 32)).astype(np.int32)).cuda()
+    bits = torch.int16 if dtype == torch.bfloat16 else torch.int32
+    for cuts, masks in (([0, 7, 5000, 12_345, vocab], None), ([0, 32, 4992, 16_000, vocab], mask)):
+        whole = lm.process_logits(x, history=history, bias_ids=ids, mask=masks, **kw)
+        for lo, hi in zip(cuts[:-1], cuts[1:]):
+            part = lm.process_logits(x[:, lo:hi], history=history - lo, bias_ids=ids - lo, mask=None if masks is None else masks[:, lo // 32:], **kw)
+            assert torch.equal(part.view(bits), whole[:, lo:hi].contiguous().view(bits))
