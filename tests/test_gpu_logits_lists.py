@@ -55,8 +55,8 @@ def test_values_are_added_once_in_list_order(kind, n, history, place):
 
 
 def test_repeated_entries_cost_no_square():
-    """The longest list of one token, or filled up with one, is some 8000 dependent additions, a few hundred microseconds; walks by every entry were a third of a second. Lists of other
-    kinds take some 20 us: a hundred times that is the limit."""
+    """The longest list of one token, or filled up with one, is some 8000 dependent additions, a few hundred microseconds; walks by every entry were a third of a second. Lists of
+    distinct tokens take 10 to 20 us: the limit is a thousand times that, a tenth of what the square cost."""
     rng = np.random.default_rng(0)
     n, vocab = 8191, 151_936
     x = torch.zeros(2, vocab, device="cuda", dtype=torch.bfloat16)
@@ -75,7 +75,7 @@ def test_repeated_entries_cost_no_square():
 
     once = fastest(rng.permutation(vocab)[:n].astype(np.int32), np.zeros(n, dtype=np.float32))
     for kind in ("equal", "padded", "twice"):
-        assert fastest(*repeated(rng, kind, vocab, n)) < 100 * once
+        assert fastest(*repeated(rng, kind, vocab, n)) < 1000 * once
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
